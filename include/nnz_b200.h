@@ -288,6 +288,118 @@ int nnz_attn_decode(const void* qkv, const float* q_norm, const float* k_norm, v
                     uint32_t n_q, uint32_t n_kv, uint32_t head_dim, float eps, float theta,
                     int rope_style, uint32_t splits, void* out, void* stream);
 
+/* ---- ragged serving over a paged KV cache ------------------------------ */
+/* Prompt chunks and single tokens of many sequences in one call, over K/V
+ * pages that the caller hands out.  No counterpart in the reference, whose
+ * cache is one contiguous slot of one sequence (transformer.metal:1601).
+ * Device pointers, asynchronous on `stream`; nothing is allocated and the
+ * current device must be the pointers' device. */
+
+/* A pool of K and V pages.  Element d of kv head h of the token in place t of
+ * page p is k[p page_stride + h head_stride + t token_stride + d]; V is laid
+ * out the same way from its own base pointer.  Strides in elements, every
+ * one a multiple of 8; k and v 16-byte aligned.  Pages stored head by head
+ * ([page][head][token][d]), token by token ([page][token][head][d]), and K
+ * and V in one allocation are all such strides. */
+typedef struct nnz_paged_kv {
+  void* k;
+  void* v;
+  int32_t dtype;                  /* NNZ_DT_F16 | NNZ_DT_BF16 */
+  uint32_t num_pages;
+  uint32_t page_size;             /* tokens per page, >= 1 */
+  uint32_t num_kv_heads;
+  uint32_t head_dim;              /* 64 or 128 */
+  int64_t page_stride, head_stride, token_stride;
+} nnz_paged_kv;
+
+/* cos and sin of position p times theta^(-2 i / head_dim), evaluated in
+ * double: table f32 [positions][head_dim / 2][2]. */
+int nnz_rope_table(float theta, uint32_t head_dim, uint32_t positions, float* table, void* stream);
+
+typedef struct nnz_norm_rope_args {
+  const void* qkv;                /* [tokens][qkv_stride], the pool's dtype: q heads | k heads | v heads */
+  int64_t qkv_stride;             /* elements, multiple of 8 */
+  uint32_t tokens;                /* 0: nothing to do */
+  uint32_t num_query_heads;
+  const float* q_norm;            /* [head_dim] RMSNorm weights of the query / key heads */
+  const float* k_norm;
+  float eps;
+  int32_t rope_style;             /* NNZ_ROPE_* */
+  const float* rope_table;        /* f32 [table_positions][head_dim / 2][2] (cos, sin) */
+  uint32_t table_positions;
+  const int32_t* positions;       /* [tokens] */
+  const int64_t* slots;           /* [tokens] page * page_size + place in the page; negative: not written */
+  void* q_out;                    /* [tokens][q_stride]; may be qkv itself */
+  int64_t q_stride;               /* elements, multiple of 8 */
+} nnz_norm_rope_args;
+
+/* RMSNorm of every query and key head, rotation by the token's position, and
+ * the new keys and values into their pages, in one pass (the decode kernel's
+ * prologue, transformer.metal:1500-1610, for any number of tokens).  Sums and
+ * products in f32, rounded once to the pool's dtype.  A position outside the
+ * table or a slot outside the pool raises NNZ_EDEVICE in nnz_stream_check;
+ * the token's q_out is then zero and its pages are left alone. */
+int nnz_qk_norm_rope_paged(const nnz_paged_kv* kv, const nnz_norm_rope_args* args, void* stream);
+
+typedef struct nnz_paged_attn_args {
+  const void* q;                  /* [tokens][q_stride], the pool's dtype; normed and rotated */
+  int64_t q_stride;               /* elements, multiple of 8 */
+  uint32_t tokens;                /* rows of q and out */
+  uint32_t num_query_heads;       /* multiple (<= 64x) of num_kv_heads */
+  uint32_t num_seqs;
+  uint32_t max_new;               /* most new tokens of one sequence (an upper bound) */
+  const int32_t* q_start;         /* [num_seqs + 1] sequence s's new tokens: rows [q_start[s], q_start[s + 1]) */
+  const int32_t* kv_len;          /* [num_seqs] its keys, the new tokens' included */
+  const int32_t* page_table;      /* [num_seqs][table_stride] pages in order; negative: absent (evicted) */
+  uint32_t table_stride;
+  float scale;                    /* 0: 1 / sqrt(head_dim) */
+  void* out;                      /* [tokens][out_stride] */
+  int64_t out_stride;             /* elements, multiple of 8 */
+  void* workspace;                /* nnz_paged_attn_workspace bytes, 256-byte aligned; one call at a time */
+  size_t workspace_bytes;
+} nnz_paged_attn_args;
+
+/* Bytes of workspace that any call with these heads and page pool needs. */
+size_t nnz_paged_attn_workspace(const nnz_paged_kv* kv, uint32_t num_query_heads);
+
+/* Causal attention of every sequence's new tokens over its pages: new token
+ * i of n attends to keys 0 .. kv_len - n + i that lie on present pages; a
+ * token that sees no key gets zeros.  Scores, softmax and sums in f32 (the
+ * probabilities enter the second product in the pool's dtype).  Rows of q
+ * outside every sequence are not read and their output is not written.  A
+ * page number >= num_pages, a kv_len beyond table_stride pages, more new
+ * tokens than max_new or a q_start outside [0, tokens] raises NNZ_EDEVICE in
+ * nnz_stream_check; such pages count as absent, keys past the table are not
+ * seen and new tokens past max_new are not computed. */
+int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* args, void* stream);
+
+typedef struct nnz_logprobs_args {
+  const void* logits;             /* [rows][stride] */
+  int32_t dtype;                  /* NNZ_DT_F32 | NNZ_DT_F16 | NNZ_DT_BF16 */
+  uint32_t rows;                  /* 0: nothing to do */
+  uint32_t n;                     /* vocabulary, >= 1 */
+  int64_t stride;                 /* elements, any >= n */
+  const int32_t* tokens;          /* [rows][num_tokens], or NULL */
+  uint32_t num_tokens;            /* given tokens per row */
+  uint32_t top_k;                 /* 0 .. 32 */
+  float* logprob;                 /* [rows][num_tokens] */
+  float* entropy;                 /* [rows], or NULL */
+  float* logsumexp;               /* [rows], or NULL */
+  int32_t* top_ids;               /* [rows][top_k] */
+  float* top_logprobs;            /* [rows][top_k] */
+} nnz_logprobs_args;
+
+/* Log probabilities (natural, f32) of given tokens under softmax(logits),
+ * the row's entropy, and the top_k most probable tokens in order (equal
+ * logits: the lower id first), from one read of the logits, which are not
+ * changed.  A logit of -infinity is a disallowed token: probability 0, never
+ * an alternative (alternatives that do not exist: id -1, -infinity).  A row
+ * with nothing allowed gives -infinity, entropy 0.  NaN or +infinity in a
+ * row makes its values NaN (ids: of the logits that are numbers).  A
+ * negative given token is no token: 0.  One >= n gives NaN and raises
+ * NNZ_EDEVICE in nnz_stream_check. */
+int nnz_token_logprobs(const nnz_logprobs_args* args, void* stream);
+
 /* ---- tokenizer: replaces Tokenizer of nnmetal/src/tokenizer.zig ------ */
 /* Byte-level BPE over a HuggingFace tokenizer.json (Qwen3 format).  Host
  * code only (no device calls).  A tokenizer is immutable after creation:

@@ -61,6 +61,33 @@ class NnzTensorDesc(C.Structure):
                 ("dims", C.c_uint32 * 4), ("data", C.c_void_p), ("nbytes", C.c_size_t)]
 
 
+class NnzPagedKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("num_pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+class NnzNormRopeArgs(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("tokens", C.c_uint32),
+                ("num_query_heads", C.c_uint32), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float),
+                ("rope_style", C.c_int32), ("rope_table", C.c_void_p), ("table_positions", C.c_uint32),
+                ("positions", C.c_void_p), ("slots", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_int64)]
+
+
+class NnzPagedAttnArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("tokens", C.c_uint32), ("num_query_heads", C.c_uint32),
+                ("num_seqs", C.c_uint32), ("max_new", C.c_uint32), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("page_table", C.c_void_p), ("table_stride", C.c_uint32), ("scale", C.c_float), ("out", C.c_void_p),
+                ("out_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class NnzLogprobsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_uint32), ("n", C.c_uint32),
+                ("stride", C.c_int64), ("tokens", C.c_void_p), ("num_tokens", C.c_uint32), ("top_k", C.c_uint32),
+                ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("logsumexp", C.c_void_p), ("top_ids", C.c_void_p),
+                ("top_logprobs", C.c_void_p)]
+
+
 class NnzGenerateResult(C.Structure):
     _fields_ = [("tokens_generated", C.c_uint32), ("prefill_ns", C.c_uint64),
                 ("decode_ns", C.c_uint64)]
@@ -103,6 +130,11 @@ SIGNATURES = [
     ("nnz_mlp", I32, [I32, I32, I32, P, P, U32, U32, U32, P, U32, P, P]),
     ("nnz_prefill_gemm", I32, [I32, I32, P, P, P, U32, U32, U32, U32, P, P, I32, P]),
     ("nnz_attn_decode", I32, [P, P, P, P, P, U32, P, U32, U32, U32, U32, F32, F32, I32, U32, P, P]),
+    ("nnz_rope_table", I32, [F32, U32, U32, P, P]),
+    ("nnz_qk_norm_rope_paged", I32, [P, P, P]),
+    ("nnz_paged_attn_workspace", SZ, [P, U32]),
+    ("nnz_paged_attn", I32, [P, P, P]),
+    ("nnz_token_logprobs", I32, [P, P]),
     ("nnz_tokenizer_from_json", I32, [C.c_char_p, SZ, P]),
     ("nnz_tokenizer_from_file", I32, [C.c_char_p, P]),
     ("nnz_tokenizer_free", I32, [P]),

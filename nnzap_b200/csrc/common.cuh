@@ -21,6 +21,7 @@ enum : int {
   ERR_BAD_TOKEN = 2,      // token id >= vocab
   ERR_BAD_POS = 4,        // position >= max_context_length
   ERR_SPIN_TIMEOUT = 8,   // a global flag/counter wait gave up
+  ERR_BAD_PAGE = 16,      // page, slot, length or row range outside its pool or table
 };
 
 // Iteration cap for every spin in this library.  try_wait suspends for a

@@ -13,6 +13,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <map>
@@ -174,6 +175,7 @@ std::string err_text(int flags) {
   if (flags & ERR_BAD_TOKEN) s += " token id >= vocab;";
   if (flags & ERR_BAD_POS) s += " position >= max_context_length;";
   if (flags & ERR_SPIN_TIMEOUT) s += " spin wait timed out;";
+  if (flags & ERR_BAD_PAGE) s += " page, slot, length or row range out of bounds;";
   return s;
 }
 
@@ -183,6 +185,32 @@ namespace nnz {
 int noalloc_take_error(int dev, int* flags);   // noalloc.cu
 // Lets other translation units of the library set nnz_last_error()'s text.
 void set_last_error(const std::string& msg) { g_err = msg; }
+
+// The current device's error word (read and cleared by nnz_stream_check) and
+// its number of SMs, for the entry points that need nothing else.  The word
+// is a file-scope device variable, so nothing is allocated.
+static __device__ int g_op_err;
+
+int op_device(int** err, int* num_sms) {
+  constexpr int kMaxDevices = 64;
+  struct Dev { std::atomic<int*> err{nullptr}; int sms = 0; };
+  static Dev devs[kMaxDevices];
+  static std::mutex mu;
+  int dev = 0;
+  NNZ_CK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return fail(NNZ_EINVAL, "device index out of range");
+  Dev& d = devs[dev];
+  int* p = d.err.load(std::memory_order_acquire);
+  if (!p) {
+    std::lock_guard<std::mutex> lk(mu);
+    NNZ_CK(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
+    NNZ_CK(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_op_err));
+    d.err.store(p, std::memory_order_release);
+  }
+  *err = p;
+  *num_sms = d.sms;
+  return NNZ_OK;
+}
 }  // namespace nnz
 
 struct nnz_model {
@@ -1884,9 +1912,15 @@ int nnz_stream_check(void* stream) {
       }
     }
     int na = 0;
-    const int rc = noalloc_take_error(dev, &na);
+    int rc = noalloc_take_error(dev, &na);
     if (rc) return rc;
     flags |= na;
+    int *op_err = nullptr, sms = 0, no = 0;
+    rc = op_device(&op_err, &sms);
+    if (rc) return rc;
+    NNZ_CK(cudaMemcpy(&no, op_err, sizeof(int), cudaMemcpyDeviceToHost));
+    if (no) NNZ_CK(cudaMemset(op_err, 0, sizeof(int)));
+    flags |= no;
     if (flags)
       return fail(flags & (ERR_MBAR_TIMEOUT | ERR_SPIN_TIMEOUT) ? NNZ_ETIMEDOUT : NNZ_EDEVICE, err_text(flags));
     return NNZ_OK;

@@ -1,0 +1,427 @@
+// Log probabilities of given tokens, the row's entropy and its most probable
+// tokens, from one read of the logits (contract: nnz_token_logprobs in
+// include/nnz_b200.h; the reference's softmax over the same logits is
+// sampleToken, nnmetal/src/transformer.zig:3833-3869).
+//
+// With M = max x, s = sum exp(x - M) and t = sum exp(x - M) (x - M):
+//   log p(i) = (x_i - M) - ln s,   H = -sum p ln p = ln s - t / s.
+// Every thread keeps (M, s, t) of its elements and rescales them when its
+// maximum grows; two such triples merge as s' = s e^d, t' = (t + s d) e^d with
+// d = M - M'.  x - M is formed before the multiplication by log2 e, so the
+// error stays relative to the difference, not to the logits' size.
+//
+// Most probable tokens: every warp holds its best 32 (value, index) pairs as
+// sorted 64-bit keys, one per lane.  An element is looked at again only if it
+// beats the warp's k-th best so far (one compare of the lane's maximum and a
+// vote per 16 or 32 elements of a lane); such elements collect in a small
+// shared buffer that is sorted and merged 32 at a time.  A warp reads
+// increasing indices, so an element equal to the k-th best is never the one
+// that a tie would choose.
+//
+// A row is cut over a cluster of CTAs (1 to 16) whose triples and lists meet
+// in the first CTA's shared memory: no workspace, no atomics, the same
+// result every time.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <string>
+#include <type_traits>
+
+#include "../../include/nnz_b200.h"
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace nnz {
+
+void set_last_error(const std::string& msg);   // engine.cu
+int op_device(int** err, int* num_sms);
+
+namespace {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpVec = 4;              // 16-byte loads per thread and step
+constexpr uint32_t kLpMaxCluster = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct LpArgs {
+  const void* x;
+  uint32_t rows, n;
+  int64_t stride;
+  const int* tokens;
+  uint32_t num_tokens, top_k;
+  float* logprob;
+  float* entropy;
+  float* lse;
+  int* top_ids;
+  float* top_lp;
+  int* err;
+};
+
+struct LpStat {
+  float m, s, t;
+};
+
+// exp of anything below is 0 in f32; differences are cut here so that
+// -infinity and the types' lowest values add 0 to t (0 times the cut).
+constexpr float kLpLow = -200.f;
+
+__device__ __forceinline__ LpStat lp_merge(const LpStat& a, const LpStat& b) {
+  const float m = fmaxf(a.m, b.m);
+  const float da = a.m == m ? 0.f : fmaxf(a.m - m, kLpLow), db = b.m == m ? 0.f : fmaxf(b.m - m, kLpLow);
+  const float ea = expf(da), eb = expf(db);
+  return {m, a.s * ea + b.s * eb, (a.t + a.s * da) * ea + (b.t + b.s * db) * eb};
+}
+
+// Larger key = larger value, then lower index; 0 = no element.
+__device__ __forceinline__ unsigned long long lp_key(float v, uint32_t idx) { return argmax_pack(v + 0.f, idx); }
+__device__ __forceinline__ float lp_value(unsigned long long k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+}
+
+__device__ __forceinline__ unsigned long long lp_exchange(unsigned long long k, int lane, int o, bool desc) {
+  const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+  const bool keep_max = ((lane & o) == 0) == desc;
+  return keep_max ? (k > other ? k : other) : (k < other ? k : other);
+}
+
+// 32 keys, one per lane, into descending order (bitonic sort).
+__device__ __forceinline__ unsigned long long lp_sort32(unsigned long long k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o > 0; o >>= 1) k = lp_exchange(k, lane, o, (lane & size) == 0);
+  return k;
+}
+
+// The best 32 of two descending lists, descending.
+__device__ __forceinline__ unsigned long long lp_merge32(unsigned long long a, unsigned long long b, int lane) {
+  const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  a = a > r ? a : r;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = lp_exchange(a, lane, o, true);
+  return a;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float lp_load1(const T* p) {
+  if constexpr (std::is_same_v<T, float>) return *p;
+  else if constexpr (std::is_same_v<T, __half>) return __half2float(*p);
+  else return __bfloat162float(*p);
+}
+
+// The 16 / sizeof(T) elements of one 16-byte vector as floats.
+template <typename T>
+__device__ __forceinline__ void lp_unpack(const uint4& u, float* x) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+  } else if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+struct LpShared {
+  unsigned long long buf[kLpWarps][64];                        // candidates of each warp
+  unsigned long long list[kLpWarps][32];
+  unsigned long long peer[kLpMaxCluster][32];                  // the cluster's lists (first CTA)
+  LpStat stat[kLpWarps];
+  LpStat peer_stat[kLpMaxCluster];
+};
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
+  constexpr int EPV = 16 / (int)sizeof(T);
+  constexpr int E = kLpVec * EPV;
+  __shared__ LpShared sh;
+  cg::cluster_group cl = cg::this_cluster();
+  const uint32_t C = cl.num_blocks(), rank = cl.block_rank();
+  const uint32_t row = blockIdx.x / C;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* xr = static_cast<const T*>(a.x) + (int64_t)row * a.stride;
+  // 16-byte granules that the row touches; element i of granule g is the
+  // row's element g EPV + i - skew
+  const uint32_t skew = (uint32_t)(reinterpret_cast<uintptr_t>(xr) & 15) / (uint32_t)sizeof(T);
+  const uint4* g0 = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(xr) & ~uintptr_t(15));
+  const uint32_t ng = (uint32_t)(((uint64_t)a.n + skew + EPV - 1) / EPV);
+  const uint32_t gb = (uint32_t)((uint64_t)ng * rank / C), ge = (uint32_t)((uint64_t)ng * (rank + 1) / C);
+
+  // one granule; elements outside the row read as -infinity (a granule that
+  // is partly outside is read element by element)
+  auto load = [&](uint32_t g) -> uint4 {
+    constexpr uint32_t neg = std::is_same_v<T, float> ? 0xFF800000u : std::is_same_v<T, __half> ? 0xFC00FC00u : 0xFF80FF80u;
+    if (g >= ge) return make_uint4(neg, neg, neg, neg);
+    const int64_t e0 = (int64_t)g * EPV - skew;
+    if (e0 >= 0 && e0 + EPV <= (int64_t)a.n) return __ldg(g0 + g);
+    uint32_t w[4] = {neg, neg, neg, neg};
+#pragma unroll
+    for (int i = 0; i < EPV; ++i)
+      if (e0 + i >= 0 && e0 + i < (int64_t)a.n) {
+        if constexpr (sizeof(T) == 4) {
+          w[i] = reinterpret_cast<const uint32_t*>(xr)[e0 + i];
+        } else {
+          const uint32_t h = reinterpret_cast<const uint16_t*>(xr)[e0 + i];
+          w[i / 2] = (i & 1) ? (w[i / 2] & 0xFFFFu) | (h << 16) : (w[i / 2] & 0xFFFF0000u) | h;
+        }
+      }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+
+  LpStat st{-INFINITY, 0.f, 0.f};
+  unsigned long long best = 0;          // lane i: the warp's i-th best
+  float thr = -INFINITY;                 // value of the warp's k-th best (warp-uniform)
+  uint32_t cnt = 0;                      // candidates waiting in the buffer (warp-uniform)
+  auto flush = [&]() {                  // the first 32 of the buffer into the list
+    __syncwarp();
+    unsigned long long k = (uint32_t)lane < cnt ? sh.buf[warp][lane] : 0ull;
+    const unsigned long long rest = (uint32_t)lane + 32 < cnt ? sh.buf[warp][lane + 32] : 0ull;
+    __syncwarp();
+    sh.buf[warp][lane] = rest;
+    cnt = cnt > 32 ? cnt - 32 : 0;
+    best = lp_merge32(best, lp_sort32(k, lane), lane);
+    const unsigned long long kth = __shfl_sync(0xffffffffu, best, (int)a.top_k - 1);
+    if (kth) thr = lp_value(kth);
+    __syncwarp();
+  };
+
+  constexpr uint32_t STEP = kLpThreads * kLpVec;
+  uint4 nxt[kLpVec];
+#pragma unroll
+  for (int u = 0; u < kLpVec; ++u) nxt[u] = load(gb + u * kLpThreads + threadIdx.x);
+  for (uint32_t g = gb; g < ge; g += STEP) {
+    float x[E];
+#pragma unroll
+    for (int u = 0; u < kLpVec; ++u) lp_unpack<T>(nxt[u], x + u * EPV);
+    if (g + STEP < ge) {
+#pragma unroll
+      for (int u = 0; u < kLpVec; ++u) nxt[u] = load(g + STEP + u * kLpThreads + threadIdx.x);
+    }
+    float cm = x[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) cm = fmaxf(cm, x[i]);
+    if (cm > st.m) {
+      const float d = fmaxf(st.m - cm, kLpLow), f = expf(d);
+      st.t = (st.t + st.s * d) * f;
+      st.s *= f;
+      st.m = cm;
+    }
+    const float mm = st.m == -INFINITY ? 0.f : st.m;
+    float s0 = 0.f, t0 = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float d = max_nan(x[i] - mm, kLpLow);
+      const float e = ex2(d * kLog2e);
+      s0 += e;
+      t0 = fmaf(e, d, t0);
+    }
+    st.s += s0;
+    st.t += t0;
+    if constexpr (TOP) {
+      const uint32_t hits = __ballot_sync(0xffffffffu, cm > thr);
+      if (hits) {
+        // with k or more lanes that hold a candidate, the k-th largest of the
+        // lanes' maxima bounds this step's k best from below
+        // (a step's indices are not in order, so its elements are held
+        // against the k-th best of the steps before it)
+        const float seen = thr;
+        float lb = -INFINITY;
+        if (__popc(hits) >= (int)a.top_k)
+          lb = lp_value(__shfl_sync(0xffffffffu, lp_sort32(lp_key(cm > thr ? cm : -INFINITY, 0u), lane), (int)a.top_k - 1));
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const bool take = x[i] > seen && x[i] >= lb;
+          const uint32_t b = __ballot_sync(0xffffffffu, take);
+          if (b) {
+            if (take) {
+              const uint32_t idx = (g + (uint32_t)(i / EPV) * kLpThreads + threadIdx.x) * EPV + i % EPV - skew;
+              sh.buf[warp][cnt + __popc(b & ((1u << lane) - 1u))] = lp_key(x[i], idx);
+            }
+            cnt += __popc(b);
+            if (cnt >= 32) flush();
+          }
+        }
+      }
+    }
+  }
+  if constexpr (TOP)
+    if (cnt) flush();
+
+  // warp -> CTA
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    LpStat b;
+    b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
+    st = lp_merge(st, b);
+  }
+  if (lane == 0) sh.stat[warp] = st;
+  if constexpr (TOP) sh.list[warp][lane] = best;
+  __syncthreads();
+  if constexpr (TOP) {
+#pragma unroll
+    for (int w = kLpWarps / 2; w > 0; w >>= 1) {
+      if (warp < w) {
+        best = lp_merge32(best, sh.list[warp + w][lane], lane);
+        sh.list[warp][lane] = best;
+      }
+      __syncthreads();
+    }
+  }
+  // CTA -> first CTA of the cluster (whose shared memory exists once every
+  // CTA of the cluster has started)
+  if (C > 1) cl.sync();
+  if (warp == 0) {
+    st = sh.stat[0];
+    for (int w = 1; w < kLpWarps; ++w) st = lp_merge(st, sh.stat[w]);
+    LpShared* dst = cl.map_shared_rank(&sh, 0);
+    if (lane == 0) dst->peer_stat[rank] = st;
+    if constexpr (TOP) dst->peer[rank][lane] = best;
+  }
+  if (C > 1) cl.sync();
+  if (rank != 0 || warp != 0) return;
+  __syncwarp();
+  st = sh.peer_stat[0];
+  for (uint32_t r = 1; r < C; ++r) st = lp_merge(st, sh.peer_stat[r]);
+  if constexpr (TOP) {
+    best = sh.peer[0][lane];
+    for (uint32_t r = 1; r < C; ++r) best = lp_merge32(best, sh.peer[r][lane], lane);
+  }
+  const float ls = logf(st.s);
+  // a row with nothing allowed: every log probability -infinity, entropy 0
+  const bool empty = st.m == -INFINITY && st.s == 0.f;
+  if (lane == 0) {
+    if (a.entropy) a.entropy[row] = empty ? 0.f : ls - st.t / st.s;
+    if (a.lse) a.lse[row] = empty ? -INFINITY : st.m + ls;
+  }
+  for (uint32_t j = lane; j < a.num_tokens; j += 32) {
+    const int t = a.tokens[(size_t)row * a.num_tokens + j];
+    float v = 0.f;
+    if (t >= (int64_t)a.n) {
+      atomicOr(a.err, ERR_BAD_TOKEN);
+      v = NAN;
+    } else if (t >= 0) {
+      v = empty ? -INFINITY : (lp_load1(xr + t) - st.m) - ls;
+    }
+    a.logprob[(size_t)row * a.num_tokens + j] = v;
+  }
+  if constexpr (TOP) {
+    if ((uint32_t)lane < a.top_k) {
+      const float v = lp_value(best);
+      const bool none = best == 0 || v == -INFINITY;
+      a.top_ids[(size_t)row * a.top_k + lane] = none ? -1 : (int)argmax_index(best);
+      a.top_lp[(size_t)row * a.top_k + lane] = none ? (st.s == st.s ? -INFINITY : NAN) : (v - st.m) - ls;
+    }
+  }
+}
+
+template <typename T, bool TOP>
+cudaError_t logprobs_go(const LpArgs& a, int sms, cudaStream_t st) {
+  static std::atomic<bool> ready{false};
+  if (!ready.load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute((const void*)&logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    ready.store(true, std::memory_order_relaxed);
+  }
+  // enough CTAs to fill the SMs, but at least a few steps of work for each
+  const uint64_t bytes = (uint64_t)a.n * sizeof(T);
+  uint32_t C = 1;
+  while (C < kLpMaxCluster && (uint64_t)a.rows * C < (uint64_t)sms * 6 && bytes / (2 * C) >= kLpThreads * kLpVec * 16) C *= 2;
+  if ((uint64_t)a.rows * C > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.rows * C);
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, &logprobs_kernel<T, TOP>, a);
+}
+
+template <typename T>
+cudaError_t logprobs_t(const LpArgs& a, int sms, cudaStream_t st) {
+  return a.top_k ? logprobs_go<T, true>(a, sms, st) : logprobs_go<T, false>(a, sms, st);
+}
+
+int refuse(int code, const char* what) noexcept {
+  try {
+    set_last_error(what);
+  } catch (...) {
+  }
+  return code;
+}
+
+}  // namespace
+}  // namespace nnz
+
+extern "C" int nnz_token_logprobs(const nnz_logprobs_args* p, void* stream) {
+  using namespace nnz;
+  if (!p) return refuse(NNZ_EINVAL, "nnz_token_logprobs: null argument");
+  if (p->rows == 0) return NNZ_OK;
+  if (p->dtype != NNZ_DT_F32 && p->dtype != NNZ_DT_F16 && p->dtype != NNZ_DT_BF16)
+    return refuse(NNZ_EINVAL, "nnz_token_logprobs: dtype must be f32, f16 or bf16");
+  const uintptr_t esz = p->dtype == NNZ_DT_F32 ? 4 : 2;
+  if (!p->logits || (reinterpret_cast<uintptr_t>(p->logits) % esz) || p->n == 0 || p->n > 0x7FFFFFF0u || p->rows > 0x7FFFFFFu ||
+      p->stride < (int64_t)p->n)
+    return refuse(NNZ_EINVAL, "nnz_token_logprobs: logits, rows, n or stride");
+  if (p->top_k > 32 || (p->top_k && (!p->top_ids || !p->top_logprobs)))
+    return refuse(NNZ_EINVAL, "nnz_token_logprobs: top_k must be 0 .. 32, with top_ids and top_logprobs");
+  if (p->num_tokens && (!p->tokens || !p->logprob)) return refuse(NNZ_EINVAL, "nnz_token_logprobs: tokens need logprob");
+  LpArgs a{};
+  int sms = 0;
+  if (const int rc = op_device(&a.err, &sms)) return rc;
+  a.x = p->logits;
+  a.rows = p->rows;
+  a.n = p->n;
+  a.stride = p->stride;
+  a.tokens = p->tokens;
+  a.num_tokens = p->num_tokens;
+  a.top_k = p->top_k;
+  a.logprob = p->logprob;
+  a.entropy = p->entropy;
+  a.lse = p->logsumexp;
+  a.top_ids = p->top_ids;
+  a.top_lp = p->top_logprobs;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = p->dtype == NNZ_DT_F32 ? logprobs_t<float>(a, sms, st)
+                      : p->dtype == NNZ_DT_F16 ? logprobs_t<__half>(a, sms, st) : logprobs_t<__nv_bfloat16>(a, sms, st);
+  if (e != cudaSuccess) {
+    try {
+      set_last_error(std::string("nnz_token_logprobs: ") + cudaGetErrorString(e));
+    } catch (...) {
+    }
+    return NNZ_ECUDA;
+  }
+  return NNZ_OK;
+}

@@ -1,0 +1,379 @@
+// Ragged serving over a paged KV cache: entry points, the rotation table,
+// the per-head norm + rotation kernel and the any-layout attention kernel.
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+#include <string>
+
+#include "../../include/nnz_b200.h"
+#include "paged.cuh"
+#include "rope_dev.cuh"
+
+namespace nnz {
+
+void set_last_error(const std::string& msg);      // engine.cu
+int op_device(int** err, int* num_sms);
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// rotation table
+// ---------------------------------------------------------------------------
+__global__ void rope_table_kernel(double l2theta, uint32_t half, uint32_t positions, float2* table) {
+  const uint64_t n = (uint64_t)positions * half;
+  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (uint64_t)gridDim.x * blockDim.x) {
+    const double f = exp2(-l2theta * (double)(i % half) / (double)half);
+    double s, c;
+    sincos((double)(i / half) * f, &s, &c);
+    table[i] = make_float2((float)c, (float)s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// per-head RMSNorm + rotation -> q_out and the pages
+// ---------------------------------------------------------------------------
+// y = x * rsqrt(mean(x^2) + eps) * w over one head, then each pair (a, b) ->
+// (a cos - b sin, a sin + b cos); pairs are (2i, 2i + 1) or (i, i + HD / 2).
+// Bound by bytes: every head is read and written once in 16-byte chunks, HD /
+// 8 lanes to a head, f32 arithmetic, one rounding.  One CTA per token: its
+// heads share the token's table row, which each lane keeps in registers.
+template <typename T, int HD, int STYLE>
+__global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs a) {
+  constexpr int LPH = HD / 8;                          // lanes per head
+  constexpr int NCS = STYLE == ROPE_PAIRWISE ? 4 : 8;   // (cos, sin) of a lane's 8 elements
+  const uint32_t tok = blockIdx.x;
+  const uint32_t hl = threadIdx.x % LPH, hg = threadIdx.x / LPH, ngrp = blockDim.x / LPH;
+  const uint32_t n_kv = a.kv.n_kv, heads = a.n_q + 2 * n_kv;
+  const uint4* src = reinterpret_cast<const uint4*>(a.qkv + (int64_t)tok * a.qkv_stride);
+  const int pos = a.positions[tok];
+  const long long slot = a.slots[tok];
+  const bool bad_pos = pos < 0 || (uint32_t)pos >= a.table_positions;
+  const bool bad_slot = slot >= (long long)a.kv.num_pages * a.kv.page_size;
+  const bool bad = bad_pos || bad_slot;
+  if (bad && threadIdx.x == 0) atomicOr(a.err, bad_pos ? ERR_BAD_POS : ERR_BAD_PAGE);
+  float2 cs[NCS];
+  {
+    const float2* tab = a.table + (size_t)(bad_pos ? 0 : pos) * (HD / 2);
+    const uint32_t i0 = STYLE == ROPE_PAIRWISE ? hl * 4 : (hl % (LPH / 2)) * 8;
+#pragma unroll
+    for (int i = 0; i < NCS; ++i) cs[i] = __ldg(tab + i0 + i);
+  }
+  int64_t page_off = 0;
+  if (!bad && slot >= 0) {
+    const long long pg = slot / a.kv.page_size;
+    page_off = pg * a.kv.page_stride + (slot - pg * a.kv.page_size) * a.kv.token_stride;
+  }
+  for (uint32_t h0 = 0; h0 < heads; h0 += ngrp) {
+    const uint32_t h = h0 + hg;
+    const bool live = h < heads;
+    uint4 u = live ? src[h * LPH + hl] : make_uint4(0u, 0u, 0u, 0u);
+    // every lane takes the shuffles (value heads too: their result is not used)
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    float x[8], ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = T16<T>::to_f2(w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+      ss = fmaf(f.x, f.x, ss);
+      ss = fmaf(f.y, f.y, ss);
+    }
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = rsqrtf(ss / (float)HD + a.eps);
+    const float4* nw = reinterpret_cast<const float4*>((h < a.n_q ? a.q_norm : a.k_norm) + hl * 8);
+    const float4 w0 = __ldg(nw), w1 = __ldg(nw + 1);
+    x[0] *= r * w0.x; x[1] *= r * w0.y; x[2] *= r * w0.z; x[3] *= r * w0.w;
+    x[4] *= r * w1.x; x[5] *= r * w1.y; x[6] *= r * w1.z; x[7] *= r * w1.w;
+    if constexpr (STYLE == ROPE_PAIRWISE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = x[2 * i], q = x[2 * i + 1];
+        x[2 * i] = p * cs[i].x - q * cs[i].y;
+        x[2 * i + 1] = p * cs[i].y + q * cs[i].x;
+      }
+    } else {
+      // element i of the first half pairs with element i of the second,
+      // LPH / 2 lanes away
+      const bool second = hl >= LPH / 2;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, x[i], LPH / 2);
+        x[i] = second ? other * cs[i].y + x[i] * cs[i].x : x[i] * cs[i].x - other * cs[i].y;
+      }
+    }
+    if (h < a.n_q + n_kv)   // a query or key head
+      u = make_uint4(T16<T>::pack(x[0], x[1]), T16<T>::pack(x[2], x[3]), T16<T>::pack(x[4], x[5]),
+                     T16<T>::pack(x[6], x[7]));
+    if (h < a.n_q) {
+      if (bad) u = make_uint4(0u, 0u, 0u, 0u);
+      reinterpret_cast<uint4*>(a.q_out + (int64_t)tok * a.q_stride)[h * LPH + hl] = u;
+    } else if (live && !bad && slot >= 0) {
+      const bool is_k = h < a.n_q + n_kv;
+      const uint32_t kh = h - a.n_q - (is_k ? 0u : n_kv);
+      uint16_t* base = is_k ? a.kv.k : a.kv.v;
+      *reinterpret_cast<uint4*>(base + page_off + (int64_t)kh * a.kv.head_stride + hl * 8) = u;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// attention over any page size and strides: one warp per (row, query head)
+// ---------------------------------------------------------------------------
+// Scores one key at a time (HD / 32 elements per lane, warp sum), online
+// softmax in f32.  No tensor cores and no split over the keys: the layouts
+// that the tiled kernels cannot load are served right, not fast.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) paged_attn_any_kernel(const PagedAttnArgs a) {
+  constexpr int EPL = HD / 32;   // elements per lane, in 2-element words
+  const int lane = threadIdx.x & 31;
+  const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const uint32_t row = (uint32_t)(unit / a.n_q), h = (uint32_t)(unit % a.n_q);
+  if (row >= a.tokens) return;
+  // the sequence of this row: the last s with q_start[s] <= row
+  uint32_t lo = 0, hi = a.num_seqs;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if ((int64_t)a.q_start[mid] <= (int64_t)row) lo = mid;
+    else hi = mid;
+  }
+  const int64_t qs = a.q_start[lo], qe = a.q_start[lo + 1];
+  if (row < qs || row >= qe) return;
+  if (row - qs >= (int64_t)a.max_new) {
+    if (lane == 0) atomicOr(a.err, ERR_BAD_PAGE);
+    return;
+  }
+  const int64_t cap = (int64_t)a.table_stride * a.kv.page_size;
+  int64_t len = a.kv_len[lo];
+  bool bad = len > cap || len < 0 || qe > (int64_t)a.tokens;
+  const int64_t last = min(len, len - (qe - qs) + (row - qs) + 1);   // keys [0, last) are visible
+  len = min(last, cap);
+  const uint16_t* qp = a.q + (int64_t)row * a.q_stride + h * HD;
+  float q[EPL], o[EPL];
+#pragma unroll
+  for (int e = 0; e < EPL; e += 2) {
+    const float2 f = T16<T>::to_f2(*reinterpret_cast<const uint32_t*>(qp + lane * EPL + e));
+    q[e] = f.x * a.scale;
+    q[e + 1] = f.y * a.scale;
+    o[e] = o[e + 1] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  const int64_t head_off = (int64_t)(h / (a.n_q / a.kv.n_kv)) * a.kv.head_stride + lane * EPL;
+  const int* pages = a.page_table + (size_t)lo * a.table_stride;
+  for (int64_t j0 = 0; j0 < len; j0 += a.kv.page_size) {
+    const int pg = pages[j0 / a.kv.page_size];
+    if (pg >= (int64_t)a.kv.num_pages) bad = true;
+    if (pg < 0 || (uint32_t)pg >= a.kv.num_pages) continue;
+    const int64_t base = (int64_t)pg * a.kv.page_stride + head_off;
+    const int n = (int)min((int64_t)a.kv.page_size, len - j0);
+    for (int t = 0; t < n; ++t) {
+      const uint16_t* kp = a.kv.k + base + t * a.kv.token_stride;
+      const uint16_t* vp = a.kv.v + base + t * a.kv.token_stride;
+      float s = 0.f, v[EPL];
+#pragma unroll
+      for (int e = 0; e < EPL; e += 2) {
+        const float2 f = T16<T>::to_f2(*reinterpret_cast<const uint32_t*>(kp + e));
+        const float2 g = T16<T>::to_f2(*reinterpret_cast<const uint32_t*>(vp + e));
+        s = fmaf(q[e], f.x, fmaf(q[e + 1], f.y, s));
+        v[e] = g.x;
+        v[e + 1] = g.y;
+      }
+      s = warp_sum(s);
+      if (s > m) {
+        const float c = expf(m - s);   // 0 at the first key
+        l *= c;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[e] *= c;
+        m = s;
+      }
+      const float p = s == -INFINITY ? 0.f : expf(s - m);
+      l += p;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] = fmaf(p, v[e], o[e]);
+    }
+  }
+  if (bad && lane == 0) atomicOr(a.err, ERR_BAD_PAGE);
+  const float r = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* op = a.out + (int64_t)row * a.out_stride + h * HD + lane * EPL;
+#pragma unroll
+  for (int e = 0; e < EPL; e += 2) *reinterpret_cast<uint32_t*>(op + e) = T16<T>::pack(o[e] * r, o[e + 1] * r);
+}
+
+}  // namespace
+
+cudaError_t rope_table_launch(float theta, uint32_t hd, uint32_t positions, float2* table, cudaStream_t st) {
+  const uint64_t n = (uint64_t)positions * (hd / 2);
+  const uint32_t grid = (uint32_t)std::min<uint64_t>((n + 255) / 256, 148 * 8);
+  rope_table_kernel<<<grid, 256, 0, st>>>(log2((double)theta), hd / 2, positions, table);
+  return cudaGetLastError();
+}
+
+template <typename T, int HD>
+static cudaError_t norm_rope_t(const NormRopeArgs& a, cudaStream_t st) {
+  if (a.rope_style == ROPE_PAIRWISE) norm_rope_kernel<T, HD, ROPE_PAIRWISE><<<a.tokens, 256, 0, st>>>(a);
+  else norm_rope_kernel<T, HD, ROPE_HALF_SPLIT><<<a.tokens, 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t norm_rope_launch(const NormRopeArgs& a, int dtype, int hd, cudaStream_t st) {
+  if (dtype == RD_F16) return hd == 128 ? norm_rope_t<__half, 128>(a, st) : norm_rope_t<__half, 64>(a, st);
+  return hd == 128 ? norm_rope_t<__nv_bfloat16, 128>(a, st) : norm_rope_t<__nv_bfloat16, 64>(a, st);
+}
+
+cudaError_t paged_attn_any_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st) {
+  const uint64_t grid = ((uint64_t)a.tokens * a.n_q + 3) / 4;
+  if (grid > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+  if (dtype == RD_F16) {
+    if (hd == 128) paged_attn_any_kernel<__half, 128><<<(uint32_t)grid, 128, 0, st>>>(a);
+    else paged_attn_any_kernel<__half, 64><<<(uint32_t)grid, 128, 0, st>>>(a);
+  } else {
+    if (hd == 128) paged_attn_any_kernel<__nv_bfloat16, 128><<<(uint32_t)grid, 128, 0, st>>>(a);
+    else paged_attn_any_kernel<__nv_bfloat16, 64><<<(uint32_t)grid, 128, 0, st>>>(a);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace nnz
+
+using namespace nnz;
+
+namespace {
+
+// No C++ exception crosses the C ABI: building the message can throw.
+int refuse(int code, const char* what) noexcept {
+  try {
+    set_last_error(what);
+  } catch (...) {
+  }
+  return code;
+}
+
+int cuda_rc(cudaError_t e, const char* who) noexcept {
+  if (e == cudaSuccess) return NNZ_OK;
+  try {
+    set_last_error(std::string(who) + ": " + cudaGetErrorString(e));
+  } catch (...) {
+  }
+  return NNZ_ECUDA;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// nullptr if `kv` can be used, else what is wrong with it.
+const char* pool_error(const nnz_paged_kv* kv) {
+  if (!kv || !kv->k || !kv->v) return "paged kv: null pool";
+  if (kv->dtype != NNZ_DT_F16 && kv->dtype != NNZ_DT_BF16) return "paged kv: dtype must be f16 or bf16";
+  if (kv->head_dim != 64 && kv->head_dim != 128) return "paged kv: head_dim must be 64 or 128";
+  if (kv->num_kv_heads == 0 || kv->num_kv_heads > 65535) return "paged kv: num_kv_heads";
+  if (kv->num_pages == 0 || kv->num_pages > 0x7FFFFFFFu) return "paged kv: num_pages";
+  if (kv->page_size == 0 || kv->page_size > 65536) return "paged kv: page_size must be 1 .. 65536";
+  if (kv->page_stride % 8 || kv->head_stride % 8 || kv->token_stride % 8 || kv->page_stride < 0 || kv->head_stride < 0 ||
+      kv->token_stride < 0)
+    return "paged kv: strides must be multiples of 8 elements";
+  if (kv->token_stride < kv->head_dim || (kv->num_kv_heads > 1 && kv->head_stride < kv->head_dim) ||
+      (kv->num_pages > 1 && kv->page_stride < kv->head_dim))
+    return "paged kv: strides smaller than a head";
+  if (!aligned16(kv->k) || !aligned16(kv->v)) return "paged kv: k and v must be 16-byte aligned";
+  return nullptr;
+}
+
+PagedPool pool_of(const nnz_paged_kv* kv) {
+  return {static_cast<uint16_t*>(kv->k), static_cast<uint16_t*>(kv->v), kv->num_pages, kv->page_size, kv->num_kv_heads,
+          kv->page_stride, kv->head_stride, kv->token_stride};
+}
+
+int dtype_of(const nnz_paged_kv* kv) { return kv->dtype == NNZ_DT_BF16 ? RD_BF16 : RD_F16; }
+
+}  // namespace
+
+extern "C" {
+
+int nnz_rope_table(float theta, uint32_t head_dim, uint32_t positions, float* table, void* stream) {
+  if (!table || positions == 0 || head_dim == 0 || head_dim % 2 || !(theta > 0.f) || (reinterpret_cast<uintptr_t>(table) & 7))
+    return refuse(NNZ_EINVAL, "nnz_rope_table: invalid arguments");
+  return cuda_rc(rope_table_launch(theta, head_dim, positions, reinterpret_cast<float2*>(table), static_cast<cudaStream_t>(stream)),
+                 "nnz_rope_table");
+}
+
+int nnz_qk_norm_rope_paged(const nnz_paged_kv* kv, const nnz_norm_rope_args* p, void* stream) {
+  if (const char* why = pool_error(kv)) return refuse(NNZ_EINVAL, why);
+  if (!p) return refuse(NNZ_EINVAL, "nnz_qk_norm_rope_paged: null argument");
+  if (p->tokens == 0) return NNZ_OK;
+  if (!p->qkv || !p->q_norm || !p->k_norm || !p->rope_table || !p->positions || !p->slots || !p->q_out)
+    return refuse(NNZ_EINVAL, "nnz_qk_norm_rope_paged: null argument");
+  const int64_t hd = kv->head_dim;
+  if (p->num_query_heads == 0 || p->num_query_heads > 65535 || p->tokens > 0x7FFFFFFFu || p->table_positions == 0 ||
+      (p->rope_style != NNZ_ROPE_PAIRWISE && p->rope_style != NNZ_ROPE_HALF_SPLIT) || !(p->eps >= 0.f))
+    return refuse(NNZ_EINVAL, "nnz_qk_norm_rope_paged: heads, tokens, table, eps or rope_style");
+  if (p->qkv_stride % 8 || p->qkv_stride < (p->num_query_heads + 2 * (int64_t)kv->num_kv_heads) * hd || p->q_stride % 8 ||
+      p->q_stride < p->num_query_heads * hd)
+    return refuse(NNZ_EINVAL, "nnz_qk_norm_rope_paged: row strides must be multiples of 8 elements that hold the heads");
+  if (!aligned16(p->qkv) || !aligned16(p->q_out) || !aligned16(p->q_norm) || !aligned16(p->k_norm) ||
+      (reinterpret_cast<uintptr_t>(p->rope_table) & 7))
+    return refuse(NNZ_EINVAL, "nnz_qk_norm_rope_paged: pointers must be 16-byte aligned");
+  NormRopeArgs a{};
+  int sms = 0;
+  if (const int rc = op_device(&a.err, &sms)) return rc;
+  a.kv = pool_of(kv);
+  a.qkv = static_cast<const uint16_t*>(p->qkv);
+  a.qkv_stride = p->qkv_stride;
+  a.tokens = p->tokens;
+  a.n_q = p->num_query_heads;
+  a.q_norm = p->q_norm;
+  a.k_norm = p->k_norm;
+  a.eps = p->eps;
+  a.rope_style = p->rope_style;
+  a.table = reinterpret_cast<const float2*>(p->rope_table);
+  a.table_positions = p->table_positions;
+  a.positions = p->positions;
+  a.slots = reinterpret_cast<const long long*>(p->slots);
+  a.q_out = static_cast<uint16_t*>(p->q_out);
+  a.q_stride = p->q_stride;
+  return cuda_rc(norm_rope_launch(a, dtype_of(kv), (int)hd, static_cast<cudaStream_t>(stream)), "nnz_qk_norm_rope_paged");
+}
+
+size_t nnz_paged_attn_workspace(const nnz_paged_kv* kv, uint32_t num_query_heads) {
+  if (pool_error(kv) || num_query_heads == 0 || num_query_heads % kv->num_kv_heads) return 0;
+  return 256;
+}
+
+int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* stream) {
+  if (const char* why = pool_error(kv)) return refuse(NNZ_EINVAL, why);
+  if (!p) return refuse(NNZ_EINVAL, "nnz_paged_attn: null argument");
+  const int64_t hd = kv->head_dim;
+  if (p->num_query_heads == 0 || p->num_query_heads % kv->num_kv_heads || p->num_query_heads / kv->num_kv_heads > 64)
+    return refuse(NNZ_EINVAL, "nnz_paged_attn: num_query_heads must be a multiple (<= 64x) of num_kv_heads");
+  if (p->tokens == 0 || p->num_seqs == 0 || p->max_new == 0) return NNZ_OK;
+  if (!p->q || !p->q_start || !p->kv_len || !p->page_table || !p->out || !p->workspace)
+    return refuse(NNZ_EINVAL, "nnz_paged_attn: null argument");
+  if (p->tokens > 0x7FFFFFFFu || p->num_seqs > 0x7FFFFFFFu || p->table_stride == 0 ||
+      (uint64_t)p->table_stride * kv->page_size > 0x7FFFFFFFu || !(p->scale >= 0.f))
+    return refuse(NNZ_EINVAL, "nnz_paged_attn: tokens, num_seqs, table_stride or scale");
+  if (p->q_stride % 8 || p->q_stride < p->num_query_heads * hd || p->out_stride % 8 || p->out_stride < p->num_query_heads * hd)
+    return refuse(NNZ_EINVAL, "nnz_paged_attn: row strides must be multiples of 8 elements that hold the heads");
+  if (!aligned16(p->q) || !aligned16(p->out) || (reinterpret_cast<uintptr_t>(p->workspace) & 255))
+    return refuse(NNZ_EINVAL, "nnz_paged_attn: q and out must be 16-byte, workspace 256-byte aligned");
+  if (p->workspace_bytes < nnz_paged_attn_workspace(kv, p->num_query_heads))
+    return refuse(NNZ_EINVAL, "nnz_paged_attn: workspace too small");
+  PagedAttnArgs a{};
+  if (const int rc = op_device(&a.err, &a.num_sms)) return rc;
+  a.kv = pool_of(kv);
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.q_stride = p->q_stride;
+  a.tokens = p->tokens;
+  a.n_q = p->num_query_heads;
+  a.num_seqs = p->num_seqs;
+  a.max_new = p->max_new;
+  a.q_start = p->q_start;
+  a.kv_len = p->kv_len;
+  a.page_table = p->page_table;
+  a.table_stride = p->table_stride;
+  a.scale = p->scale > 0.f ? p->scale : 1.f / sqrtf((float)hd);
+  a.out = static_cast<uint16_t*>(p->out);
+  a.out_stride = p->out_stride;
+  a.ws = p->workspace;
+  return cuda_rc(paged_attn_any_launch(a, dtype_of(kv), (int)hd, static_cast<cudaStream_t>(stream)), "nnz_paged_attn");
+}
+
+}  // extern "C"
