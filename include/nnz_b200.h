@@ -351,7 +351,7 @@ typedef struct nnz_paged_attn_args {
   const int32_t* q_start;         /* [num_seqs + 1] sequence s's new tokens: rows [q_start[s], q_start[s + 1]) */
   const int32_t* kv_len;          /* [num_seqs] its keys, the new tokens' included */
   const int32_t* page_table;      /* [num_seqs][table_stride] pages in order; negative: absent (evicted) */
-  uint32_t table_stride;
+  uint32_t table_stride;          /* table_stride * page_size <= 2^31 - 2^16 */
   float scale;                    /* 0: 1 / sqrt(head_dim) */
   void* out;                      /* [tokens][out_stride] */
   int64_t out_stride;             /* elements, multiple of 8 */

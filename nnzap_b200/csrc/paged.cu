@@ -7,7 +7,8 @@
 #include <string>
 
 #include "../../include/nnz_b200.h"
-#include "paged.cuh"
+#include "paged_sched.cuh"
+#include "paged_tma.cuh"
 #include "rope_dev.cuh"
 
 namespace nnz {
@@ -139,7 +140,10 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(const PagedAttnArgs
     else hi = mid;
   }
   const int64_t qs = a.q_start[lo], qe = a.q_start[lo + 1];
-  if (row < qs || row >= qe) return;
+  if (row < qs || row >= qe || qs < 0) {
+    if (qs < 0 && lane == 0) atomicOr(a.err, ERR_BAD_PAGE);
+    return;
+  }
   if (row - qs >= (int64_t)a.max_new) {
     if (lane == 0) atomicOr(a.err, ERR_BAD_PAGE);
     return;
@@ -200,7 +204,172 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(const PagedAttnArgs
   for (int e = 0; e < EPL; e += 2) *reinterpret_cast<uint32_t*>(op + e) = T16<T>::pack(o[e] * r, o[e + 1] * r);
 }
 
+// ---------------------------------------------------------------------------
+// merge of split tasks
+// ---------------------------------------------------------------------------
+// Parts k (max m_k, sum l_k, o_k) of a row: M = max m_k, out = sum 2^(m_k - M)
+// o_k / sum 2^(m_k - M) l_k.  A block looks at `span` workers' headers and
+// takes 16 rows of each split task; its 8 warps share the rows, and the parts
+// of a row where there are fewer than 8 of them.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a, const PartWs ws, uint32_t workers, uint32_t span) {
+  constexpr int E = HD / 32;
+  __shared__ float red[8][HD + 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t G = a.n_q / a.kv.n_kv;
+  pdl_wait();
+  const uint32_t w0 = blockIdx.x * span, w1 = min(w0 + span, workers);
+  for (uint32_t w = w0; w < w1; ++w) {
+    const PartHeader h = ws.head[w];
+    if (h.parts == 0) continue;
+    const int rbase = blockIdx.y * 16, rows = min(16, (int)h.rows - rbase);
+    if (rows <= 0) continue;
+    const int sw = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;   // warps to a row
+    const int split = warp % sw;
+    for (int r0 = 0; r0 < rows; r0 += 8 / sw) {
+      const int row = rbase + r0 + warp / sw;
+      const bool live = row < rbase + rows;
+      float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
+      if (live) {
+        for (uint32_t k0 = split; k0 < h.parts; k0 += 4 * sw) {
+          float pm[4], pl[4], po[4][E];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t k = k0 + i * sw;
+            pm[i] = -INFINITY;
+            pl[i] = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) po[i][e] = 0.f;
+            if (k < h.parts) {
+              const float* p = ws.slot((uint64_t)w + k, k == 0 ? 1 : 0, HD);
+              pm[i] = __ldcg(p + row);
+              pl[i] = __ldcg(p + ws.R + row);
+              const float* po_ = p + 2 * ws.R + (size_t)row * HD + lane * E;
+              if constexpr (E == 4) {
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(po_));
+                po[i][0] = f.x; po[i][1] = f.y; po[i][2] = f.z; po[i][3] = f.w;
+              } else {
+                const float2 f = __ldcg(reinterpret_cast<const float2*>(po_));
+                po[i][0] = f.x; po[i][1] = f.y;
+              }
+            }
+          }
+          float mn = m;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mn = fmaxf(mn, pm[i]);
+          const float ms = mn == -INFINITY ? 0.f : mn;
+          const float c = exp2f(m - ms);
+          m = mn;
+          l *= c;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] *= c;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float f = exp2f(pm[i] - ms);
+            l = fmaf(f, pl[i], l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(f, po[i][e], o[e]);
+          }
+        }
+      }
+      if (sw > 1) {
+        if (lane == 0) {
+          red[warp][HD] = m;
+          red[warp][HD + 1] = l;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) red[warp][lane * E + e] = o[e];
+        __syncthreads();
+        if (split == 0) {
+          float mn = m;
+          for (int i = 1; i < sw; ++i) mn = fmaxf(mn, red[warp + i][HD]);
+          const float ms = mn == -INFINITY ? 0.f : mn;
+          const float c = exp2f(m - ms);
+          l *= c;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] *= c;
+          for (int i = 1; i < sw; ++i) {
+            const float f = exp2f(red[warp + i][HD] - ms);
+            l = fmaf(f, red[warp + i][HD + 1], l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(f, red[warp + i][lane * E + e], o[e]);
+          }
+        }
+        __syncthreads();
+      }
+      if (live && split == 0) {
+        const float il = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* op = a.out + ((int64_t)h.row0 + row / G) * a.out_stride + ((int64_t)h.kvh * G + row % G) * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(op + e) = T16<T>::pack(o[e] * il, o[e + 1] * il);
+      }
+    }
+  }
+}
+
 }  // namespace
+
+cudaError_t paged_merge_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  const uint32_t span = std::max(1u, workers / (uint32_t)a.num_sms);
+  cfg.gridDim = dim3((workers + span - 1) / span, (ws.R + 15) / 16);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (dtype == RD_F16)
+    return hd == 128 ? cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__half, 128>, a, ws, workers, span)
+                     : cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__half, 64>, a, ws, workers, span);
+  return hd == 128 ? cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__nv_bfloat16, 128>, a, ws, workers, span)
+                   : cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__nv_bfloat16, 64>, a, ws, workers, span);
+}
+
+namespace {
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+bool encode16(CUtensorMap* tm, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+  const EncodeFn enc = encode_fn();
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  return enc && enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+bool paged_tensor_map(CUtensorMap* tm, const PagedPool& kv, const void* base, int hd, uint32_t keys) {
+  const cuuint64_t dims[4] = {(cuuint64_t)hd, kv.page_size, kv.n_kv, kv.num_pages};
+  // a dimension of one element takes any stride
+  const cuuint64_t strides[3] = {(cuuint64_t)kv.token_stride * 2, (cuuint64_t)(kv.n_kv > 1 ? kv.head_stride : kv.token_stride) * 2,
+                                 (cuuint64_t)(kv.num_pages > 1 ? kv.page_stride : kv.token_stride) * 2};
+  const cuuint32_t box[4] = {64, keys, 1, 1};
+  return encode16(tm, base, 4, dims, strides, box);
+}
+
+bool paged_q_map(CUtensorMap* tm, const PagedAttnArgs& a, int hd, uint32_t heads, uint32_t tokens) {
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, a.n_q, a.tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)a.q_stride * 2};
+  const cuuint32_t box[3] = {64, heads, tokens};
+  return encode16(tm, a.q, 3, dims, strides, box);
+}
 
 cudaError_t rope_table_launch(float theta, uint32_t hd, uint32_t positions, float2* table, cudaStream_t st) {
   const uint64_t n = (uint64_t)positions * (hd / 2);
@@ -335,7 +504,10 @@ int nnz_qk_norm_rope_paged(const nnz_paged_kv* kv, const nnz_norm_rope_args* p, 
 
 size_t nnz_paged_attn_workspace(const nnz_paged_kv* kv, uint32_t num_query_heads) {
   if (pool_error(kv) || num_query_heads == 0 || num_query_heads % kv->num_kv_heads) return 0;
-  return 256;
+  int* err = nullptr;
+  int sms = 0;
+  if (op_device(&err, &sms)) sms = 148;   // no device: the size for a full B200
+  return std::max<size_t>(256, part_ws_bytes(paged_stream_workers(sms), kStreamRows, kv->head_dim));
 }
 
 int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* stream) {
@@ -348,7 +520,7 @@ int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* s
   if (!p->q || !p->q_start || !p->kv_len || !p->page_table || !p->out || !p->workspace)
     return refuse(NNZ_EINVAL, "nnz_paged_attn: null argument");
   if (p->tokens > 0x7FFFFFFFu || p->num_seqs > 0x7FFFFFFFu || p->table_stride == 0 ||
-      (uint64_t)p->table_stride * kv->page_size > 0x7FFFFFFFu || !(p->scale >= 0.f))
+      (uint64_t)p->table_stride * kv->page_size > 0x7FFF0000u || !(p->scale >= 0.f))
     return refuse(NNZ_EINVAL, "nnz_paged_attn: tokens, num_seqs, table_stride or scale");
   if (p->q_stride % 8 || p->q_stride < p->num_query_heads * hd || p->out_stride % 8 || p->out_stride < p->num_query_heads * hd)
     return refuse(NNZ_EINVAL, "nnz_paged_attn: row strides must be multiples of 8 elements that hold the heads");
@@ -373,7 +545,13 @@ int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* s
   a.out = static_cast<uint16_t*>(p->out);
   a.out_stride = p->out_stride;
   a.ws = p->workspace;
-  return cuda_rc(paged_attn_any_launch(a, dtype_of(kv), (int)hd, static_cast<cudaStream_t>(stream)), "nnz_paged_attn");
+  // The tiled kernels copy boxes of 8 or 16 keys of one page; a page whose
+  // size is no multiple of 8 would end inside one.
+  const bool tiled = kv->page_size % 8 == 0;
+  const uint64_t rows = (uint64_t)a.max_new * (a.n_q / a.kv.n_kv);
+  const cudaError_t e = tiled && rows <= kStreamRows ? paged_stream_launch(a, dtype_of(kv), (int)hd, static_cast<cudaStream_t>(stream))
+                                                     : paged_attn_any_launch(a, dtype_of(kv), (int)hd, static_cast<cudaStream_t>(stream));
+  return cuda_rc(e, "nnz_paged_attn");
 }
 
 }  // extern "C"

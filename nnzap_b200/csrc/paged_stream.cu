@@ -1,0 +1,421 @@
+// Attention of few query rows over paged K/V (at most 16 rows per sequence
+// and kv head: single tokens, drafts of a few tokens): bound by the bytes of
+// K and V.
+//
+// Every warp is a worker of the shared cut (paged_sched.cuh): it streams its
+// run of 16-key units through a private ring of shared memory, each unit four
+// (or, with pages whose size is only a multiple of 8, eight) TMA copies of K
+// and V halves with the 128-byte swizzle, issued one per lane, so a unit's
+// page may lie anywhere and ldmatrix reads without conflicts.  S = Q K^T and
+// O += P V are mma.m16n8k16 with the G heads of every new token as rows; the
+// online softmax keeps its f32 maximum and sum in the score fragments' lanes.
+// The ring runs ahead across task boundaries.  Page numbers are read 32
+// copies ahead, one per lane.
+//
+// Absent pages and keys past the length are not loaded or not trusted: their
+// scores are masked, their V rows zeroed in shared memory.
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <atomic>
+
+#include "paged_sched.cuh"
+#include "paged_tma.cuh"
+
+namespace nnz {
+
+namespace {
+
+constexpr int kStWarps = 4;
+constexpr int kStKeys = 16;
+
+template <int HD>
+struct StShape {
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kBoxB = kStKeys * 128;                 // 16 keys x 64 dims
+  static constexpr int kStageB = 2 * kHalves * kBoxB;          // K halves, V halves
+  static constexpr int kStages = HD == 128 ? 3 : 6;
+  static constexpr int kWarpB = kStages * kStageB + 1024;      // + barriers and flags, whole swizzle atoms
+  static constexpr int kSmem = kStWarps * kWarpB + 1024;       // + alignment
+};
+
+struct StArgs {
+  CUtensorMap tmK, tmV;
+  PagedAttnArgs a;
+  PartWs ws;
+  uint32_t workers, min_per;
+  uint32_t box;        // keys per copy: 16 or 8
+  float sl2;           // scale * log2(e)
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (T16<T>::kBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+
+// 16-byte chunk ch (dims 8 ch ..) of key row r of a tile of swizzled boxes.
+__device__ __forceinline__ uint32_t st_off(int r, int ch) {
+  return (uint32_t)((ch >> 3) * (kStKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ bool finite16(uint32_t w, bool bf16) {
+  const uint32_t e = bf16 ? 0x7F807F80u : 0x7C007C00u;
+  return (w & e & 0xFFFFu) != (e & 0xFFFFu) && (w & e & 0xFFFF0000u) != (e & 0xFFFF0000u);
+}
+
+// ROWS8: at most 8 query rows (the lower half of every fragment is absent).
+template <typename T, int HD, bool ROWS8>
+__global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __grid_constant__ StArgs t) {
+  using S = StShape<HD>;
+  constexpr int NR = ROWS8 ? 1 : 2;        // fragment row halves
+  constexpr int KS = HD / 16;              // K steps of S
+  constexpr int NT = HD / 8;               // n tiles of O
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const PagedAttnArgs& a = t.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  uint8_t* ring = smem + warp * S::kWarpB;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + S::kStages * S::kStageB);
+  volatile uint32_t* there = reinterpret_cast<uint32_t*>(bars + S::kStages);   // copies present, one bit each
+  if (lane == 0) {
+    for (int s = 0; s < S::kStages; ++s) mbar_init(&bars[s], 1);
+    fence_barrier_init();
+  }
+  const int G = (int)(a.n_q / a.kv.n_kv);
+  const int QT = (int)a.max_new;           // one tile holds all rows
+  pdl_wait();
+  pdl_launch();
+  uint32_t per = 1;
+  const BlockStart bs = block_start<kStWarps * 32>(a, QT, kStKeys, [&](uint64_t total) -> uint64_t {
+    per = max((uint32_t)((total + t.workers - 1) / t.workers), t.min_per);
+    return (uint64_t)blockIdx.x * kStWarps * per;
+  });
+  const uint64_t worker = (uint64_t)blockIdx.x * kStWarps + warp;
+  const uint64_t u0 = worker * per, u1 = min(u0 + per, bs.total);
+  PartHeader hdr{0, 0, 0, 0};
+  Cursor c;
+  bool work = u0 < u1;
+  if (work) {
+    c.s = bs.seq;
+    work = cursor_seq(a, c, QT, kStKeys) && cursor_skip(a, c, u0 - bs.before, QT, kStKeys);
+  }
+  if (!work) {
+    if (lane == 0) t.ws.head[worker] = hdr;
+    return;
+  }
+
+  // ---- producer: copies of one unit, one per lane ----
+  Cursor pc = c;
+  uint32_t left = (uint32_t)(u1 - u0);      // units still to be issued
+  const uint32_t nb = kStKeys / t.box;       // copies along the keys of a unit
+  const uint32_t ncopy = nb * 2 * S::kHalves;
+  uint32_t page0 = 0, npage = 0;             // key boxes whose page numbers the lanes hold
+  int my_page = -1;
+  uint32_t my_at = 0;
+  auto issue = [&](int stg) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the slot was read, and maybe zeroed, by this warp
+    __syncwarp();
+    const uint32_t b0 = pc.unit * nb;
+    if (b0 < page0 || b0 + nb > page0 + npage) {
+      page0 = b0;
+      npage = 32;
+      const uint32_t key = (page0 + lane) * t.box, pi = key / a.kv.page_size;
+      my_at = key - pi * a.kv.page_size;
+      my_page = -1;
+      if ((int64_t)key < pc.q.seen(pc.q.rows - 1)) {
+        my_page = __ldg(a.page_table + (size_t)pc.s * a.table_stride + pi);
+        if (my_page >= (int64_t)a.kv.num_pages) {
+          atomicOr(a.err, ERR_BAD_PAGE);
+          my_page = -1;
+        }
+      }
+    }
+    // lane i copies box i % nb of part i / nb (K halves, then V halves)
+    const uint32_t bi = (uint32_t)lane % nb, part = (uint32_t)lane / nb;
+    const int pg = __shfl_sync(0xffffffffu, my_page, (int)(b0 - page0 + bi));
+    const uint32_t at = __shfl_sync(0xffffffffu, my_at, (int)(b0 - page0 + bi));
+    const bool go = (uint32_t)lane < ncopy && pg >= 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, go);
+    if (lane == 0) {
+      there[stg] = mask & ((1u << nb) - 1u);
+      mbar_arrive_expect_tx(&bars[stg], (uint32_t)__popc(mask) * t.box * 128);
+    }
+    __syncwarp();
+    if (go)
+      tma_load_4d(ring + stg * S::kStageB + part * S::kBoxB + bi * t.box * 128, part < S::kHalves ? &t.tmK : &t.tmV,
+                  (int)(part % S::kHalves) * 64, (int)at, (int)pc.kvh, pg, &bars[stg]);
+    __syncwarp();
+    --left;
+    if (++pc.unit == pc.units) {
+      npage = 0;
+      if (left) cursor_next_task(a, pc, QT, kStKeys);
+    }
+  };
+  int pstg = 0;
+  for (int s = 0; s < S::kStages && left; ++s) {
+    issue(pstg);
+    pstg = pstg + 1 == S::kStages ? 0 : pstg + 1;
+  }
+
+  bool failed = false;
+  int cstg = 0;
+  uint32_t phase = 0;       // bit s: parity of stage s
+  uint64_t u = u0;
+  for (;;) {
+    const uint32_t take = (uint32_t)min((uint64_t)(c.units - c.unit), u1 - u);   // units of this task here
+    const int nrow = c.q.rows * G;
+    // query fragments of row g (and g + 8): row = token * G + head
+    uint32_t qa[KS][2 * NR];
+    int limit[NR];           // keys that the row sees
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int row = g + 8 * r;
+      const bool ok = row < nrow;
+      const int tok = ok ? row / G : 0;
+      limit[r] = ok ? (int)c.q.seen(tok) : 0;
+      const uint16_t* qp = a.q + (c.q.row0 + tok) * a.q_stride + (int64_t)(c.kvh * G + (ok ? row - tok * G : 0)) * HD + 2 * q4;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        qa[ks][r] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * ks)) : 0u;
+        qa[ks][NR + r] = ok ? __ldg(reinterpret_cast<const uint32_t*>(qp + 16 * ks + 8)) : 0u;
+      }
+    }
+    const int seen_all = (int)c.q.seen(0), seen_any = (int)c.q.seen(c.q.rows - 1);
+    float o[NT][2 * NR];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2 * NR; ++e) o[j][e] = 0.f;
+    float m[NR], l[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+    }
+    for (uint32_t i = 0; i < take; ++i) {
+      if (!failed) failed = !mbar_wait(&bars[cstg], (phase >> cstg) & 1u, a.err);
+      phase ^= 1u << cstg;
+      const uint32_t kb = smem_u32(ring + cstg * S::kStageB), vb = kb + S::kHalves * S::kBoxB;
+      const int key0 = (int)(c.unit + i) * kStKeys;
+      const uint32_t have = there[cstg];
+      const bool all_there = have == (1u << nb) - 1u;
+      auto present = [&](int k) { return all_there || ((have >> (nb == 1 ? 0 : k >> 3)) & 1u); };   // k: key of the unit
+      if (!all_there || key0 + kStKeys > seen_any) {
+        // V rows that nothing may look at: zero, so that 0 * V stays 0
+        for (int k = lane; k < kStKeys * HD / 8; k += 32) {
+          const int r = k / (HD / 8);
+          if (!present(r) || key0 + r >= seen_any)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vb + st_off(r, k % (HD / 8))), "r"(0u) : "memory");
+        }
+        __syncwarp();
+      }
+      // S = Q K^T: two n tiles of 8 keys
+      float s[2][4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int kq = 0; kq < KS / 2; ++kq) {
+          uint32_t r0, r1, r2, r3;
+          ldsm4(kb + st_off(nt * 8 + (lane & 7), 4 * kq + (lane >> 3)), r0, r1, r2, r3);
+          mma16<T>(s[nt], qa[2 * kq][0], ROWS8 ? 0u : qa[2 * kq][NR - 1], qa[2 * kq][NR], ROWS8 ? 0u : qa[2 * kq][2 * NR - 1], r0, r1);
+          mma16<T>(s[nt], qa[2 * kq + 1][0], ROWS8 ? 0u : qa[2 * kq + 1][NR - 1], qa[2 * kq + 1][NR],
+                   ROWS8 ? 0u : qa[2 * kq + 1][2 * NR - 1], r2, r3);
+        }
+      }
+      uint32_t pa[2][2];       // [key half][row half]
+      float pv[NR][4];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = (e >> 1) * 8 + 2 * q4 + (e & 1);
+          const float x = s[e >> 1][2 * r + (e & 1)] * t.sl2;
+          pv[r][e] = key0 + k < limit[r] && present(k) ? x : -INFINITY;
+          mx = fmaxf(mx, pv[r][e]);
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[r], mx);
+        const float ms = mn == -INFINITY ? 0.f : mn;      // nothing seen yet: every p is exp2(-inf) = 0
+        const float al = exp2f(m[r] - ms);
+        m[r] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pv[r][e] = exp2f(pv[r][e] - ms);
+          sum += pv[r][e];
+        }
+        l[r] = l[r] * al + sum;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          o[j][2 * r] *= al;
+          o[j][2 * r + 1] *= al;
+        }
+        pa[0][r] = T16<T>::pack(pv[r][0], pv[r][1]);
+        pa[1][r] = T16<T>::pack(pv[r][2], pv[r][3]);
+      }
+      if (key0 + kStKeys > seen_all && nrow > G) {
+        // Keys that some rows see and others do not: a non-finite V row would
+        // reach the others as 0 * V.  Such a row (rare) is added in f32 to the
+        // rows that see it and zeroed for the product.
+        uint32_t bad = 0;      // lane r < 16: row r has a non-finite element
+        if (lane < kStKeys)
+          for (int ch = 0; ch < HD / 8; ++ch) {
+            uint32_t w0, w1, w2, w3;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(vb + st_off(lane, ch)) : "memory");
+            constexpr bool bf = T16<T>::kBf16;
+            bad |= !(finite16(w0, bf) && finite16(w1, bf) && finite16(w2, bf) && finite16(w3, bf));
+          }
+        uint32_t rows = __ballot_sync(0xffffffffu, bad != 0);
+        while (rows) {
+          const int k = __ffs(rows) - 1;
+          rows &= rows - 1;
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            float p = 0.f;     // p of (row g + 8 r, key k): held by lane 4 g + (k % 8) / 2
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = __shfl_sync(0xffffffffu, pv[r][e], (lane & ~3) | ((k & 7) >> 1));
+              if (e == (k >> 3) * 2 + (k & 1)) p = x;
+            }
+            if (key0 + k < limit[r])
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                uint32_t w;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(vb + st_off(k, j) + 4 * q4) : "memory");
+                const float2 f = T16<T>::to_f2(w);
+                o[j][2 * r] = fmaf(p, f.x, o[j][2 * r]);
+                o[j][2 * r + 1] = fmaf(p, f.y, o[j][2 * r + 1]);
+              }
+          }
+          __syncwarp();
+          if (lane < HD / 8)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vb + st_off(k, lane)), "r"(0u) : "memory");
+          __syncwarp();
+        }
+      }
+      // O += P V
+#pragma unroll
+      for (int jp = 0; jp < NT / 2; ++jp) {
+        uint32_t r0, r1, r2, r3;
+        ldsm4t(vb + st_off((lane & 7) + 8 * ((lane >> 3) & 1), 2 * jp + (lane >> 4)), r0, r1, r2, r3);
+        if constexpr (ROWS8) {
+          float d0[4] = {o[2 * jp][0], o[2 * jp][1], 0.f, 0.f}, d1[4] = {o[2 * jp + 1][0], o[2 * jp + 1][1], 0.f, 0.f};
+          mma16<T>(d0, pa[0][0], 0u, pa[1][0], 0u, r0, r1);
+          mma16<T>(d1, pa[0][0], 0u, pa[1][0], 0u, r2, r3);
+          o[2 * jp][0] = d0[0];
+          o[2 * jp][1] = d0[1];
+          o[2 * jp + 1][0] = d1[0];
+          o[2 * jp + 1][1] = d1[1];
+        } else {
+          mma16<T>(reinterpret_cast<float(&)[4]>(o[2 * jp]), pa[0][0], pa[0][NR - 1], pa[1][0], pa[1][NR - 1], r0, r1);
+          mma16<T>(reinterpret_cast<float(&)[4]>(o[2 * jp + 1]), pa[0][0], pa[0][NR - 1], pa[1][0], pa[1][NR - 1], r2, r3);
+        }
+      }
+      __syncwarp();
+      if (left) issue(cstg);   // refill the slot just consumed
+      cstg = cstg + 1 == S::kStages ? 0 : cstg + 1;
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    const uint64_t t0 = u - c.unit, t1 = t0 + c.units;       // the task's units
+    if (take == c.units) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int row = g + 8 * r;
+        if (row >= nrow) continue;
+        const float il = l[r] == 0.f ? 0.f : 1.f / l[r];
+        uint16_t* op = a.out + (c.q.row0 + row / G) * a.out_stride + (int64_t)(c.kvh * G + row % G) * HD + 2 * q4;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) *reinterpret_cast<uint32_t*>(op + 8 * j) = T16<T>::pack(o[j][2 * r] * il, o[j][2 * r + 1] * il);
+      }
+    } else {
+      const bool first = c.unit == 0;
+      float* slot = t.ws.slot(worker, first ? 1 : 0, HD);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int row = g + 8 * r;
+        if (row >= nrow) continue;
+        if (q4 == 0) {
+          slot[row] = m[r];
+          slot[kStreamRows + row] = l[r];
+        }
+        float* op = slot + 2 * kStreamRows + row * HD + 2 * q4;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(op + 8 * j) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+      }
+      if (first) hdr = {(uint32_t)c.q.row0, c.kvh, (uint32_t)nrow, (uint32_t)((t1 - 1) / per - worker + 1)};
+    }
+    u += take;
+    c.unit += take;
+    if (u >= u1) break;
+    cursor_next_task(a, c, QT, kStKeys);
+  }
+  if (lane == 0) t.ws.head[worker] = hdr;
+}
+
+template <typename T, int HD, bool ROWS8>
+cudaError_t stream_go(const StArgs& t, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t e = raise_smem((const void*)&paged_stream_kernel<T, HD, ROWS8>, StShape<HD>::kSmem, ready);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(t.workers / kStWarps);
+  cfg.blockDim = dim3(kStWarps * 32);
+  cfg.dynamicSmemBytes = StShape<HD>::kSmem;
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, &paged_stream_kernel<T, HD, ROWS8>, t);
+}
+
+template <typename T>
+cudaError_t stream_t(const StArgs& t, int hd, cudaStream_t st) {
+  const bool r8 = (uint64_t)t.a.max_new * (t.a.n_q / t.a.kv.n_kv) <= 8;
+  if (hd == 128) return r8 ? stream_go<T, 128, true>(t, st) : stream_go<T, 128, false>(t, st);
+  return r8 ? stream_go<T, 64, true>(t, st) : stream_go<T, 64, false>(t, st);
+}
+
+}  // namespace
+
+uint32_t paged_stream_workers(int num_sms) { return (uint32_t)num_sms * 2 * kStWarps; }
+
+cudaError_t paged_stream_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st) {
+  StArgs t;
+  t.a = a;
+  t.workers = paged_stream_workers(a.num_sms);
+  t.ws = part_ws(a.ws, t.workers, kStreamRows);
+  t.min_per = 1;
+  t.box = a.kv.page_size % 16 ? 8 : 16;
+  t.sl2 = a.scale * 1.4426950408889634f;
+  if (!paged_tensor_map(&t.tmK, a.kv, a.kv.k, hd, t.box) || !paged_tensor_map(&t.tmV, a.kv, a.kv.v, hd, t.box))
+    return cudaErrorInvalidValue;
+  const cudaError_t e = dtype == RD_F16 ? stream_t<__half>(t, hd, st) : stream_t<__nv_bfloat16>(t, hd, st);
+  if (e != cudaSuccess) return e;
+  return paged_merge_launch(a, t.ws, t.workers, dtype, hd, st);
+}
+
+}  // namespace nnz

@@ -1,0 +1,39 @@
+// TMA access to a page pool: a 4-D tensor map [page][kv head][token][d] of
+// 16-bit elements whose boxes are `keys` tokens x 64 dims of one page and
+// head, 128-byte swizzled.
+#pragma once
+#include <cuda.h>
+
+#include <atomic>
+
+#include "paged.cuh"
+
+namespace nnz {
+
+// x: dim (0 or 64), y: token within the page.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tm, int x, int y, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// False if the driver entry point is missing or it refuses the strides.
+bool paged_tensor_map(CUtensorMap* tm, const PagedPool& kv, const void* base, int hd, uint32_t keys);
+// Rows of q as [token][head][d]: boxes of `heads` heads x `tokens` tokens x 64 dims.
+bool paged_q_map(CUtensorMap* tm, const PagedAttnArgs& a, int hd, uint32_t heads, uint32_t tokens);
+
+// Raises a kernel's dynamic shared-memory limit, once per device.
+inline cudaError_t raise_smem(const void* fn, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+}  // namespace nnz
