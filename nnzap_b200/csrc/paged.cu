@@ -507,7 +507,8 @@ size_t nnz_paged_attn_workspace(const nnz_paged_kv* kv, uint32_t num_query_heads
   int* err = nullptr;
   int sms = 0;
   if (op_device(&err, &sms)) sms = 148;   // no device: the size for a full B200
-  return std::max<size_t>(256, part_ws_bytes(paged_stream_workers(sms), kStreamRows, kv->head_dim));
+  return std::max(part_ws_bytes(paged_stream_workers(sms), kStreamRows, kv->head_dim),
+                  part_ws_bytes((uint32_t)sms, kUmmaRows, kv->head_dim));
 }
 
 int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* stream) {
@@ -545,12 +546,14 @@ int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* s
   a.out = static_cast<uint16_t*>(p->out);
   a.out_stride = p->out_stride;
   a.ws = p->workspace;
-  // The tiled kernels copy boxes of 8 or 16 keys of one page; a page whose
+  // The tiled kernels copy boxes of 8 keys or more of one page; a page whose
   // size is no multiple of 8 would end inside one.
   const bool tiled = kv->page_size % 8 == 0;
   const uint64_t rows = (uint64_t)a.max_new * (a.n_q / a.kv.n_kv);
-  const cudaError_t e = tiled && rows <= kStreamRows ? paged_stream_launch(a, dtype_of(kv), (int)hd, static_cast<cudaStream_t>(stream))
-                                                     : paged_attn_any_launch(a, dtype_of(kv), (int)hd, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int dt = dtype_of(kv);
+  const cudaError_t e = !tiled ? paged_attn_any_launch(a, dt, (int)hd, st)
+                      : rows <= kStreamRows ? paged_stream_launch(a, dt, (int)hd, st) : paged_umma_launch(a, dt, (int)hd, st);
   return cuda_rc(e, "nnz_paged_attn");
 }
 

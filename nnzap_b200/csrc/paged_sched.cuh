@@ -236,5 +236,8 @@ cudaError_t paged_merge_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_
 constexpr uint32_t kStreamRows = 16;
 uint32_t paged_stream_workers(int num_sms);
 cudaError_t paged_stream_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st);
+// Many query rows: 2 x 128 to a CTA, tcgen05 (paged_umma.cu).
+constexpr uint32_t kUmmaRows = 256;
+cudaError_t paged_umma_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st);
 
 }  // namespace nnz

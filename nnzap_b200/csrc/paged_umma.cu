@@ -1,0 +1,625 @@
+// Attention of many query rows over paged K/V on tcgen05: prompt chunks, alone
+// or mixed with single tokens.
+//
+// A task is 2 x 128 rows, (token, head) pairs of one sequence and kv head
+// with the G heads fastest, so the heads of a group share every K/V tile; its
+// units are tiles of 128 keys, and the units of all tasks are cut into equal
+// runs, one per CTA and SM (paged_sched.cuh).  Per unit, for each of the two
+// row tiles:
+//   S = Q K^T           tcgen05.mma, operands in shared memory, f32 in TMEM
+//   P = 2^(S c - m)     one thread per row: online softmax out of TMEM, P in
+//                       the pool's type over the S it came from
+//   O += P V            tcgen05.mma, P from TMEM, V as stored (MN-major B)
+// so while one row tile's softmax runs, the tensor cores work for the other.
+// m lags behind the running maximum by up to 2^8 (a row's O is rescaled only
+// when the maximum has grown by more, which after the first tiles is rare): P
+// up to 256 costs no precision, the sums are f32.
+//
+// Roles: warps 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (thread =
+// TMEM lane = row), warp 8 TMA (Q, then K and V tiles into one ring, boxes of
+// one page each, one per lane), warp 9 MMA issue, warp 10 walks the
+// run of units and hands out its parts (11 only makes the third warpgroup
+// whole).  Boxes of absent pages and
+// past the length are loaded from beyond the pool's last page: the copy
+// engine fills them with zeros, so no stale byte meets the product.
+//
+// TMEM: S / P of the two row tiles at columns 0 and 128, O at 256 and 384.
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "paged_sched.cuh"
+#include "paged_tma.cuh"
+#include "umma.cuh"
+
+namespace nnz {
+
+namespace {
+
+constexpr int kUmKeys = 128;
+constexpr int kUmThreads = 384;
+// Registers a thread: 384 x 168 at launch; the two softmax warpgroups take 208
+// each (a row of S stays in registers), the third goes down to 80: 2 x 128 x
+// 208 + 128 x 80 = 63488 of 64512.
+constexpr int kUmRegsSoftmax = 208, kUmRegsIssue = 80;
+constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
+constexpr int kSegs = 4;                          // segments in flight
+constexpr int kPres = 8;                          // units whose page masks are kept
+constexpr float kLag = 8.f;                       // log2 of the largest P
+
+template <int HD>
+struct UmShape {
+  static constexpr uint32_t kTileB = (HD / 64) * kHalfB;      // Q, K or V tile of 128 rows
+  static constexpr int kStages = HD == 128 ? 5 : 8;
+  static constexpr uint32_t OFF_KV = 2 * kTileB;
+  static constexpr uint32_t OFF_BAR = OFF_KV + kStages * kTileB;
+  static constexpr int kBars = 2 * kStages + 8 + kPres + 2 * kSegs;
+  static constexpr uint32_t OFF_MISC = OFF_BAR + kBars * 8;
+  static constexpr uint32_t kSmem = OFF_MISC + 128 + kSegs * 128 + 1024;
+};
+
+struct UmArgs {
+  CUtensorMap tmQ, tmK, tmV;
+  PagedAttnArgs a;
+  PartWs ws;
+  uint32_t workers, min_per;
+  uint32_t box;       // keys per copy: 8 .. 128
+  uint32_t pt;        // tokens per row tile: 128 / G
+  float sl2;          // scale * log2(e)
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// D(tmem) (+)= A(tmem) B(smem), kind::f16.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// 32 columns of this thread's TMEM lane; complete only after tm_wait_ld.
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]),
+        "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+        "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+}
+// Waits for this thread's TMEM loads; v is tied to the wait so that no use of
+// it can be scheduled before.
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+  asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                    "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <bool BF16>
+__host__ __device__ constexpr uint32_t um_idesc(int M, int N) {
+  return idesc_f16(M, N) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+}
+
+// 16-bit words with a non-finite element (exponent all ones).
+template <bool BF16>
+__device__ __forceinline__ uint32_t bad_mask(uint32_t w) {
+  constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
+  return ((w & e) == e ? 0xFFFFu : 0u) | (((w >> 16) & e) == e ? 0xFFFF0000u : 0u);
+}
+
+// The part of one task in a CTA's run, as warp 10 hands it to the others.
+struct Segment {
+  uint32_t take;       // units (0: the run is over)
+  uint32_t unit;       // first unit within the task
+  uint32_t n[2];       // units that each row tile looks at (from the first)
+  uint32_t parts;      // 0: the whole task; else the parts it is split into
+  uint32_t s, kvh;
+  int row0;            // q / out row of the task's first token
+  int rows;            // tokens of the task
+  uint32_t marks[8];   // keys with a non-finite V, among the task's last 256 (set by the MMA warp)
+  int d, e;            // token i of the task sees keys [0, clamp(d + i, 0, e))
+
+  __device__ __forceinline__ int seen(int i) const { return max(0, min(d + i, e)); }
+};
+// Adds the non-finite V elements d0 .. d0 + 31 of the marked keys that the
+// row sees (a NaN or an infinity times a positive probability is itself).
+template <bool BF16>
+__device__ __forceinline__ void add_nonfinite(const PagedAttnArgs& a, const Segment& g, const volatile uint32_t* marks, int limit, int d0, float (&o)[32]) {
+  const int base = max(0, g.seen(g.rows - 1) - 256);
+  for (int w = 0; w < 8; ++w) {
+    uint32_t bits = marks[w];
+    while (bits) {
+      const int key = base + 32 * w + __ffs(bits) - 1;
+      bits &= bits - 1;
+      if (key >= limit) continue;
+      const uint32_t pi = (uint32_t)key / a.kv.page_size;
+      const int pg = __ldg(a.page_table + (size_t)g.s * a.table_stride + pi);
+      const uint16_t* vp = a.kv.v + (int64_t)pg * a.kv.page_stride + (int64_t)g.kvh * a.kv.head_stride +
+                           (int64_t)((uint32_t)key - pi * a.kv.page_size) * a.kv.token_stride + d0;
+#pragma unroll
+      for (int d = 0; d < 32; d += 2) {
+        const uint32_t e = *reinterpret_cast<const uint32_t*>(vp + d);
+        const uint32_t b = bad_mask<BF16>(e);
+        const float2 f = T16<std::conditional_t<BF16, __nv_bfloat16, __half>>::to_f2(e & b);
+        o[d] += f.x;
+        o[d + 1] += f.y;
+      }
+    }
+  }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_constant__ UmArgs t) {
+  using S = UmShape<HD>;
+  constexpr bool BF = T16<T>::kBf16;
+  constexpr int NH = HD / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const PagedAttnArgs& a = t.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(sm + S::OFF_BAR);
+  uint64_t* kv_empty = kv_full + S::kStages;
+  uint64_t* q_full = kv_empty + S::kStages;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;        // [2] S of a row tile complete
+  uint64_t* p_full = s_full + 2;         // [2] P written, O rescaled (4 warps)
+  uint64_t* pv_done = p_full + 2;        // [2] P V complete
+  uint64_t* pres_full = pv_done + 2;     // [kPres] page mask of a unit written
+  uint64_t* seg_full = pres_full + kPres;   // [kSegs]
+  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 10 other warps are done with it
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + S::OFF_MISC);
+  volatile uint32_t* pres = tslot + 1;   // [kPres] one bit per box of the unit: page present
+  Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_MISC + 128);
+  const uint32_t G = a.n_q / a.kv.n_kv;
+  const int PT = (int)t.pt, QT = 2 * PT;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(kv_full + i, 1);
+      mbar_init(kv_empty + i, 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(pv_done + i, 1);
+    }
+    for (int i = 0; i < kPres; ++i) mbar_init(pres_full + i, 1);
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(seg_full + i, 1);
+      mbar_init(seg_empty + i, 10);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tslot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch();
+  uint32_t per = 1;
+  const BlockStart bs = block_start<kUmThreads>(a, QT, kUmKeys, [&](uint64_t total) -> uint64_t {
+    per = max((uint32_t)((total + t.workers - 1) / t.workers), t.min_per);
+    return (uint64_t)blockIdx.x * per;
+  });
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  Segment g;
+  bool failed = false;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!failed) failed = !mbar_wait(bar, parity & 1u, a.err);
+  };
+
+  // segment k of the run; every warp but 10 takes them in order
+  auto segment = [&](uint32_t k, Segment& g) -> bool {
+    wait(seg_full + k % kSegs, k / kSegs);
+    g = segs[k % kSegs];
+    return g.take != 0 && !failed;
+  };
+  auto segment_done = [&](uint32_t k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive1(seg_empty + k % kSegs);
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUmRegsIssue));
+  if (warp == 8) {
+    // ---------------- TMA ----------------
+    const uint32_t nb = kUmKeys / t.box;
+    const uint32_t bi = (uint32_t)lane % nb, half = (uint32_t)lane / nb;
+    const bool copies = half < (uint32_t)NH;
+    uint32_t stage_use = 0, unit_no = 0;
+    for (uint32_t seg = 0; segment(seg, g); ++seg) {
+      const int last = g.seen(g.rows - 1);
+      const int* pages = a.page_table + (size_t)g.s * a.table_stride;
+      // page of this lane's box of unit i; -1 where there is none
+      auto page_of = [&](uint32_t i, uint32_t& at) -> int {
+        const uint32_t key = (g.unit + i) * kUmKeys + bi * t.box;
+        at = 0;
+        if (key >= (uint32_t)last) return -1;
+        const uint32_t pi = key / a.kv.page_size;
+        at = key - pi * a.kv.page_size;
+        const int p = __ldg(pages + pi);
+        if (p >= 0 && (uint32_t)p >= a.kv.num_pages) {
+          atomicOr(a.err, ERR_BAD_PAGE);
+          return -1;
+        }
+        return p;
+      };
+      uint32_t at, nat = 0;
+      int pg = page_of(0, at), npg = -1;
+      for (uint32_t i = 0; i < g.take; ++i) {
+        if (i + 1 < g.take) npg = page_of(i + 1, nat);
+        const uint32_t mask = __ballot_sync(0xffffffffu, (uint32_t)lane < nb && pg >= 0);
+        const int slot = (int)(unit_no % kPres);
+        if (lane == 0) {
+          pres[slot] = mask;
+          mbar_arrive1(pres_full + slot);
+        }
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t st = stage_use % S::kStages, round = stage_use / S::kStages;
+          if (round) wait(kv_empty + st, round - 1);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(kv_full + st, S::kTileB);
+          __syncwarp();
+          if (copies)
+            tma_load_4d(sm + S::OFF_KV + st * S::kTileB + half * kHalfB + bi * t.box * 128, kv ? &t.tmV : &t.tmK, (int)half * 64, (int)at,
+                        (int)g.kvh, pg >= 0 ? pg : (int)a.kv.num_pages, kv_full + st);
+          ++stage_use;
+          if (kv == 0 && i == 0) {
+            // the queries, once the previous segment's products have read theirs
+            if (seg) wait(q_empty, seg - 1);
+            __syncwarp();
+            const int tiles = PT < g.rows ? 2 : 1;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(q_full, (uint32_t)tiles * NH * G * PT * 128);
+              for (int x = 0; x < tiles; ++x)
+                for (int h = 0; h < NH; ++h)
+                  tma_load_3d(sm + x * S::kTileB + h * kHalfB, &t.tmQ, h * 64, (int)(g.kvh * G), g.row0 + x * PT, q_full);
+            }
+            __syncwarp();
+          }
+        }
+        pg = npg;
+        at = nat;
+        ++unit_no;
+      }
+      segment_done(seg);
+    }
+  } else if (warp == 9) {
+    // ---------------- MMA ----------------
+    constexpr uint32_t id_s = um_idesc<BF>(128, 128), id_o = um_idesc<BF>(128, HD) | (1u << 16);
+    uint32_t stage_use = 0, np[2] = {0, 0};
+    auto issue_s = [&](int x, uint32_t st) {
+      if (lane == 0) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const uint64_t da = smem_desc_sw128(sm + x * S::kTileB + h * kHalfB);
+          const uint64_t db = smem_desc_sw128(sm + S::OFF_KV + st * S::kTileB + h * kHalfB);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) umma_f16(tmem + x * 128, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), id_s, (h | kk) != 0);
+        }
+        umma_commit(s_full + x);
+      }
+      __syncwarp();
+    };
+    auto issue_o = [&](int x, uint32_t st, bool acc) {
+      if (lane == 0) {
+#pragma unroll
+        for (int kk = 0; kk < kUmKeys / 16; ++kk)
+          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, smem_desc_sw128_mn(sm + S::OFF_KV + st * S::kTileB + kk * 16 * 128), id_o,
+                  acc || kk != 0);
+        umma_commit(pv_done + x);
+      }
+      __syncwarp();
+    };
+    auto release = [&](uint64_t* bar) {
+      if (lane == 0) umma_commit(bar);
+      __syncwarp();
+    };
+    for (uint32_t seg = 0; segment(seg, g); ++seg) {
+      const int seen_all = g.seen(0), seen_any = g.seen(g.rows - 1);
+      wait(q_full, seg);
+      for (uint32_t i = 0; i <= g.take; ++i) {
+        // K of unit i, V of unit i - 1 (the ring holds K0 V0 K1 V1 ...)
+        const uint32_t ku = stage_use + 2 * i, vu = stage_use + 2 * i - 1;
+        const uint32_t ks = ku % S::kStages, vs = vu % S::kStages;
+        if (i < g.take) wait(kv_full + ks, ku / S::kStages);
+        if (i > 0) {
+          wait(kv_full + vs, vu / S::kStages);
+          const int key0 = (int)((g.unit + i - 1) * kUmKeys);
+          if (key0 + kUmKeys > seen_all) {
+            // Keys that not every row sees: a V row past the length is zeroed
+            // (its box holds earlier keys), and so is every non-finite element
+            // of the others, or 0 * V would reach the rows that do not see it;
+            // the epilogue adds it to those that do.
+            const int base = max(0, seen_any - 256);   // key of the first mark
+            for (int e = lane; e < kUmKeys * HD / 8; e += 32) {
+              const int r = e / (HD / 8), ch = e % (HD / 8);
+              uint8_t* p = sm + S::OFF_KV + vs * S::kTileB + (ch >> 3) * kHalfB + sw128_off((uint32_t)r, (uint32_t)(ch & 7));
+              uint4* p4 = reinterpret_cast<uint4*>(p);
+              if (key0 + r >= seen_any) {
+                *p4 = make_uint4(0u, 0u, 0u, 0u);
+              } else if (key0 + r >= seen_all) {
+                uint4 w = *p4;
+                const uint32_t b0 = bad_mask<BF>(w.x), b1 = bad_mask<BF>(w.y), b2 = bad_mask<BF>(w.z), b3 = bad_mask<BF>(w.w);
+                if (b0 | b1 | b2 | b3) {
+                  *p4 = make_uint4(w.x & ~b0, w.y & ~b1, w.z & ~b2, w.w & ~b3);
+                  const uint32_t bit = (uint32_t)(key0 + r - base);
+                  atomicOr(segs[seg % kSegs].marks + (bit >> 5), 1u << (bit & 31));
+                }
+              }
+            }
+            fence_async_smem();
+            __threadfence_block();
+            __syncwarp();
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (i > 0 && i - 1 < g.n[x]) {
+            wait(p_full + x, np[x]);
+            ++np[x];
+            tc_fence_after();
+            issue_o(x, vs, i > 1);
+          }
+          if (i < g.n[x]) {
+            tc_fence_after();
+            issue_s(x, ks);
+          }
+        }
+        if (i > 0) release(kv_empty + vs);
+        if (i < g.take) release(kv_empty + ks);
+        if (i + 1 == g.take) release(q_empty);
+      }
+      stage_use += 2 * g.take;
+      segment_done(seg);
+    }
+    if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
+  } else if (warp == 10) {
+    // ---------------- the run, task by task ----------------
+    const uint64_t u0 = (uint64_t)blockIdx.x * per, u1 = min(u0 + per, bs.total);
+    uint64_t u = u0;
+    Cursor c;
+    bool more = u0 < u1;
+    if (more) {
+      c.s = bs.seq;
+      more = cursor_seq(a, c, QT, kUmKeys) && cursor_skip(a, c, u0 - bs.before, QT, kUmKeys);
+    }
+    for (uint32_t k = 0;; ++k) {
+      Segment o{};
+      if (more && u < u1) {
+        o.take = (uint32_t)min((uint64_t)(c.units - c.unit), u1 - u);
+        o.unit = c.unit;
+        o.s = c.s;
+        o.kvh = c.kvh;
+        const int tok0 = c.qt * QT;
+        o.row0 = (int)c.q.row0 + tok0;
+        o.rows = min(QT, c.q.rows - tok0);
+        o.e = (int)min(max(c.q.len, (int64_t)0), c.q.cap);
+        o.d = (int)max(c.q.len - c.q.n + 1 + tok0, (int64_t)-(1 << 30));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i * PT < o.rows) {
+            const uint32_t un = max(1u, ((uint32_t)o.seen(min((i + 1) * PT, o.rows) - 1) + kUmKeys - 1) / kUmKeys);
+            o.n[i] = un > c.unit ? min(un - c.unit, o.take) : 0;
+          }
+        if (o.take != c.units) {
+          const uint64_t t0 = u - c.unit;
+          o.parts = (uint32_t)((t0 + c.units - 1) / per - t0 / per + 1);
+        }
+        u += o.take;
+        if (u < u1) more = cursor_next_task(a, c, QT, kUmKeys);
+      }
+      if (k >= kSegs) wait(seg_empty + k % kSegs, k / kSegs - 1);
+      __syncwarp();
+      if (lane == 0) {
+        segs[k % kSegs] = o;
+        mbar_arrive1(seg_full + k % kSegs);
+      }
+      if (o.take == 0 || failed) break;
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUmRegsSoftmax));
+    // ---------------- softmax and epilogue of row tile x ----------------
+    const int x = warp >> 2;
+    const uint32_t r = 32u * (warp & 3) + lane;
+    const uint32_t tl = tmem + ((32u * (warp & 3)) << 16);
+    const uint32_t tS = tl + x * 128, tO = tl + 256 + x * 128;
+    uint32_t ns = 0, unit_no = 0;       // units of this row tile, units of the run
+    PartHeader hdr{0, 0, 0, 0};
+    for (uint32_t seg = 0; segment(seg, g); ++seg) {
+      const int tok = x * PT + (int)(r / G);         // token of the task
+      const bool live = r < (uint32_t)PT * G && tok < g.rows;
+      const int limit = live ? g.seen(tok) : 0;
+      const bool tile = x * PT < g.rows;
+      const int seen_all = g.seen(x * PT);
+      float m = -INFINITY, l = 0.f;
+      for (uint32_t i = 0; i < g.n[x]; ++i) {
+        const uint32_t un = unit_no + i;
+        wait(s_full + x, ns);
+        tc_fence_after();
+        wait(pres_full + un % kPres, un / kPres);   // written before the unit's K was asked for
+        const uint32_t mask = pres[un % kPres];
+        float s[128];
+        {
+          uint32_t v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tm_ld32(tS + 32 * c, v[c]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tm_wait_ld(v[c]);
+#pragma unroll
+          for (int e = 0; e < 128; ++e) s[e] = __uint_as_float(v[e >> 5][e & 31]);
+        }
+        const int key0 = (int)((g.unit + i) * kUmKeys);
+        const bool all_there = mask == (1u << (kUmKeys / t.box)) - 1u;
+        if (!all_there || key0 + kUmKeys > seen_all) {
+          const uint32_t sh = 31 - __clz(t.box);
+          const int end = limit - key0;
+#pragma unroll
+          for (int e = 0; e < 128; ++e) {
+            const bool ok = e < end && ((mask >> (e >> sh)) & 1u);
+            s[e] = ok ? s[e] : -INFINITY;
+          }
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * t.sl2;
+        // (top is NaN only for a row whose scores are: then so is its result)
+        const bool grow = top > m + kLag;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mn = grow ? top : m;
+          const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+          l *= f;
+          m = mn;
+          if (i > 0) {
+            wait(pv_done + x, ns - 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t w[32];
+              tm_ld32(tO + 32 * c, w);
+              tm_wait_ld(w);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+              tmem_st32(tO + 32 * c, w);
+            }
+          }
+        }
+        const float ms = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float p0 = ex2(fmaf(s[64 * c + 2 * e], t.sl2, -ms)), p1 = ex2(fmaf(s[64 * c + 2 * e + 1], t.sl2, -ms));
+            sum[e & 1] += p0;
+            sum[2 + (e & 1)] += p1;
+            w[e] = T16<T>::pack(p0, p1);
+          }
+          tmem_st32(tS + 32 * c, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(p_full + x);
+        ++ns;
+      }
+      unit_no += g.take;
+      if (tile) {
+        const bool whole = g.parts == 0, first = g.unit == 0;
+        const float il = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const uint32_t rr = (uint32_t)x * PT * G + r;
+        uint16_t* op = a.out + (int64_t)(g.row0 + tok) * a.out_stride + (int64_t)(g.kvh * G + r % G) * HD;
+        float* slot = t.ws.slot(blockIdx.x, first ? 1 : 0, HD);
+        float* part = slot + 2 * t.ws.R + (size_t)rr * HD;
+        if (live && !whole) {
+          slot[rr] = m;
+          slot[t.ws.R + rr] = l;
+        }
+        if (first && !whole) hdr = {(uint32_t)g.row0, g.kvh, (uint32_t)g.rows * G, g.parts};
+        if (g.n[x]) {
+          wait(pv_done + x, ns - 1);
+          tc_fence_after();
+        }
+        const volatile uint32_t* mk = segs[seg % kSegs].marks;
+        uint32_t marks = 0;      // some key of the segment has a non-finite V
+        if (g.n[x])
+          for (int w = 0; w < 8; ++w) marks |= mk[w];
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t w[32];
+          float o[32];
+          if (g.n[x]) {
+            tm_ld32(tO + 32 * c, w);
+            tm_wait_ld(w);
+          }
+#pragma unroll
+          for (int d = 0; d < 32; ++d) o[d] = g.n[x] ? __uint_as_float(w[d]) * il : 0.f;
+          if (marks) add_nonfinite<BF>(a, g, mk, limit, 32 * c, o);
+          if (live && whole) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 8)
+              *reinterpret_cast<uint4*>(op + 32 * c + d) = make_uint4(T16<T>::pack(o[d], o[d + 1]), T16<T>::pack(o[d + 2], o[d + 3]),
+                                                                      T16<T>::pack(o[d + 4], o[d + 5]), T16<T>::pack(o[d + 6], o[d + 7]));
+          } else if (live) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 4) *reinterpret_cast<float4*>(part + 32 * c + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+          }
+        }
+        tc_fence_before();
+      }
+      segment_done(seg);
+    }
+    if (threadIdx.x == 0) t.ws.head[blockIdx.x] = hdr;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <typename T, int HD>
+cudaError_t umma_go(const UmArgs& t, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t e = raise_smem((const void*)&paged_umma_kernel<T, HD>, (int)UmShape<HD>::kSmem, ready);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(t.workers);
+  cfg.blockDim = dim3(kUmThreads);
+  cfg.dynamicSmemBytes = UmShape<HD>::kSmem;
+  cfg.stream = st;
+  return cudaLaunchKernelEx(&cfg, &paged_umma_kernel<T, HD>, t);
+}
+
+}  // namespace
+
+cudaError_t paged_umma_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st) {
+  UmArgs t;
+  t.a = a;
+  t.workers = (uint32_t)a.num_sms;
+  t.ws = part_ws(a.ws, t.workers, kUmmaRows);
+  t.min_per = 1;
+  t.box = 8;
+  while (t.box < (uint32_t)kUmKeys && a.kv.page_size % (2 * t.box) == 0) t.box *= 2;
+  const uint32_t G = a.n_q / a.kv.n_kv;
+  t.pt = 128 / G;
+  t.sl2 = a.scale * 1.4426950408889634f;
+  if (!paged_tensor_map(&t.tmK, a.kv, a.kv.k, hd, t.box) || !paged_tensor_map(&t.tmV, a.kv, a.kv.v, hd, t.box) ||
+      !paged_q_map(&t.tmQ, a, hd, G, t.pt))
+    return cudaErrorInvalidValue;
+  cudaError_t e;
+  if (dtype == RD_F16) e = hd == 128 ? umma_go<__half, 128>(t, st) : umma_go<__half, 64>(t, st);
+  else e = hd == 128 ? umma_go<__nv_bfloat16, 128>(t, st) : umma_go<__nv_bfloat16, 64>(t, st);
+  if (e != cudaSuccess) return e;
+  return paged_merge_launch(a, t.ws, t.workers, dtype, hd, st);
+}
+
+}  // namespace nnz
