@@ -10,17 +10,16 @@
 // d = M - M'.  x - M is formed before the multiplication by log2 e, so the
 // error stays relative to the difference, not to the logits' size.
 //
-// Most probable tokens: every warp holds its best 32 (value, index) pairs as
-// sorted 64-bit keys, one per lane.  An element is looked at again only if it
-// beats the warp's k-th best so far (one compare of the lane's maximum and a
-// vote per 16 or 32 elements of a lane); such elements collect in a small
-// shared buffer that is sorted and merged 32 at a time.  A warp reads
-// increasing indices, so an element equal to the k-th best is never the one
-// that a tie would choose.
+// Most probable tokens cost the stream nothing but a store: every thread's
+// maximum of each step (16 or 32 elements) goes to shared memory.  The k-th
+// largest of the 256 threads' overall maxima bounds the CTA's k best from
+// below; the steps whose maximum reaches it (about k of them) are read again,
+// 64 bytes each, and their elements collected as sorted 64-bit (value, index)
+// keys, 32 to a list, one per lane of a warp.
 //
 // A row is cut over a cluster of CTAs (1 to 16) whose triples and lists meet
-// in the first CTA's shared memory: no workspace, no atomics, the same
-// result every time.
+// in the first CTA's shared memory: no workspace, no atomics on memory, the
+// same result every time.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -90,8 +89,14 @@ __device__ __forceinline__ unsigned long long lp_exchange(unsigned long long k, 
   return keep_max ? (k > other ? k : other) : (k < other ? k : other);
 }
 
+__device__ __forceinline__ uint32_t lp_exchange(uint32_t k, int lane, int o, bool desc) {
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, k, o);
+  return ((lane & o) == 0) == desc ? max(k, other) : min(k, other);
+}
+
 // 32 keys, one per lane, into descending order (bitonic sort).
-__device__ __forceinline__ unsigned long long lp_sort32(unsigned long long k, int lane) {
+template <typename K>
+__device__ __forceinline__ K lp_sort32(K k, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
@@ -100,8 +105,9 @@ __device__ __forceinline__ unsigned long long lp_sort32(unsigned long long k, in
 }
 
 // The best 32 of two descending lists, descending.
-__device__ __forceinline__ unsigned long long lp_merge32(unsigned long long a, unsigned long long b, int lane) {
-  const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
+template <typename K>
+__device__ __forceinline__ K lp_merge32(K a, K b, int lane) {
+  const K r = __shfl_sync(0xffffffffu, b, 31 - lane);
   a = a > r ? a : r;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a = lp_exchange(a, lane, o, true);
@@ -149,19 +155,57 @@ __device__ __forceinline__ void lp_unpack(const uint4& u, float* x) {
   }
 }
 
+constexpr int kLpSlots = 24;      // step maxima kept per thread; longer slices keep one per 2, 4, .. steps
+
 struct LpShared {
+  float smax[kLpSlots][kLpThreads];
   unsigned long long buf[kLpWarps][64];                        // candidates of each warp
   unsigned long long list[kLpWarps][32];
+  uint32_t tmax[kLpWarps][32];
   unsigned long long peer[kLpMaxCluster][32];                  // the cluster's lists (first CTA)
   LpStat stat[kLpWarps];
   LpStat peer_stat[kLpMaxCluster];
 };
+struct LpSharedNoTop {
+  LpStat stat[kLpWarps];
+  LpStat peer_stat[kLpMaxCluster];
+};
+
+// Butterfly over groups of W lanes.
+template <int W>
+__device__ __forceinline__ LpStat lp_warp_merge(LpStat st) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    LpStat b;
+    b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
+    st = lp_merge(st, b);
+  }
+  return st;
+}
+
+// The CTA's best 32 from one descending list per warp: in warp 0's `mine` and
+// in lists[0], after a barrier of the CTA.
+template <typename K>
+__device__ __forceinline__ void lp_tree(K (*lists)[32], K& mine, int warp, int lane) {
+  lists[warp][lane] = mine;
+  __syncthreads();
+#pragma unroll
+  for (int w = kLpWarps / 2; w > 0; w >>= 1) {
+    if (warp < w) {
+      mine = lp_merge32(mine, lists[warp + w][lane], lane);
+      lists[warp][lane] = mine;
+    }
+    __syncthreads();
+  }
+}
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
   constexpr int EPV = 16 / (int)sizeof(T);
   constexpr int E = kLpVec * EPV;
-  __shared__ LpShared sh;
+  __shared__ std::conditional_t<TOP, LpShared, LpSharedNoTop> sh;
   cg::cluster_group cl = cg::this_cluster();
   const uint32_t C = cl.num_blocks(), rank = cl.block_rank();
   const uint32_t row = blockIdx.x / C;
@@ -196,27 +240,16 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
   };
 
   LpStat st{-INFINITY, 0.f, 0.f};
-  unsigned long long best = 0;          // lane i: the warp's i-th best
-  float thr = -INFINITY;                 // value of the warp's k-th best (warp-uniform)
-  uint32_t cnt = 0;                      // candidates waiting in the buffer (warp-uniform)
-  auto flush = [&]() {                  // the first 32 of the buffer into the list
-    __syncwarp();
-    unsigned long long k = (uint32_t)lane < cnt ? sh.buf[warp][lane] : 0ull;
-    const unsigned long long rest = (uint32_t)lane + 32 < cnt ? sh.buf[warp][lane + 32] : 0ull;
-    __syncwarp();
-    sh.buf[warp][lane] = rest;
-    cnt = cnt > 32 ? cnt - 32 : 0;
-    best = lp_merge32(best, lp_sort32(k, lane), lane);
-    const unsigned long long kth = __shfl_sync(0xffffffffu, best, (int)a.top_k - 1);
-    if (kth) thr = lp_value(kth);
-    __syncwarp();
-  };
-
   constexpr uint32_t STEP = kLpThreads * kLpVec;
   uint4 nxt[kLpVec];
 #pragma unroll
   for (int u = 0; u < kLpVec; ++u) nxt[u] = load(gb + u * kLpThreads + threadIdx.x);
-  for (uint32_t g = gb; g < ge; g += STEP) {
+  const uint32_t steps = (ge - gb + STEP - 1) / STEP;
+  int shift = 0;                     // 2^shift steps share a slot of smax
+  while ((steps + (1u << shift) - 1) >> shift > (uint32_t)kLpSlots) ++shift;
+  float slot_max = -INFINITY;
+  uint32_t step = 0;
+  for (uint32_t g = gb; g < ge; g += STEP, ++step) {
     float x[E];
 #pragma unroll
     for (int u = 0; u < kLpVec; ++u) lp_unpack<T>(nxt[u], x + u * EPV);
@@ -245,75 +278,103 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
     st.s += s0;
     st.t += t0;
     if constexpr (TOP) {
-      const uint32_t hits = __ballot_sync(0xffffffffu, cm > thr);
-      if (hits) {
-        // with k or more lanes that hold a candidate, the k-th largest of the
-        // lanes' maxima bounds this step's k best from below
-        // (a step's indices are not in order, so its elements are held
-        // against the k-th best of the steps before it)
-        const float seen = thr;
-        float lb = -INFINITY;
-        if (__popc(hits) >= (int)a.top_k)
-          lb = lp_value(__shfl_sync(0xffffffffu, lp_sort32(lp_key(cm > thr ? cm : -INFINITY, 0u), lane), (int)a.top_k - 1));
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const bool take = x[i] > seen && x[i] >= lb;
-          const uint32_t b = __ballot_sync(0xffffffffu, take);
-          if (b) {
-            if (take) {
-              const uint32_t idx = (g + (uint32_t)(i / EPV) * kLpThreads + threadIdx.x) * EPV + i % EPV - skew;
-              sh.buf[warp][cnt + __popc(b & ((1u << lane) - 1u))] = lp_key(x[i], idx);
-            }
-            cnt += __popc(b);
-            if (cnt >= 32) flush();
-          }
-        }
-      }
+      slot_max = (step & ((1u << shift) - 1)) == 0 ? cm : fmaxf(slot_max, cm);
+      sh.smax[step >> shift][threadIdx.x] = slot_max;
     }
   }
-  if constexpr (TOP)
-    if (cnt) flush();
 
+  const float thread_max = st.m;
   // warp -> CTA
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    LpStat b;
-    b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-    st = lp_merge(st, b);
-  }
+  st = lp_warp_merge<32>(st);
   if (lane == 0) sh.stat[warp] = st;
-  if constexpr (TOP) sh.list[warp][lane] = best;
-  __syncthreads();
+  unsigned long long best = 0;          // lane i: the i-th best so far
   if constexpr (TOP) {
-#pragma unroll
-    for (int w = kLpWarps / 2; w > 0; w >>= 1) {
-      if (warp < w) {
-        best = lp_merge32(best, sh.list[warp + w][lane], lane);
-        sh.list[warp][lane] = best;
-      }
-      __syncthreads();
+    // the k-th largest of the threads' maxima
+    uint32_t tk = lp_sort32(float_key(thread_max + 0.f), lane);
+    lp_tree(sh.tmax, tk, warp, lane);
+    const float floor_ = lp_value((unsigned long long)sh.tmax[0][a.top_k - 1] << 32);
+
+    // The steps of this warp's threads that reach it are read again, four
+    // loads at a time; lane: vector lane / EPV of the step, element lane % EPV.
+    const uint32_t slots = (steps + (1u << shift) - 1) >> shift;
+    uint32_t mine = 0;                   // slots of this thread
+    for (uint32_t sl = 0; sl < slots; ++sl) {
+      const float v = sh.smax[sl][threadIdx.x];
+      if (v >= floor_ && v > -INFINITY) mine |= 1u << sl;
     }
+    uint32_t cnt = 0;                    // candidates waiting in the buffer (warp-uniform)
+    unsigned long long kth = 0;           // the list's k-th key
+    auto flush = [&]() {                 // the first 32 of the buffer into the list
+      __syncwarp();
+      const unsigned long long k = (uint32_t)lane < cnt ? sh.buf[warp][lane] : 0ull;
+      const unsigned long long rest = (uint32_t)lane + 32 < cnt ? sh.buf[warp][lane + 32] : 0ull;
+      __syncwarp();
+      sh.buf[warp][lane] = rest;
+      cnt = cnt > 32 ? cnt - 32 : 0;
+      best = lp_merge32(best, lp_sort32(k, lane), lane);
+      kth = __shfl_sync(0xffffffffu, best, (int)a.top_k - 1);
+      __syncwarp();
+    };
+    uint32_t src = 0, sl = 0, sub = 0;   // thread (lane), slot and step of the next load
+    uint32_t owners = __ballot_sync(0xffffffffu, mine != 0);
+    while (owners || sub) {
+      float xv[4];
+      uint32_t idx[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        xv[q] = -INFINITY;
+        idx[q] = 0;
+        if (!(owners || sub)) continue;
+        if (sub == 0) {
+          src = (uint32_t)__ffs(owners) - 1;
+          sl = (uint32_t)__ffs(__shfl_sync(0xffffffffu, mine, (int)src)) - 1;
+          if ((uint32_t)lane == src) mine &= mine - 1;
+          owners = __ballot_sync(0xffffffffu, mine != 0);
+        }
+        const uint32_t gr = gb + ((sl << shift) + sub) * STEP + (lane / EPV) * kLpThreads + warp * 32 + src;
+        const int64_t e = (int64_t)gr * EPV + lane % EPV - skew;
+        if (lane < E && gr < ge && e >= 0 && e < (int64_t)a.n) xv[q] = lp_load1(xr + e);
+        idx[q] = (uint32_t)e;
+        sub = (sub + 1) & ((1u << shift) - 1);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned long long key = xv[q] >= floor_ && xv[q] > -INFINITY ? lp_key(xv[q], idx[q]) : 0ull;
+        const bool take = key > kth;
+        const uint32_t b = __ballot_sync(0xffffffffu, take);
+        if (take) sh.buf[warp][cnt + __popc(b & ((1u << lane) - 1u))] = key;
+        cnt += __popc(b);
+        if (cnt >= 32) flush();
+      }
+    }
+    if (cnt) flush();
+    lp_tree(sh.list, best, warp, lane);
+  } else {
+    __syncthreads();
   }
   // CTA -> first CTA of the cluster (whose shared memory exists once every
   // CTA of the cluster has started)
-  if (C > 1) cl.sync();
-  if (warp == 0) {
-    st = sh.stat[0];
-    for (int w = 1; w < kLpWarps; ++w) st = lp_merge(st, sh.stat[w]);
-    LpShared* dst = cl.map_shared_rank(&sh, 0);
-    if (lane == 0) dst->peer_stat[rank] = st;
-    if constexpr (TOP) dst->peer[rank][lane] = best;
-  }
-  if (C > 1) cl.sync();
-  if (rank != 0 || warp != 0) return;
-  __syncwarp();
-  st = sh.peer_stat[0];
-  for (uint32_t r = 1; r < C; ++r) st = lp_merge(st, sh.peer_stat[r]);
-  if constexpr (TOP) {
-    best = sh.peer[0][lane];
-    for (uint32_t r = 1; r < C; ++r) best = lp_merge32(best, sh.peer[r][lane], lane);
+  if (C > 1) {
+    cl.sync();
+    if (warp == 0) {
+      st = lp_warp_merge<kLpWarps>(sh.stat[lane % kLpWarps]);
+      auto* dst = cl.map_shared_rank(&sh, 0);
+      if (lane == 0) dst->peer_stat[rank] = st;
+      if constexpr (TOP) dst->peer[rank][lane] = best;
+    }
+    cl.sync();
+    if (rank != 0) return;
+    if constexpr (TOP) {
+      best = 0;
+      for (uint32_t r = warp; r < C; r += kLpWarps) best = lp_merge32(best, sh.peer[r][lane], lane);
+      lp_tree(sh.list, best, warp, lane);
+    }
+    if (warp != 0) return;
+    st = (uint32_t)lane % kLpMaxCluster < C ? sh.peer_stat[lane % kLpMaxCluster] : LpStat{-INFINITY, 0.f, 0.f};
+    st = lp_warp_merge<(int)kLpMaxCluster>(st);
+  } else {
+    if (warp != 0) return;
+    st = lp_warp_merge<kLpWarps>(sh.stat[lane % kLpWarps]);
   }
   const float ls = logf(st.s);
   // a row with nothing allowed: every log probability -infinity, entropy 0

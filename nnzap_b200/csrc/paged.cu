@@ -37,18 +37,35 @@ __global__ void rope_table_kernel(double l2theta, uint32_t half, uint32_t positi
 // y = x * rsqrt(mean(x^2) + eps) * w over one head, then each pair (a, b) ->
 // (a cos - b sin, a sin + b cos); pairs are (2i, 2i + 1) or (i, i + HD / 2).
 // Bound by bytes: every head is read and written once in 16-byte chunks, HD /
-// 8 lanes to a head, f32 arithmetic, one rounding.  One CTA per token: its
-// heads share the token's table row, which each lane keeps in registers.
+// 8 lanes to a head, f32 arithmetic, one rounding.  One CTA of 4 warps per
+// token; a thread asks for all its chunks (up to kNrUnroll) before it waits
+// for the position, the table row that depends on it, or the slot, so a CTA
+// pays two memory latencies and the 8 CTAs of an SM keep 128 KB in flight.
+constexpr int kNrThreads = 128, kNrUnroll = 4;
+
 template <typename T, int HD, int STYLE>
-__global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs a) {
+__global__ void __launch_bounds__(kNrThreads, 8) norm_rope_kernel(const NormRopeArgs a) {
   constexpr int LPH = HD / 8;                          // lanes per head
   constexpr int NCS = STYLE == ROPE_PAIRWISE ? 4 : 8;   // (cos, sin) of a lane's 8 elements
+  constexpr uint32_t HPS = kNrThreads / LPH;            // heads per step of the CTA
   const uint32_t tok = blockIdx.x;
-  const uint32_t hl = threadIdx.x % LPH, hg = threadIdx.x / LPH, ngrp = blockDim.x / LPH;
+  const uint32_t hl = threadIdx.x % LPH, hg = threadIdx.x / LPH;
   const uint32_t n_kv = a.kv.n_kv, heads = a.n_q + 2 * n_kv;
   const uint4* src = reinterpret_cast<const uint4*>(a.qkv + (int64_t)tok * a.qkv_stride);
+  uint4 u[kNrUnroll];
+#pragma unroll
+  for (int i = 0; i < kNrUnroll; ++i) {
+    const uint32_t h = hg + i * HPS;
+    u[i] = h < heads ? __ldcs(src + h * LPH + hl) : make_uint4(0u, 0u, 0u, 0u);
+  }
   const int pos = a.positions[tok];
   const long long slot = a.slots[tok];
+  float4 wq[2], wk[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    wq[i] = __ldg(reinterpret_cast<const float4*>(a.q_norm + hl * 8) + i);
+    wk[i] = __ldg(reinterpret_cast<const float4*>(a.k_norm + hl * 8) + i);
+  }
   const bool bad_pos = pos < 0 || (uint32_t)pos >= a.table_positions;
   const bool bad_slot = slot >= (long long)a.kv.num_pages * a.kv.page_size;
   const bool bad = bad_pos || bad_slot;
@@ -65,56 +82,66 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs a) {
     const long long pg = slot / a.kv.page_size;
     page_off = pg * a.kv.page_stride + (slot - pg * a.kv.page_size) * a.kv.token_stride;
   }
-  for (uint32_t h0 = 0; h0 < heads; h0 += ngrp) {
-    const uint32_t h = h0 + hg;
-    const bool live = h < heads;
-    uint4 u = live ? src[h * LPH + hl] : make_uint4(0u, 0u, 0u, 0u);
-    // every lane takes the shuffles (value heads too: their result is not used)
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    float x[8], ss = 0.f;
+  for (uint32_t h0 = 0; h0 < heads; h0 += kNrUnroll * HPS) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = T16<T>::to_f2(w[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-      ss = fmaf(f.x, f.x, ss);
-      ss = fmaf(f.y, f.y, ss);
-    }
+    for (int i = 0; i < kNrUnroll; ++i) {
+      const uint32_t h = h0 + i * HPS + hg;
+      if (h0 + i * HPS >= heads) break;               // the same for every thread
+      const bool live = h < heads;
+      // every lane takes the shuffles (value heads too: their result is not used)
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+      float x[8], ss = 0.f;
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss / (float)HD + a.eps);
-    const float4* nw = reinterpret_cast<const float4*>((h < a.n_q ? a.q_norm : a.k_norm) + hl * 8);
-    const float4 w0 = __ldg(nw), w1 = __ldg(nw + 1);
-    x[0] *= r * w0.x; x[1] *= r * w0.y; x[2] *= r * w0.z; x[3] *= r * w0.w;
-    x[4] *= r * w1.x; x[5] *= r * w1.y; x[6] *= r * w1.z; x[7] *= r * w1.w;
-    if constexpr (STYLE == ROPE_PAIRWISE) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = x[2 * i], q = x[2 * i + 1];
-        x[2 * i] = p * cs[i].x - q * cs[i].y;
-        x[2 * i + 1] = p * cs[i].y + q * cs[i].x;
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = T16<T>::to_f2(w[e]);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+        ss = fmaf(f.x, f.x, ss);
+        ss = fmaf(f.y, f.y, ss);
       }
-    } else {
-      // element i of the first half pairs with element i of the second,
-      // LPH / 2 lanes away
-      const bool second = hl >= LPH / 2;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = __shfl_xor_sync(0xffffffffu, x[i], LPH / 2);
-        x[i] = second ? other * cs[i].y + x[i] * cs[i].x : x[i] * cs[i].x - other * cs[i].y;
+      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss / (float)HD + a.eps);
+      const bool is_q = h < a.n_q;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4 nw = is_q ? wq[e] : wk[e];
+        x[4 * e] *= r * nw.x;
+        x[4 * e + 1] *= r * nw.y;
+        x[4 * e + 2] *= r * nw.z;
+        x[4 * e + 3] *= r * nw.w;
       }
-    }
-    if (h < a.n_q + n_kv)   // a query or key head
-      u = make_uint4(T16<T>::pack(x[0], x[1]), T16<T>::pack(x[2], x[3]), T16<T>::pack(x[4], x[5]),
-                     T16<T>::pack(x[6], x[7]));
-    if (h < a.n_q) {
-      if (bad) u = make_uint4(0u, 0u, 0u, 0u);
-      reinterpret_cast<uint4*>(a.q_out + (int64_t)tok * a.q_stride)[h * LPH + hl] = u;
-    } else if (live && !bad && slot >= 0) {
-      const bool is_k = h < a.n_q + n_kv;
-      const uint32_t kh = h - a.n_q - (is_k ? 0u : n_kv);
-      uint16_t* base = is_k ? a.kv.k : a.kv.v;
-      *reinterpret_cast<uint4*>(base + page_off + (int64_t)kh * a.kv.head_stride + hl * 8) = u;
+      if constexpr (STYLE == ROPE_PAIRWISE) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = x[2 * e], q = x[2 * e + 1];
+          x[2 * e] = p * cs[e].x - q * cs[e].y;
+          x[2 * e + 1] = p * cs[e].y + q * cs[e].x;
+        }
+      } else {
+        // element e of the first half pairs with element e of the second,
+        // LPH / 2 lanes away
+        const bool second = hl >= LPH / 2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float other = __shfl_xor_sync(0xffffffffu, x[e], LPH / 2);
+          x[e] = second ? other * cs[e].y + x[e] * cs[e].x : x[e] * cs[e].x - other * cs[e].y;
+        }
+      }
+      uint4 y = u[i];
+      if (h < a.n_q + n_kv)   // a query or key head
+        y = make_uint4(T16<T>::pack(x[0], x[1]), T16<T>::pack(x[2], x[3]), T16<T>::pack(x[4], x[5]), T16<T>::pack(x[6], x[7]));
+      if (is_q) {
+        if (bad) y = make_uint4(0u, 0u, 0u, 0u);
+        reinterpret_cast<uint4*>(a.q_out + (int64_t)tok * a.q_stride)[h * LPH + hl] = y;
+      } else if (live && !bad && slot >= 0) {
+        const bool is_k = h < a.n_q + n_kv;
+        const uint32_t kh = h - a.n_q - (is_k ? 0u : n_kv);
+        uint16_t* base = is_k ? a.kv.k : a.kv.v;
+        *reinterpret_cast<uint4*>(base + page_off + (int64_t)kh * a.kv.head_stride + hl * 8) = y;
+      }
+      const uint32_t hn = h + kNrUnroll * HPS;
+      if (hn < heads) u[i] = __ldcs(src + hn * LPH + hl);
     }
   }
 }
@@ -380,8 +407,8 @@ cudaError_t rope_table_launch(float theta, uint32_t hd, uint32_t positions, floa
 
 template <typename T, int HD>
 static cudaError_t norm_rope_t(const NormRopeArgs& a, cudaStream_t st) {
-  if (a.rope_style == ROPE_PAIRWISE) norm_rope_kernel<T, HD, ROPE_PAIRWISE><<<a.tokens, 256, 0, st>>>(a);
-  else norm_rope_kernel<T, HD, ROPE_HALF_SPLIT><<<a.tokens, 256, 0, st>>>(a);
+  if (a.rope_style == ROPE_PAIRWISE) norm_rope_kernel<T, HD, ROPE_PAIRWISE><<<a.tokens, kNrThreads, 0, st>>>(a);
+  else norm_rope_kernel<T, HD, ROPE_HALF_SPLIT><<<a.tokens, kNrThreads, 0, st>>>(a);
   return cudaGetLastError();
 }
 

@@ -31,8 +31,14 @@ _DTYPES = {torch.float16: capi.NNZ_DT_F16, torch.bfloat16: capi.NNZ_DT_BF16, tor
 _ROPE = {"pairwise": capi.NNZ_ROPE_PAIRWISE, "half_split": capi.NNZ_ROPE_HALF_SPLIT}
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(device: int | None = None) -> int:
+    """The current stream's handle (the raw query skips building a Stream object, about a microsecond)."""
+    if _raw_stream is not None and device is not None:
+        return _raw_stream(device)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _need(ok: bool, what: str) -> None:
@@ -67,7 +73,7 @@ class PagedKV:
         _need(k.is_cuda and k.device == v.device, "pages must be on one CUDA device")
         _need(k.stride() == v.stride() and k.stride(3) == 1, "k and v pages need equal strides and adjacent elements")
         self.k, self.v = k, v
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.index = k.dtype, k.device, k.device.index
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         c = capi.NnzPagedKv()
         c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype]
@@ -123,7 +129,7 @@ class QKNormRope:
         a.positions = _index(positions, torch.int32, (n,), kv.device, "positions")
         a.slots = _index(slots, torch.int64, (n,), kv.device, "slots")
         a.qkv, a.q_out, a.tokens = qkv.data_ptr(), out.data_ptr(), n
-        rc = self._fn(kv._ref, self._ref, _stream())
+        rc = self._fn(kv._ref, self._ref, _stream(kv.index))
         if rc:
             check(rc)
         return out
@@ -162,7 +168,7 @@ class PagedAttention:
         a.page_table = _index(page_table, torch.int32, (seqs, page_table.shape[1]), kv.device, "page_table")
         a.table_stride = page_table.shape[1]
         a.q, a.out, a.tokens, a.num_seqs, a.max_new = q.data_ptr(), out.data_ptr(), n, seqs, max_new
-        rc = self._fn(kv._ref, self._ref, _stream())
+        rc = self._fn(kv._ref, self._ref, _stream(kv.index))
         if rc:
             check(rc)
         return out
@@ -194,20 +200,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     else:
         m = 1 if tokens.dim() == 1 else tokens.shape[1]
         a.tokens = _index(tokens, torch.int32, (rows,) if tokens.dim() == 1 else (rows, m), dev, "tokens")
-    # one allocation for all outputs: logprob | entropy | logsumexp | top
-    f = torch.empty(rows * (m + 2 + 2 * top_k), dtype=torch.float32, device=dev)
-    p = f.data_ptr()
-    at = [0, rows * m, rows * (m + 1), rows * (m + 2), rows * (m + 2 + top_k)]
-    a.logits, a.dtype, a.rows, a.n, a.num_tokens, a.top_k = logits.data_ptr(), _DTYPES[logits.dtype], rows, n, m, top_k
+    f32 = {"dtype": torch.float32, "device": dev}
+    lp = None if tokens is None else torch.empty(tokens.shape, **f32)
+    ent, lse = torch.empty(rows, **f32), torch.empty(rows, **f32)
+    ids = top = None
+    if top_k:
+        ids, top = torch.empty((rows, top_k), dtype=torch.int32, device=dev), torch.empty((rows, top_k), **f32)
+        a.top_k, a.top_ids, a.top_logprobs = top_k, ids.data_ptr(), top.data_ptr()
+    if m:
+        a.num_tokens, a.logprob = m, lp.data_ptr()
+    a.logits, a.dtype, a.rows, a.n = logits.data_ptr(), _DTYPES[logits.dtype], rows, n
     a.stride = logits.stride(0) if rows > 1 else n
-    a.logprob, a.entropy, a.logsumexp = p, p + 4 * at[1], p + 4 * at[2]
-    a.top_ids, a.top_logprobs = p + 4 * at[3], p + 4 * at[4]
-    rc = lib().nnz_token_logprobs(C.byref(a), _stream())
+    a.entropy, a.logsumexp = ent.data_ptr(), lse.data_ptr()
+    rc = lib().nnz_token_logprobs(C.byref(a), _stream(dev.index))
     if rc:
         check(rc)
-    return TokenLogprobs(
-        f[:at[1]].view(tokens.shape) if tokens is not None else None, f[at[1]:at[2]], f[at[2]:at[3]],
-        f[at[3]:at[4]].view(torch.int32).view(rows, top_k) if top_k else None, f[at[4]:].view(rows, top_k) if top_k else None)
+    return TokenLogprobs(lp, ent, lse, ids, top)
 
 
 def stream_check() -> None:
