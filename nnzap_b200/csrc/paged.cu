@@ -338,6 +338,85 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a,
 
 }  // namespace
 
+namespace {
+
+// The tiled kernel's parts, [HD / 4][R][4]: a block takes 32 rows of one
+// split task, lane = row, a warp HD / 8 dims, so every load is 512 bytes in
+// a row and a lane's output whole sectors.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_merge_tile_kernel(const PagedAttnArgs a, const PartWs ws) {
+  constexpr int N4 = HD / 32;          // float4 per thread
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t G = a.n_q / a.kv.n_kv;
+  pdl_wait();
+  const PartHeader h = ws.head[blockIdx.x];
+  const uint32_t row = blockIdx.y * 32 + lane;
+  if (row >= h.rows || h.parts == 0) return;
+  float m = -INFINITY, l = 0.f, o[N4][4];
+#pragma unroll
+  for (int i = 0; i < N4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  for (uint32_t k0 = 0; k0 < h.parts; k0 += 2) {
+    float pm[2], pl[2];
+    float4 po[2][N4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t k = k0 + j;
+      pm[j] = -INFINITY;
+      pl[j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < N4; ++i) po[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < h.parts) {
+        const float* p = ws.slot((uint64_t)blockIdx.x + k, k == 0 ? 1 : 0, HD);
+        pm[j] = __ldcg(p + row);
+        pl[j] = __ldcg(p + ws.R + row);
+        const float4* q = reinterpret_cast<const float4*>(p + 2 * ws.R) + row;
+#pragma unroll
+        for (int i = 0; i < N4; ++i) po[j][i] = __ldcg(q + (size_t)(warp * N4 + i) * ws.R);
+      }
+    }
+    const float mn = fmaxf(m, fmaxf(pm[0], pm[1]));
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    const float c = exp2f(m - ms), f0 = exp2f(pm[0] - ms), f1 = exp2f(pm[1] - ms);
+    m = mn;
+    l = l * c + f0 * pl[0] + f1 * pl[1];
+#pragma unroll
+    for (int i = 0; i < N4; ++i) {
+      o[i][0] = o[i][0] * c + f0 * po[0][i].x + f1 * po[1][i].x;
+      o[i][1] = o[i][1] * c + f0 * po[0][i].y + f1 * po[1][i].y;
+      o[i][2] = o[i][2] * c + f0 * po[0][i].z + f1 * po[1][i].z;
+      o[i][3] = o[i][3] * c + f0 * po[0][i].w + f1 * po[1][i].w;
+    }
+  }
+  const float il = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* op = a.out + ((int64_t)h.row0 + row / G) * a.out_stride + ((int64_t)h.kvh * G + row % G) * HD + warp * N4 * 4;
+#pragma unroll
+  for (int i = 0; i < N4; i += 2)
+    *reinterpret_cast<uint4*>(op + 4 * i) = make_uint4(T16<T>::pack(o[i][0] * il, o[i][1] * il), T16<T>::pack(o[i][2] * il, o[i][3] * il),
+                                                       T16<T>::pack(o[i + 1][0] * il, o[i + 1][1] * il),
+                                                       T16<T>::pack(o[i + 1][2] * il, o[i + 1][3] * il));
+}
+
+}  // namespace
+
+cudaError_t paged_merge_tile_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(workers, (ws.R + 31) / 32);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (dtype == RD_F16)
+    return hd == 128 ? cudaLaunchKernelEx(&cfg, &paged_merge_tile_kernel<__half, 128>, a, ws)
+                     : cudaLaunchKernelEx(&cfg, &paged_merge_tile_kernel<__half, 64>, a, ws);
+  return hd == 128 ? cudaLaunchKernelEx(&cfg, &paged_merge_tile_kernel<__nv_bfloat16, 128>, a, ws)
+                   : cudaLaunchKernelEx(&cfg, &paged_merge_tile_kernel<__nv_bfloat16, 64>, a, ws);
+}
+
 cudaError_t paged_merge_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   const uint32_t span = std::max(1u, workers / (uint32_t)a.num_sms);

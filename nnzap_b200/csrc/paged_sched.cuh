@@ -207,7 +207,8 @@ struct PartHeader {
   uint32_t parts;   // 0: the worker holds no first part of a split task
 };
 
-// One slot: R maxima (log2 domain), R sums, R x HD sums of p v.
+// One slot: R maxima (log2 domain), R sums, R x HD sums of p v (row by row
+// from the streaming kernel, [HD / 4][R][4] from the tiled one).
 __host__ __device__ constexpr size_t slot_floats(uint32_t R, uint32_t hd) { return (size_t)R * (hd + 2); }
 
 struct PartWs {
@@ -230,6 +231,7 @@ inline PartWs part_ws(void* ws, uint32_t workers, uint32_t R) {
 // Merges the parts of split tasks into the output (paged.cu); launched with
 // programmatic dependent launch behind the kernel that left them.
 cudaError_t paged_merge_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st);
+cudaError_t paged_merge_tile_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st);
 
 // Few query rows per kv head and sequence (at most 16): keys streamed by
 // independent warps (paged_stream.cu).

@@ -11,17 +11,20 @@
 //                       the pool's type over the S it came from
 //   O += P V            tcgen05.mma, P from TMEM, V as stored (MN-major B)
 // so while one row tile's softmax runs, the tensor cores work for the other.
-// m lags behind the running maximum by up to 2^8 (a row's O is rescaled only
-// when the maximum has grown by more, which after the first tiles is rare): P
-// up to 256 costs no precision, the sums are f32.
+// m lags behind the running maximum: a unit's P is computed with the m that
+// the row has, in one pass over S, and only if a score turns out to be more
+// than 8 (in log2) above it does the row take its new maximum, rescale O and
+// compute the unit again, which after the first units is rare.  P up to 256
+// costs no precision, the sums are f32.  Units at the diagonal, at the end or
+// with absent pages take two passes and masks.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (thread =
 // TMEM lane = row), warp 8 TMA (Q, then K and V tiles into one ring, boxes of
 // one page each, one per lane), warp 9 MMA issue, warp 10 walks the
-// run of units and hands out its parts (11 only makes the third warpgroup
-// whole).  Boxes of absent pages and
-// past the length are loaded from beyond the pool's last page: the copy
-// engine fills them with zeros, so no stale byte meets the product.
+// run of units and hands out its parts, warp 11 cleans the V tiles at the
+// diagonal and at the end.  Boxes of absent pages and past the length are
+// loaded from beyond the pool's last page: the copy engine fills them with
+// zeros, so no stale byte meets the product.
 //
 // TMEM: S / P of the two row tiles at columns 0 and 128, O at 256 and 384.
 #include <cuda_runtime.h>
@@ -40,10 +43,10 @@ namespace {
 
 constexpr int kUmKeys = 128;
 constexpr int kUmThreads = 384;
-// Registers a thread: 384 x 168 at launch; the two softmax warpgroups take 208
-// each (a row of S stays in registers), the third goes down to 80: 2 x 128 x
-// 208 + 128 x 80 = 63488 of 64512.
-constexpr int kUmRegsSoftmax = 208, kUmRegsIssue = 80;
+// Registers a thread: 384 x 168 at launch; the two softmax warpgroups take 216
+// each (a unit's P and two quarters of S), the third goes down to 72: 2 x 128
+// x 216 + 128 x 72 = 64512.
+constexpr int kUmRegsSoftmax = 216, kUmRegsIssue = 72;
 constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
 constexpr int kPres = 8;                          // units whose page masks are kept
@@ -55,7 +58,7 @@ struct UmShape {
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr uint32_t OFF_KV = 2 * kTileB;
   static constexpr uint32_t OFF_BAR = OFF_KV + kStages * kTileB;
-  static constexpr int kBars = 2 * kStages + 8 + kPres + 2 * kSegs;
+  static constexpr int kBars = 2 * kStages + 8 + 2 * kPres + 2 * kSegs;
   static constexpr uint32_t OFF_MISC = OFF_BAR + kBars * 8;
   static constexpr uint32_t kSmem = OFF_MISC + 128 + kSegs * 128 + 1024;
 };
@@ -116,6 +119,94 @@ __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// Two f32 at a time (one instruction each).
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+
+// Which keys of a unit a row sees: the first `end`, on pages whose bit is set
+// (one bit per 2^sh keys).
+struct KeyMask {
+  int end;
+  uint32_t bits, sh;
+  __device__ __forceinline__ bool operator()(int e) const { return e < end && ((bits >> (e >> sh)) & 1u); }
+};
+
+// Sets the scores of a row's 128 keys that it does not see to -infinity, in
+// TMEM, and returns the largest of the others.  (Rolled: this runs a few times
+// per task, and instructions have to be fetched.)
+__device__ __forceinline__ float um_mask(uint32_t tS, const KeyMask& see) {
+  float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t v[32];
+    tm_ld32(tS + 32 * c, v);
+    tm_wait_ld(v);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      v[e] = see(32 * c + e) ? v[e] : 0xFF800000u;
+      mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(v[e]));
+    }
+    tmem_st32(tS + 32 * c, v);
+  }
+  return fmaxf(mx[0], mx[1]);
+}
+
+// P = 2^(S sl2 - ms) of a row's 128 keys as 64 words of the pool's type, their
+// f32 sum, and the largest score.  The next quarter of S is on its way while
+// one is worked on.
+template <typename T>
+__device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32_t (&w)[64], float& sum, float& top) {
+  const uint64_t k2 = pair2(sl2, sl2), m2 = pair2(-ms, -ms);
+  uint64_t acc[2] = {0ull, 0ull};
+  float mx[2] = {-INFINITY, -INFINITY};
+  uint32_t v[2][32];
+  tm_ld32(tS, v[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tm_wait_ld(v[c & 1]);
+    if (c < 3) tm_ld32(tS + 32 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float a = __uint_as_float(v[c & 1][e]), b = __uint_as_float(v[c & 1][e + 1]);
+      mx[(e >> 1) & 1] = fmaxf(fmaxf(mx[(e >> 1) & 1], a), b);
+      const float2 y = split2(fma2(pair2(a, b), k2, m2));
+      const float p0 = ex2(y.x), p1 = ex2(y.y);
+      acc[(e >> 1) & 1] = add2(acc[(e >> 1) & 1], pair2(p0, p1));
+      w[16 * c + e / 2] = T16<T>::pack(p0, p1);
+    }
+  }
+  const float2 t = split2(add2(acc[0], acc[1]));
+  sum = t.x + t.y;
+  top = fmaxf(mx[0], mx[1]);
+}
+
+// One lane of the warp, known as such to the compiler: behind a plain test of
+// the lane it takes every tcgen05.mma for divergent code (S: 900 -> 585 cycles
+// for its 8 instructions, P V: 1900 -> 700).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
 }
 
 template <bool BF16>
@@ -187,9 +278,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint64_t* s_full = q_empty + 1;        // [2] S of a row tile complete
   uint64_t* p_full = s_full + 2;         // [2] P written, O rescaled (4 warps)
   uint64_t* pv_done = p_full + 2;        // [2] P V complete
-  uint64_t* pres_full = pv_done + 2;     // [kPres] page mask of a unit written
+  uint64_t* v_ready = pv_done + 2;       // [kPres] a unit's V tile is ready for the product
+  uint64_t* pres_full = v_ready + kPres; // [kPres] page mask of a unit written
   uint64_t* seg_full = pres_full + kPres;   // [kSegs]
-  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 10 other warps are done with it
+  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 11 other warps are done with it
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + S::OFF_MISC);
   volatile uint32_t* pres = tslot + 1;   // [kPres] one bit per box of the unit: page present
   Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_MISC + 128);
@@ -198,7 +290,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
+      mbar_init(kv_empty + i, 2);     // the products and warp 11
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -207,10 +299,13 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       mbar_init(p_full + i, 4);
       mbar_init(pv_done + i, 1);
     }
-    for (int i = 0; i < kPres; ++i) mbar_init(pres_full + i, 1);
+    for (int i = 0; i < kPres; ++i) {
+      mbar_init(v_ready + i, 1);
+      mbar_init(pres_full + i, 1);
+    }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(seg_full + i, 1);
-      mbar_init(seg_empty + i, 10);
+      mbar_init(seg_empty + i, 11);
     }
     fence_barrier_init();
   }
@@ -314,9 +409,9 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   } else if (warp == 9) {
     // ---------------- MMA ----------------
     constexpr uint32_t id_s = um_idesc<BF>(128, 128), id_o = um_idesc<BF>(128, HD) | (1u << 16);
-    uint32_t stage_use = 0, np[2] = {0, 0};
+    uint32_t stage_use = 0, np[2] = {0, 0}, unit_no = 0;
     auto issue_s = [&](int x, uint32_t st) {
-      if (lane == 0) {
+      if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
           const uint64_t da = smem_desc_sw128(sm + x * S::kTileB + h * kHalfB);
@@ -329,7 +424,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       __syncwarp();
     };
     auto issue_o = [&](int x, uint32_t st, bool acc) {
-      if (lane == 0) {
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kUmKeys / 16; ++kk)
           umma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, smem_desc_sw128_mn(sm + S::OFF_KV + st * S::kTileB + kk * 16 * 128), id_o,
@@ -339,11 +434,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       __syncwarp();
     };
     auto release = [&](uint64_t* bar) {
-      if (lane == 0) umma_commit(bar);
+      if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
     for (uint32_t seg = 0; segment(seg, g); ++seg) {
-      const int seen_all = g.seen(0), seen_any = g.seen(g.rows - 1);
       wait(q_full, seg);
       for (uint32_t i = 0; i <= g.take; ++i) {
         // K of unit i, V of unit i - 1 (the ring holds K0 V0 K1 V1 ...)
@@ -352,33 +446,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         if (i < g.take) wait(kv_full + ks, ku / S::kStages);
         if (i > 0) {
           wait(kv_full + vs, vu / S::kStages);
-          const int key0 = (int)((g.unit + i - 1) * kUmKeys);
-          if (key0 + kUmKeys > seen_all) {
-            // Keys that not every row sees: a V row past the length is zeroed
-            // (its box holds earlier keys), and so is every non-finite element
-            // of the others, or 0 * V would reach the rows that do not see it;
-            // the epilogue adds it to those that do.
-            const int base = max(0, seen_any - 256);   // key of the first mark
-            for (int e = lane; e < kUmKeys * HD / 8; e += 32) {
-              const int r = e / (HD / 8), ch = e % (HD / 8);
-              uint8_t* p = sm + S::OFF_KV + vs * S::kTileB + (ch >> 3) * kHalfB + sw128_off((uint32_t)r, (uint32_t)(ch & 7));
-              uint4* p4 = reinterpret_cast<uint4*>(p);
-              if (key0 + r >= seen_any) {
-                *p4 = make_uint4(0u, 0u, 0u, 0u);
-              } else if (key0 + r >= seen_all) {
-                uint4 w = *p4;
-                const uint32_t b0 = bad_mask<BF>(w.x), b1 = bad_mask<BF>(w.y), b2 = bad_mask<BF>(w.z), b3 = bad_mask<BF>(w.w);
-                if (b0 | b1 | b2 | b3) {
-                  *p4 = make_uint4(w.x & ~b0, w.y & ~b1, w.z & ~b2, w.w & ~b3);
-                  const uint32_t bit = (uint32_t)(key0 + r - base);
-                  atomicOr(segs[seg % kSegs].marks + (bit >> 5), 1u << (bit & 31));
-                }
-              }
-            }
-            fence_async_smem();
-            __threadfence_block();
-            __syncwarp();
-          }
+          wait(v_ready + unit_no % kPres, unit_no / kPres);   // warp 11 has seen to it
+          ++unit_no;
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -444,6 +513,50 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       }
       if (o.take == 0 || failed) break;
     }
+  } else {
+    // ---------------- V tiles with keys that not every row sees ----------------
+    // A V row past the length is zeroed (its box holds earlier keys), and so is
+    // every non-finite element of a row that some rows see and others do not,
+    // or 0 * V would reach the others; the epilogue adds it to those that do.
+    uint32_t stage_use = 0, unit_no = 0;
+    for (uint32_t seg = 0; segment(seg, g); ++seg) {
+      const int seen_all = g.seen(0), seen_any = g.seen(g.rows - 1);
+      const int base = max(0, seen_any - 256);   // key of the first mark
+      for (uint32_t i = 0; i < g.take; ++i) {
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv, ++stage_use) {
+          const uint32_t st = stage_use % S::kStages;
+          wait(kv_full + st, stage_use / S::kStages);
+          const int key0 = (int)((g.unit + i) * kUmKeys);
+          if (kv && key0 + kUmKeys > seen_all) {
+            const int r0 = max(0, seen_all - key0);
+            constexpr int CH = HD / 8;           // 16-byte chunks of a row
+#pragma unroll 4
+            for (int e = r0 * CH + lane; e < kUmKeys * CH; e += 32) {
+              const int r = e / CH, ch = e % CH;
+              uint4* p4 = reinterpret_cast<uint4*>(sm + S::OFF_KV + st * S::kTileB + (ch >> 3) * kHalfB + sw128_off((uint32_t)r, (uint32_t)(ch & 7)));
+              const bool gone = key0 + r >= seen_any;
+              const uint4 w = *p4;
+              const uint32_t b0 = bad_mask<BF>(w.x), b1 = bad_mask<BF>(w.y), b2 = bad_mask<BF>(w.z), b3 = bad_mask<BF>(w.w);
+              const bool bad = (b0 | b1 | b2 | b3) != 0;
+              if (gone || bad) *p4 = gone ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w.x & ~b0, w.y & ~b1, w.z & ~b2, w.w & ~b3);
+              if (bad && !gone) {
+                const uint32_t bit = (uint32_t)(key0 + r - base);
+                atomicOr(segs[seg % kSegs].marks + (bit >> 5), 1u << (bit & 31));
+              }
+            }
+            fence_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) {
+            if (kv) mbar_arrive1(v_ready + unit_no % kPres);
+            mbar_arrive1(kv_empty + st);
+          }
+        }
+        ++unit_no;
+      }
+      segment_done(seg);
+    }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUmRegsSoftmax));
@@ -467,67 +580,47 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         tc_fence_after();
         wait(pres_full + un % kPres, un / kPres);   // written before the unit's K was asked for
         const uint32_t mask = pres[un % kPres];
-        float s[128];
-        {
-          uint32_t v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tm_ld32(tS + 32 * c, v[c]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tm_wait_ld(v[c]);
-#pragma unroll
-          for (int e = 0; e < 128; ++e) s[e] = __uint_as_float(v[e >> 5][e & 31]);
-        }
         const int key0 = (int)((g.unit + i) * kUmKeys);
-        const bool all_there = mask == (1u << (kUmKeys / t.box)) - 1u;
-        if (!all_there || key0 + kUmKeys > seen_all) {
-          const uint32_t sh = 31 - __clz(t.box);
-          const int end = limit - key0;
-#pragma unroll
-          for (int e = 0; e < 128; ++e) {
-            const bool ok = e < end && ((mask >> (e >> sh)) & 1u);
-            s[e] = ok ? s[e] : -INFINITY;
-          }
+        const bool masked = mask != (1u << (kUmKeys / t.box)) - 1u || key0 + kUmKeys > seen_all;
+        uint32_t w[64];
+        float sum, top = -INFINITY;
+        bool again = masked || i == 0;      // the maximum first
+        if (again) {
+          const KeyMask see{masked ? limit - key0 : kUmKeys, masked ? mask : 0xFFFFFFFFu, (uint32_t)(31 - __clz(t.box))};
+          top = um_mask(tS, see) * t.sl2;
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * t.sl2;
-        // (top is NaN only for a row whose scores are: then so is its result)
-        const bool grow = top > m + kLag;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float mn = grow ? top : m;
-          const float f = m == -INFINITY ? 0.f : ex2(m - mn);
-          l *= f;
-          m = mn;
-          if (i > 0) {
-            wait(pv_done + x, ns - 1);
-            tc_fence_after();
+        for (;;) {
+          if (again) {
+            // (NaN scores are no maximum; they make the row's sum NaN)
+            const bool grow = live && top > m + kLag;
+            if (__any_sync(0xffffffffu, grow)) {
+              const float mn = grow ? top : m;
+              const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+              l *= f;
+              m = mn;
+              if (i > 0) {
+                wait(pv_done + x, ns - 1);
+                tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t w[32];
-              tm_ld32(tO + 32 * c, w);
-              tm_wait_ld(w);
+                for (int c = 0; c < HD / 32; ++c) {
+                  uint32_t o[32];
+                  tm_ld32(tO + 32 * c, o);
+                  tm_wait_ld(o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
-              tmem_st32(tO + 32 * c, w);
+                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st32(tO + 32 * c, o);
+                }
+              }
             }
           }
+          um_pass<T>(tS, t.sl2, m == -INFINITY ? 0.f : m, w, sum, top);
+          top *= t.sl2;
+          if (again || !__any_sync(0xffffffffu, live && top > m + kLag)) break;
+          again = true;
         }
-        const float ms = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float p0 = ex2(fmaf(s[64 * c + 2 * e], t.sl2, -ms)), p1 = ex2(fmaf(s[64 * c + 2 * e + 1], t.sl2, -ms));
-            sum[e & 1] += p0;
-            sum[2 + (e & 1)] += p1;
-            w[e] = T16<T>::pack(p0, p1);
-          }
-          tmem_st32(tS + 32 * c, w);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += sum;
+        tmem_st32(tS, reinterpret_cast<uint32_t(&)[32]>(w[0]));
+        tmem_st32(tS + 32, reinterpret_cast<uint32_t(&)[32]>(w[32]));
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive1(p_full + x);
@@ -540,7 +633,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         const uint32_t rr = (uint32_t)x * PT * G + r;
         uint16_t* op = a.out + (int64_t)(g.row0 + tok) * a.out_stride + (int64_t)(g.kvh * G + r % G) * HD;
         float* slot = t.ws.slot(blockIdx.x, first ? 1 : 0, HD);
-        float* part = slot + 2 * t.ws.R + (size_t)rr * HD;
+        float* part = slot + 2 * t.ws.R + (size_t)rr * 4;   // [HD / 4][R][4]: lanes side by side
         if (live && !whole) {
           slot[rr] = m;
           slot[t.ws.R + rr] = l;
@@ -572,7 +665,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
                                                                       T16<T>::pack(o[d + 4], o[d + 5]), T16<T>::pack(o[d + 6], o[d + 7]));
           } else if (live) {
 #pragma unroll
-            for (int d = 0; d < 32; d += 4) *reinterpret_cast<float4*>(part + 32 * c + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+            for (int d = 0; d < 32; d += 4)
+              *reinterpret_cast<float4*>(part + (size_t)(32 * c + d) * t.ws.R) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
           }
         }
         tc_fence_before();
@@ -619,7 +713,7 @@ cudaError_t paged_umma_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStr
   if (dtype == RD_F16) e = hd == 128 ? umma_go<__half, 128>(t, st) : umma_go<__half, 64>(t, st);
   else e = hd == 128 ? umma_go<__nv_bfloat16, 128>(t, st) : umma_go<__nv_bfloat16, 64>(t, st);
   if (e != cudaSuccess) return e;
-  return paged_merge_launch(a, t.ws, t.workers, dtype, hd, st);
+  return paged_merge_tile_launch(a, t.ws, t.workers, dtype, hd, st);
 }
 
 }  // namespace nnz
