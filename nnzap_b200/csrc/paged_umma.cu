@@ -11,12 +11,12 @@
 //                       the pool's type over the S it came from
 //   O += P V            tcgen05.mma, P from TMEM, V as stored (MN-major B)
 // so while one row tile's softmax runs, the tensor cores work for the other.
-// m lags behind the running maximum: a unit's P is computed with the m that
-// the row has, in one pass over S, and only if a score turns out to be more
-// than 8 (in log2) above it does the row take its new maximum, rescale O and
-// compute the unit again, which after the first units is rare.  P up to 256
-// costs no precision, the sums are f32.  Units at the diagonal, at the end or
-// with absent pages take two passes and masks.
+// m only follows the row's maximum from afar: it starts at 0, a unit's P is
+// computed with the m that the row has, in one pass over S, and only if a
+// score turns out to be more than 8 (in log2) above it (in the row's first
+// unit also: the maximum more than 4 below) does the row take its maximum for
+// m, rescale O and compute the unit again, which after the first units is
+// rare.  P up to 256 costs no precision, the sums are f32.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (thread =
 // TMEM lane = row), warp 8 TMA (Q, then K and V tiles into one ring, boxes of
@@ -50,7 +50,7 @@ constexpr int kUmRegsSoftmax = 216, kUmRegsIssue = 72;
 constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
 constexpr int kPres = 8;                          // units whose page masks are kept
-constexpr float kLag = 8.f;                       // log2 of the largest P
+constexpr float kLag = 8.f, kUnder = 4.f;         // how far (log2) a row's maximum may lie above / at first below its m
 
 template <int HD>
 struct UmShape {
@@ -115,6 +115,17 @@ __device__ __forceinline__ void tm_wait_ld(uint32_t (&v)[32]) {
   asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
                     "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
+// 32 columns of this thread's TMEM lane; complete after tcgen05.wait::st.
+__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+      "r"(v[31])
+      : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -143,32 +154,29 @@ __device__ __forceinline__ float2 split2(uint64_t a) {
   return r;
 }
 
-// Which keys of a unit a row sees: the first `end`, on pages whose bit is set
-// (one bit per 2^sh keys).
-struct KeyMask {
-  int end;
-  uint32_t bits, sh;
-  __device__ __forceinline__ bool operator()(int e) const { return e < end && ((bits >> (e >> sh)) & 1u); }
-};
-
 // Sets the scores of a row's 128 keys that it does not see to -infinity, in
-// TMEM, and returns the largest of the others.  (Rolled: this runs a few times
-// per task, and instructions have to be fetched.)
-__device__ __forceinline__ float um_mask(uint32_t tS, const KeyMask& see) {
-  float mx[2] = {-INFINITY, -INFINITY};
+// TMEM: it sees the first `end`, on pages whose bit is set (one bit per 2^sh
+// keys).  (Rolled: this runs a few times per task, and instructions have to
+// be fetched.)
+__device__ __forceinline__ void um_mask(uint32_t tS, int end, uint32_t bits, uint32_t sh) {
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
+    uint32_t see = end >= 32 * c + 32 ? 0xFFFFFFFFu : end <= 32 * c ? 0u : (1u << (end - 32 * c)) - 1u;
+    const uint32_t pg = bits >> ((32 * c) >> sh);          // first page bit of this quarter
+    if (sh >= 5) {
+      if (!(pg & 1u)) see = 0;
+    } else {
+      for (int e = 0; e < 32; e += 1 << sh)
+        if (!((pg >> (e >> sh)) & 1u)) see &= ~(((1u << (1 << sh)) - 1u) << e);
+    }
+    if (__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) continue;
     uint32_t v[32];
     tm_ld32(tS + 32 * c, v);
     tm_wait_ld(v);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      v[e] = see(32 * c + e) ? v[e] : 0xFF800000u;
-      mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(v[e]));
-    }
+    for (int e = 0; e < 32; ++e) v[e] = (see >> e) & 1u ? v[e] : 0xFF800000u;
     tmem_st32(tS + 32 * c, v);
   }
-  return fmaxf(mx[0], mx[1]);
 }
 
 // P = 2^(S sl2 - ms) of a row's 128 keys as 64 words of the pool's type, their
@@ -194,6 +202,10 @@ __device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32
       acc[(e >> 1) & 1] = add2(acc[(e >> 1) & 1], pair2(p0, p1));
       w[16 * c + e / 2] = T16<T>::pack(p0, p1);
     }
+    // the quarter's work stays before the wait for the next one
+    uint32_t* q = w + 16 * c;
+    asm volatile("" : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]), "+r"(q[8]),
+                      "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]));
   }
   const float2 t = split2(add2(acc[0], acc[1]));
   sum = t.x + t.y;
@@ -573,7 +585,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       const int limit = live ? g.seen(tok) : 0;
       const bool tile = x * PT < g.rows;
       const int seen_all = g.seen(x * PT);
-      float m = -INFINITY, l = 0.f;
+      float m = 0.f, l = 0.f, scale = 1.f;
       for (uint32_t i = 0; i < g.n[x]; ++i) {
         const uint32_t un = unit_no + i;
         wait(s_full + x, ns);
@@ -583,44 +595,41 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         const int key0 = (int)((g.unit + i) * kUmKeys);
         const bool masked = mask != (1u << (kUmKeys / t.box)) - 1u || key0 + kUmKeys > seen_all;
         uint32_t w[64];
-        float sum, top = -INFINITY;
-        bool again = masked || i == 0;      // the maximum first
-        if (again) {
-          const KeyMask see{masked ? limit - key0 : kUmKeys, masked ? mask : 0xFFFFFFFFu, (uint32_t)(31 - __clz(t.box))};
-          top = um_mask(tS, see) * t.sl2;
-        }
+        float sum, top;
+        if (masked) um_mask(tS, limit - key0, mask, 31 - __clz(t.box));
         for (;;) {
-          if (again) {
-            // (NaN scores are no maximum; they make the row's sum NaN)
-            const bool grow = live && top > m + kLag;
-            if (__any_sync(0xffffffffu, grow)) {
-              const float mn = grow ? top : m;
-              const float f = m == -INFINITY ? 0.f : ex2(m - mn);
-              l *= f;
-              m = mn;
-              if (i > 0) {
-                wait(pv_done + x, ns - 1);
-                tc_fence_after();
+          um_pass<T>(tS, t.sl2, m, w, sum, top);
+          top *= t.sl2;
+          // (NaN scores are no maximum; they make the row's sum NaN.)  The
+          // first unit's maximum may not lie far below m either, or P would
+          // leave the 16-bit type's normal range.
+          const bool off = live && (top > m + kLag || (l == 0.f && top < m - kUnder && top > -INFINITY));
+          if (!__any_sync(0xffffffffu, off)) break;
+          if (off) {
+            const float f = l == 0.f ? 1.f : ex2(m - top);   // nothing to rescale yet
+            m = top;
+            l *= f;
+            scale = f;
+          }
+          if (i > 0) {
+            wait(pv_done + x, ns - 1);
+            tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; ++c) {
-                  uint32_t o[32];
-                  tm_ld32(tO + 32 * c, o);
-                  tm_wait_ld(o);
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tm_ld32(tO + 32 * c, o);
+              tm_wait_ld(o);
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tmem_st32(tO + 32 * c, o);
-                }
-              }
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale);
+              tmem_st32(tO + 32 * c, o);
             }
           }
-          um_pass<T>(tS, t.sl2, m == -INFINITY ? 0.f : m, w, sum, top);
-          top *= t.sl2;
-          if (again || !__any_sync(0xffffffffu, live && top > m + kLag)) break;
-          again = true;
+          scale = 1.f;
         }
         l += sum;
-        tmem_st32(tS, reinterpret_cast<uint32_t(&)[32]>(w[0]));
-        tmem_st32(tS + 32, reinterpret_cast<uint32_t(&)[32]>(w[32]));
+        tm_st32(tS, w);
+        tm_st32(tS + 32, w + 32);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive1(p_full + x);
@@ -635,7 +644,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         float* slot = t.ws.slot(blockIdx.x, first ? 1 : 0, HD);
         float* part = slot + 2 * t.ws.R + (size_t)rr * 4;   // [HD / 4][R][4]: lanes side by side
         if (live && !whole) {
-          slot[rr] = m;
+          slot[rr] = l == 0.f ? -INFINITY : m;
           slot[t.ws.R + rr] = l;
         }
         if (first && !whole) hdr = {(uint32_t)g.row0, g.kvh, (uint32_t)g.rows * G, g.parts};
