@@ -54,10 +54,37 @@ __device__ __forceinline__ uint32_t tile_units(const SeqInfo& q, int qt, int QT,
   return k <= KT ? 1u : (uint32_t)((k + KT - 1) / KT);
 }
 
+// sum of floor((x i + y) / m) over i < n (Euclid on the lattice points).
+__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t x, uint32_t y) {
+  uint64_t sum = 0;
+  for (;;) {
+    if (x >= m) {
+      sum += (uint64_t)n * (n - 1) / 2 * (x / m);
+      x %= m;
+    }
+    if (y >= m) {
+      sum += (uint64_t)n * (y / m);
+      y %= m;
+    }
+    const uint64_t last = (uint64_t)x * n + y;
+    if (last < m) return sum;
+    n = (uint32_t)(last / m);
+    y = (uint32_t)(last % m);
+    const uint32_t t = m;
+    m = x;
+    x = t;
+  }
+}
+
 // Units of one kv head of one sequence.
 __device__ __forceinline__ uint64_t head_units(const SeqInfo& q, int QT, int KT) {
-  uint64_t u = 0;
-  for (int qt = 0; qt * QT < q.rows; ++qt) u += tile_units(q, qt, QT, KT);
+  const int tiles = (q.rows + QT - 1) / QT;
+  if (tiles <= 1) return tiles ? tile_units(q, 0, QT, KT) : 0;
+  const int64_t a0 = q.len - q.n + QT;       // keys that the first tile's last row sees
+  if (a0 >= 1 && q.len - q.n + q.rows <= q.cap && a0 + (int64_t)tiles * QT < (1ll << 31))
+    return floor_sum((uint32_t)tiles - 1, (uint32_t)KT, (uint32_t)QT, (uint32_t)a0 + KT - 1) + tile_units(q, tiles - 1, QT, KT);
+  uint64_t u = 0;                             // rows without keys, or keys past the table
+  for (int qt = 0; qt < tiles; ++qt) u += tile_units(q, qt, QT, KT);
   return u;
 }
 
@@ -99,104 +126,83 @@ __device__ __forceinline__ bool cursor_next_task(const PagedAttnArgs& a, Cursor&
   return true;
 }
 
-// Moves to the unit `skip` units on.
-__device__ __forceinline__ bool cursor_skip(const PagedAttnArgs& a, Cursor& c, uint64_t skip, int QT, int KT) {
-  for (;;) {
-    if (c.unit == 0 && c.qt == 0) {   // whole heads first
-      const uint64_t hu = head_units(c.q, QT, KT);
-      const uint64_t heads = a.kv.n_kv - c.kvh;
-      if (skip >= hu * heads) {
-        skip -= hu * heads;
-        ++c.s;
-        if (!cursor_seq(a, c, QT, KT)) return false;
-        continue;
-      }
-      c.kvh += (uint32_t)(skip / hu);
-      skip %= hu;
-      c.units = tile_units(c.q, 0, QT, KT);
-      while (skip >= c.units) {
-        skip -= c.units;
-        ++c.qt;
-        c.units = tile_units(c.q, c.qt, QT, KT);
-      }
-      c.unit = (uint32_t)skip;
-      return true;
-    }
-    const uint64_t rest = c.units - c.unit;
-    if (skip < rest) {
-      c.unit += (uint32_t)skip;
-      return true;
-    }
-    skip -= rest;
-    if (!cursor_next_task(a, c, QT, KT)) return false;
+__device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Inclusive sum over the lanes up to this one.
+template <typename V>
+__device__ __forceinline__ V warp_scan(V v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
   }
+  return v;
 }
 
-// All units, and the sequence that holds unit `want(total)` with the units
-// before it: every thread of the block calls this (NT threads, a multiple of
-// 32).  `want` maps the total to the block's first unit.  Lengths that are
-// out of range are reported by the thread that reads them.
-struct BlockStart {
-  uint64_t total, first, before;
-  uint32_t seq;
-};
+// All units (and tasks), a lane per sequence; `mine`: the lane's units in the
+// last 32 sequences.  One lane of one warp of the grid reports lengths that
+// are out of range.
+__device__ __forceinline__ uint64_t warp_total(const PagedAttnArgs& a, int QT, int KT, int lane, bool report, uint64_t& mine, uint64_t* tasks) {
+  uint64_t total = 0, nt = 0;
+  for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += 32) {
+    mine = 0;
+    if (s0 + lane < a.num_seqs) {
+      const SeqInfo q = seq_info(a, s0 + lane);
+      if (report && seq_bad(a, q)) atomicOr(a.err, ERR_BAD_PAGE);
+      mine = head_units(q, QT, KT) * a.kv.n_kv;
+      nt += (uint64_t)((q.rows + QT - 1) / QT) * a.kv.n_kv;
+    }
+    total += mine;
+  }
+  if (tasks) *tasks = warp_sum64(nt);
+  return warp_sum64(total);
+}
 
-template <int NT, typename Want>
-__device__ __forceinline__ BlockStart block_start(const PagedAttnArgs& a, int QT, int KT, Want want) {
-  __shared__ unsigned long long wsum[NT / 32];
-  __shared__ unsigned long long found_before;
-  __shared__ uint32_t found_seq;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  auto units_of = [&](uint32_t s, bool report) -> unsigned long long {
-    if (s >= a.num_seqs) return 0ull;
-    const SeqInfo q = seq_info(a, s);
-    if (report && seq_bad(a, q)) atomicOr(a.err, ERR_BAD_PAGE);
-    return q.rows > 0 ? head_units(q, QT, KT) * a.kv.n_kv : 0ull;
-  };
-  BlockStart b;
-  b.total = 0;
-  unsigned long long mine = 0;   // of the last chunk that this thread looked at
-  for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += NT) {
-    mine = units_of(s0 + tid, blockIdx.x == 0);
-    unsigned long long v = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) wsum[warp] = v;
-    __syncthreads();
-    for (int w = 0; w < NT / 32; ++w) b.total += wsum[w];
-    __syncthreads();
+// The place of unit `want` (below the total) of the concatenated tasks.
+__device__ __forceinline__ void warp_find(const PagedAttnArgs& a, int QT, int KT, int lane, uint64_t want, uint64_t mine, Cursor& c) {
+  uint64_t before = 0;
+  for (uint32_t s0 = 0;; s0 += 32) {
+    if (a.num_seqs > 32) {
+      mine = 0;
+      if (s0 + lane < a.num_seqs) mine = head_units(seq_info(a, s0 + lane), QT, KT) * a.kv.n_kv;
+    }
+    const uint64_t inc = before + warp_scan(mine, lane);
+    const uint32_t hit = __ballot_sync(0xffffffffu, want < inc);
+    if (hit || s0 + 32 >= a.num_seqs) {
+      const int l = hit ? __ffs(hit) - 1 : 0;
+      c.s = s0 + l;
+      want -= __shfl_sync(0xffffffffu, inc - mine, l);
+      break;
+    }
+    before = __shfl_sync(0xffffffffu, inc, 31);
   }
-  b.first = want(b.total);
-  b.seq = 0;
-  b.before = 0;
-  if (b.first >= b.total) return b;
-  unsigned long long base = 0;
-  for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += NT) {
-    if (a.num_seqs > NT) mine = units_of(s0 + tid, false);
-    unsigned long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += t;
-    }
-    if (lane == 31) wsum[warp] = inc;
-    __syncthreads();
-    unsigned long long off = base, all = base;
-    for (int w = 0; w < NT / 32; ++w) {
-      if (w < warp) off += wsum[w];
-      all += wsum[w];
-    }
-    if (b.first >= off + inc - mine && b.first < off + inc) {
-      found_seq = s0 + tid;
-      found_before = off + inc - mine;
-    }
-    __syncthreads();
-    if (b.first < all) break;
-    base = all;
+  c.q = seq_info(a, c.s);
+  const uint64_t hu = head_units(c.q, QT, KT);
+  uint32_t rel;
+  if (want < 0xFFFFFFFFull && hu < 0xFFFFFFFFull) {   // 32-bit division
+    c.kvh = (uint32_t)want / (uint32_t)hu;
+    rel = (uint32_t)want % (uint32_t)hu;
+  } else {
+    c.kvh = (uint32_t)(want / hu);
+    rel = (uint32_t)(want % hu);
   }
-  b.seq = found_seq;
-  b.before = found_before;
-  return b;
+  // the tile: 32 at a time
+  for (int q0 = 0;; q0 += 32) {
+    const uint32_t tu = (int64_t)(q0 + lane) * QT < c.q.rows ? tile_units(c.q, q0 + lane, QT, KT) : 0;
+    const uint32_t inc = warp_scan(tu, lane);
+    const uint32_t hit = __ballot_sync(0xffffffffu, rel < inc);
+    if (hit || (int64_t)(q0 + 32) * QT >= c.q.rows) {
+      const int l = hit ? __ffs(hit) - 1 : 0;
+      c.qt = q0 + l;
+      c.units = __shfl_sync(0xffffffffu, tu, l);
+      c.unit = rel - __shfl_sync(0xffffffffu, inc - tu, l);
+      break;
+    }
+    rel -= __shfl_sync(0xffffffffu, inc, 31);
+  }
 }
 
 // ---- workspace: headers, then two slots of partials per worker ----------

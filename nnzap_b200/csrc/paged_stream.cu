@@ -101,28 +101,23 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
     for (int s = 0; s < S::kStages; ++s) mbar_init(&bars[s], 1);
     fence_barrier_init();
   }
+  __syncwarp();
   const int G = (int)(a.n_q / a.kv.n_kv);
   const int QT = (int)a.max_new;           // one tile holds all rows
   pdl_wait();
   pdl_launch();
-  uint32_t per = 1;
-  const BlockStart bs = block_start<kStWarps * 32>(a, QT, kStKeys, [&](uint64_t total) -> uint64_t {
-    per = max((uint32_t)((total + t.workers - 1) / t.workers), t.min_per);
-    return (uint64_t)blockIdx.x * kStWarps * per;
-  });
   const uint64_t worker = (uint64_t)blockIdx.x * kStWarps + warp;
-  const uint64_t u0 = worker * per, u1 = min(u0 + per, bs.total);
+  uint64_t mine = 0;
+  const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine, nullptr);
+  const uint32_t per = max((uint32_t)((total + t.workers - 1) / t.workers), t.min_per);
+  const uint64_t u0 = worker * per, u1 = min(u0 + per, total);
   PartHeader hdr{0, 0, 0, 0};
-  Cursor c;
-  bool work = u0 < u1;
-  if (work) {
-    c.s = bs.seq;
-    work = cursor_seq(a, c, QT, kStKeys) && cursor_skip(a, c, u0 - bs.before, QT, kStKeys);
-  }
-  if (!work) {
+  if (u0 >= u1) {
     if (lane == 0) t.ws.head[worker] = hdr;
     return;
   }
+  Cursor c;
+  warp_find(a, QT, kStKeys, lane, u0, mine, c);
 
   // ---- producer: copies of one unit, one per lane ----
   Cursor pc = c;

@@ -19,10 +19,10 @@
 // rare.  P up to 256 costs no precision, the sums are f32.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (thread =
-// TMEM lane = row), warp 8 TMA (Q, then K and V tiles into one ring, boxes of
-// one page each, one per lane), warp 9 MMA issue, warp 10 walks the
-// run of units and hands out its parts, warp 11 cleans the V tiles at the
-// diagonal and at the end.  Boxes of absent pages and past the length are
+// TMEM lane = row), warp 8 finds the CTA's run of units, hands its parts to the
+// others and loads them (Q, then K and V tiles into one ring, boxes of one page
+// each, one per lane), warp 9 MMA issue, warp 11 cleans the V tiles at the
+// diagonal and at the end (10 only makes the third warpgroup whole).  Boxes of absent pages and past the length are
 // loaded from beyond the pool's last page: the copy engine fills them with
 // zeros, so no stale byte meets the product.
 //
@@ -49,6 +49,7 @@ constexpr int kUmThreads = 384;
 constexpr int kUmRegsSoftmax = 216, kUmRegsIssue = 72;
 constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
+constexpr uint32_t kPartCost = 3;                 // what a part costs besides its units, in units (queries, epilogue, merge)
 constexpr int kPres = 8;                          // units whose page masks are kept
 constexpr float kLag = 8.f, kUnder = 4.f;         // how far (log2) a row's maximum may lie above / at first below its m
 
@@ -67,7 +68,7 @@ struct UmArgs {
   CUtensorMap tmQ, tmK, tmV;
   PagedAttnArgs a;
   PartWs ws;
-  uint32_t workers, min_per;
+  uint32_t workers;
   uint32_t box;       // keys per copy: 8 .. 128
   uint32_t pt;        // tokens per row tile: 128 / G
   float sl2;          // scale * log2(e)
@@ -154,11 +155,19 @@ __device__ __forceinline__ float2 split2(uint64_t a) {
   return r;
 }
 
-// 2^a, 2^b for a, b >= -126 on the FMA pipe: a = n + f with n the nearest
-// integer (adding 1.5 x 2^23 leaves it in the low mantissa bits), |f| <= 1/2,
-// 2^f by its degree-4 polynomial of least largest relative error (2.6e-6,
-// fitted by reweighted least squares), n added to the exponent.
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^a, 2^b on the FMA pipe: a = n + f with n the nearest integer (adding 1.5 x
+// 2^23 leaves it in the low mantissa bits), |f| <= 1/2, 2^f by its degree-4
+// polynomial of least largest relative error (2.6e-6, fitted by reweighted
+// least squares), 2^n from its exponent bits.  Below -127: 0; NaN: NaN.
 __device__ __forceinline__ float2 ex2_fma(float a, float b) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));     // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
   const uint64_t y = pair2(a, b);
   const uint64_t t = add2(y, pair2(12582912.f, 12582912.f));
   const uint64_t n = add2(t, pair2(-12582912.f, -12582912.f));
@@ -167,9 +176,8 @@ __device__ __forceinline__ float2 ex2_fma(float a, float b) {
   p = fma2(p, f, pair2(0.2402474433f, 0.2402474433f));
   p = fma2(p, f, pair2(0.6931217909f, 0.6931217909f));
   p = fma2(p, f, pair2(0.9999992847f, 0.9999992847f));
-  const float2 q = split2(p), k = split2(t);
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(k.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(k.y) << 23)));
+  const float2 k = split2(t);
+  return split2(mul2(p, pair2(__int_as_float((__float_as_int(k.x) << 23) + 0x3F800000), __int_as_float((__float_as_int(k.y) << 23) + 0x3F800000))));
 }
 
 // Sets the scores of a row's 128 keys that it does not see to -infinity, in
@@ -218,7 +226,7 @@ __device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32
       const float2 y = split2(fma2(pair2(a, b), k2, m2));
       // a quarter of the exponentials on the FMA pipe: both row tiles' on the
       // special-function units alone take 2 x 1024 cycles per unit
-      const float2 q = ((e >> 1) & 3) == 3 ? ex2_fma(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f)) : make_float2(ex2(y.x), ex2(y.y));
+      const float2 q = ((e >> 1) & 3) == 3 ? ex2_fma(y.x, y.y) : make_float2(ex2(y.x), ex2(y.y));
       acc[(e >> 1) & 1] = add2(acc[(e >> 1) & 1], pair2(q.x, q.y));
       w[16 * c + e / 2] = T16<T>::pack(q.x, q.y);
     }
@@ -253,7 +261,7 @@ __device__ __forceinline__ uint32_t bad_mask(uint32_t w) {
   return ((w & e) == e ? 0xFFFFu : 0u) | (((w >> 16) & e) == e ? 0xFFFF0000u : 0u);
 }
 
-// The part of one task in a CTA's run, as warp 10 hands it to the others.
+// The part of one task in a CTA's run, as warp 8 hands it to the others.
 struct Segment {
   uint32_t take;       // units (0: the run is over)
   uint32_t unit;       // first unit within the task
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint64_t* v_ready = pv_done + 2;       // [kPres] a unit's V tile is ready for the product
   uint64_t* pres_full = v_ready + kPres; // [kPres] page mask of a unit written
   uint64_t* seg_full = pres_full + kPres;   // [kSegs]
-  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 11 other warps are done with it
+  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 10 other warps are done with it
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + S::OFF_MISC);
   volatile uint32_t* pres = tslot + 1;   // [kPres] one bit per box of the unit: page present
   Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_MISC + 128);
@@ -337,9 +345,13 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(seg_full + i, 1);
-      mbar_init(seg_empty + i, 11);
+      mbar_init(seg_empty + i, 10);
     }
     fence_barrier_init();
+  }
+  if (warp == 8 && lane < 3) {
+    const CUtensorMap* tm = lane == 0 ? &t.tmQ : lane == 1 ? &t.tmK : &t.tmV;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tslot)) : "memory");
@@ -347,11 +359,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   }
   pdl_wait();
   pdl_launch();
-  uint32_t per = 1;
-  const BlockStart bs = block_start<kUmThreads>(a, QT, kUmKeys, [&](uint64_t total) -> uint64_t {
-    per = max((uint32_t)((total + t.workers - 1) / t.workers), t.min_per);
-    return (uint64_t)blockIdx.x * per;
-  });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     if (!failed) failed = !mbar_wait(bar, parity & 1u, a.err);
   };
 
-  // segment k of the run; every warp but 10 takes them in order
+  // part k of the run; warps 0-7, 9 and 11 take them in order from warp 8
   auto segment = [&](uint32_t k, Segment& g) -> bool {
     wait(seg_full + k % kSegs, k / kSegs);
     g = segs[k % kSegs];
@@ -376,17 +383,124 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUmRegsIssue));
   if (warp == 8) {
-    // ---------------- TMA ----------------
+    // ---------------- the run, and its TMA ----------------
+    uint64_t mine = 0, tasks = 0;
+    const uint64_t total = warp_total(a, QT, kUmKeys, lane, blockIdx.x == 0, mine, &tasks);
+    const uint32_t P = t.workers, per = max(1u, (uint32_t)((total + P - 1) / P));
+    // One part per CTA where that costs no more than kPartCost units over the
+    // even cut: with at most P tasks, the smallest q that cuts them into parts
+    // of at most q units, P of them or fewer.
+    Cursor c;
+    uint32_t part = 0, parts = 0, end = 0;     // one-part runs: part of c's task, its end
+    uint64_t u = 0, u1 = 0;                    // even runs: units [u, u1)
+    bool more = false, even = true;
+    if (tasks <= P && a.num_seqs <= 32) {
+      const SeqInfo q = (uint32_t)lane < a.num_seqs ? seq_info(a, (uint32_t)lane) : SeqInfo{0, 0, 0, 0, 0};
+      const int nt = (q.rows + QT - 1) / QT, inc = warp_scan(nt, lane), D = __shfl_sync(0xffffffffu, inc, 31);
+      // entry j (a tile of one sequence, for every kv head): lanes hold j = lane + 32 i
+      constexpr int kPer = 5;                  // P <= 160
+      uint32_t eu[kPer], es[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int j = lane + 32 * i;
+        eu[i] = es[i] = 0;
+        if (32 * i >= D) continue;
+        // its sequence: the lanes whose tiles end at or before j
+        int s = 0;
+        for (uint32_t l = 0; l < a.num_seqs; ++l) s += __shfl_sync(0xffffffffu, inc, (int)l) <= j ? 1 : 0;
+        const int first = __shfl_sync(0xffffffffu, inc - nt, s & 31);
+        if (j < D) {
+          es[i] = (uint32_t)s;
+          eu[i] = tile_units(seq_info(a, (uint32_t)s), j - first, QT, kUmKeys);
+        }
+      }
+      const uint32_t cap = P / a.kv.n_kv;      // parts of all entries, per kv head
+      for (uint32_t q_ = per; q_ <= per + kPartCost && D <= 32 * kPer; ++q_) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) n += 32 * i < D ? (eu[i] + q_ - 1) / q_ : 0;
+        if (__reduce_add_sync(0xffffffffu, n) > cap) continue;
+        // parts in order of entry, kv head, part
+        even = false;
+        uint32_t before = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (32 * i >= D) continue;
+          const uint32_t np = (eu[i] + q_ - 1) / q_, all = np * a.kv.n_kv;
+          const uint32_t incl = before + warp_scan(all, lane);
+          const uint32_t hit = __ballot_sync(0xffffffffu, blockIdx.x < incl && blockIdx.x >= incl - all);
+          if (hit) {
+            const int l = __ffs(hit) - 1;
+            const uint32_t rel = blockIdx.x - __shfl_sync(0xffffffffu, incl - all, l);
+            parts = __shfl_sync(0xffffffffu, np, l);
+            c.units = __shfl_sync(0xffffffffu, eu[i], l);
+            c.s = __shfl_sync(0xffffffffu, es[i], l);
+            c.kvh = rel / parts;
+            part = rel % parts;
+            c.qt = l + 32 * i - (int)__shfl_sync(0xffffffffu, inc - nt, (int)c.s);
+            c.unit = c.units * part / parts;
+            end = c.units * (part + 1) / parts;
+            more = true;
+          }
+          before = __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (more) c.q = seq_info(a, c.s);
+        break;
+      }
+    }
+    if (even) {
+      u = (uint64_t)blockIdx.x * per;
+      u1 = min(u + per, total);
+      more = u < u1;
+      if (more) warp_find(a, QT, kUmKeys, lane, u, mine, c);
+    }
+
     const uint32_t nb = kUmKeys / t.box;
     const uint32_t bi = (uint32_t)lane % nb, half = (uint32_t)lane / nb;
     const bool copies = half < (uint32_t)NH;
     uint32_t stage_use = 0, unit_no = 0;
-    for (uint32_t seg = 0; segment(seg, g); ++seg) {
-      const int last = g.seen(g.rows - 1);
-      const int* pages = a.page_table + (size_t)g.s * a.table_stride;
+    for (uint32_t seg = 0;; ++seg) {
+      // ---- the next part: to the other warps ----
+      Segment o{};
+      if (more) {
+        o.take = even ? (uint32_t)min((uint64_t)(c.units - c.unit), u1 - u) : end - c.unit;
+        o.unit = c.unit;
+        o.s = c.s;
+        o.kvh = c.kvh;
+        const int tok0 = c.qt * QT;
+        o.row0 = (int)c.q.row0 + tok0;
+        o.rows = min(QT, c.q.rows - tok0);
+        o.e = (int)min(max(c.q.len, (int64_t)0), c.q.cap);
+        o.d = (int)max(c.q.len - c.q.n + 1 + tok0, (int64_t)-(1 << 30));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i * PT < o.rows) {
+            const uint32_t un = max(1u, ((uint32_t)o.seen(min((i + 1) * PT, o.rows) - 1) + kUmKeys - 1) / kUmKeys);
+            o.n[i] = un > c.unit ? min(un - c.unit, o.take) : 0;
+          }
+        if (!even) {
+          o.parts = parts > 1 ? parts : 0;
+        } else if (o.take != c.units) {
+          const uint64_t t0 = u - c.unit;
+          o.parts = (uint32_t)((t0 + c.units - 1) / per - t0 / per + 1);
+        }
+      }
+      if (seg >= kSegs) wait(seg_empty + seg % kSegs, seg / kSegs - 1);
+      __syncwarp();
+      if (lane == 0) {
+        segs[seg % kSegs] = o;
+        mbar_arrive1(seg_full + seg % kSegs);
+      }
+      if (o.take == 0 || failed) break;
+      u += o.take;
+      more = even && u < u1 && cursor_next_task(a, c, QT, kUmKeys);
+
+      // ---- its loads ----
+      const int last = o.seen(o.rows - 1);
+      const int* pages = a.page_table + (size_t)o.s * a.table_stride;
       // page of this lane's box of unit i; -1 where there is none
       auto page_of = [&](uint32_t i, uint32_t& at) -> int {
-        const uint32_t key = (g.unit + i) * kUmKeys + bi * t.box;
+        const uint32_t key = (o.unit + i) * kUmKeys + bi * t.box;
         at = 0;
         if (key >= (uint32_t)last) return -1;
         const uint32_t pi = key / a.kv.page_size;
@@ -400,14 +514,30 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       };
       uint32_t at, nat = 0;
       int pg = page_of(0, at), npg = -1;
-      for (uint32_t i = 0; i < g.take; ++i) {
-        if (i + 1 < g.take) npg = page_of(i + 1, nat);
+      // the queries: at once for the first part, later once the previous part's
+      // products have read theirs (its first K tile does not wait for that)
+      auto queries = [&] {
+        if (seg) wait(q_empty, seg - 1);
+        __syncwarp();
+        const int tiles = PT < o.rows ? 2 : 1;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, (uint32_t)tiles * NH * G * PT * 128);
+          for (int x = 0; x < tiles; ++x)
+            for (int h = 0; h < NH; ++h)
+              tma_load_3d(sm + x * S::kTileB + h * kHalfB, &t.tmQ, h * 64, (int)(o.kvh * G), o.row0 + x * PT, q_full);
+        }
+        __syncwarp();
+      };
+      if (seg == 0) queries();
+      for (uint32_t i = 0; i < o.take; ++i) {
+        if (i + 1 < o.take) npg = page_of(i + 1, nat);
         const uint32_t mask = __ballot_sync(0xffffffffu, (uint32_t)lane < nb && pg >= 0);
         const int slot = (int)(unit_no % kPres);
         if (lane == 0) {
           pres[slot] = mask;
           mbar_arrive1(pres_full + slot);
         }
+#pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t st = stage_use % S::kStages, round = stage_use / S::kStages;
           if (round) wait(kv_empty + st, round - 1);
@@ -416,27 +546,14 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           __syncwarp();
           if (copies)
             tma_load_4d(sm + S::OFF_KV + st * S::kTileB + half * kHalfB + bi * t.box * 128, kv ? &t.tmV : &t.tmK, (int)half * 64, (int)at,
-                        (int)g.kvh, pg >= 0 ? pg : (int)a.kv.num_pages, kv_full + st);
+                        (int)o.kvh, pg >= 0 ? pg : (int)a.kv.num_pages, kv_full + st);
           ++stage_use;
-          if (kv == 0 && i == 0) {
-            // the queries, once the previous segment's products have read theirs
-            if (seg) wait(q_empty, seg - 1);
-            __syncwarp();
-            const int tiles = PT < g.rows ? 2 : 1;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(q_full, (uint32_t)tiles * NH * G * PT * 128);
-              for (int x = 0; x < tiles; ++x)
-                for (int h = 0; h < NH; ++h)
-                  tma_load_3d(sm + x * S::kTileB + h * kHalfB, &t.tmQ, h * 64, (int)(g.kvh * G), g.row0 + x * PT, q_full);
-            }
-            __syncwarp();
-          }
+          if (kv == 0 && i == 0 && seg) queries();
         }
         pg = npg;
         at = nat;
         ++unit_no;
       }
-      segment_done(seg);
     }
   } else if (warp == 9) {
     // ---------------- MMA ----------------
@@ -502,50 +619,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       segment_done(seg);
     }
     if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
-  } else if (warp == 10) {
-    // ---------------- the run, task by task ----------------
-    const uint64_t u0 = (uint64_t)blockIdx.x * per, u1 = min(u0 + per, bs.total);
-    uint64_t u = u0;
-    Cursor c;
-    bool more = u0 < u1;
-    if (more) {
-      c.s = bs.seq;
-      more = cursor_seq(a, c, QT, kUmKeys) && cursor_skip(a, c, u0 - bs.before, QT, kUmKeys);
-    }
-    for (uint32_t k = 0;; ++k) {
-      Segment o{};
-      if (more && u < u1) {
-        o.take = (uint32_t)min((uint64_t)(c.units - c.unit), u1 - u);
-        o.unit = c.unit;
-        o.s = c.s;
-        o.kvh = c.kvh;
-        const int tok0 = c.qt * QT;
-        o.row0 = (int)c.q.row0 + tok0;
-        o.rows = min(QT, c.q.rows - tok0);
-        o.e = (int)min(max(c.q.len, (int64_t)0), c.q.cap);
-        o.d = (int)max(c.q.len - c.q.n + 1 + tok0, (int64_t)-(1 << 30));
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i * PT < o.rows) {
-            const uint32_t un = max(1u, ((uint32_t)o.seen(min((i + 1) * PT, o.rows) - 1) + kUmKeys - 1) / kUmKeys);
-            o.n[i] = un > c.unit ? min(un - c.unit, o.take) : 0;
-          }
-        if (o.take != c.units) {
-          const uint64_t t0 = u - c.unit;
-          o.parts = (uint32_t)((t0 + c.units - 1) / per - t0 / per + 1);
-        }
-        u += o.take;
-        if (u < u1) more = cursor_next_task(a, c, QT, kUmKeys);
-      }
-      if (k >= kSegs) wait(seg_empty + k % kSegs, k / kSegs - 1);
-      __syncwarp();
-      if (lane == 0) {
-        segs[k % kSegs] = o;
-        mbar_arrive1(seg_full + k % kSegs);
-      }
-      if (o.take == 0 || failed) break;
-    }
-  } else {
+  } else if (warp == 11) {
     // ---------------- V tiles with keys that not every row sees ----------------
     // A V row past the length is zeroed (its box holds earlier keys), and so is
     // every non-finite element of a row that some rows see and others do not,
@@ -729,7 +803,6 @@ cudaError_t paged_umma_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStr
   t.a = a;
   t.workers = (uint32_t)a.num_sms;
   t.ws = part_ws(a.ws, t.workers, kUmmaRows);
-  t.min_per = 1;
   t.box = 8;
   while (t.box < (uint32_t)kUmKeys && a.kv.page_size % (2 * t.box) == 0) t.box *= 2;
   const uint32_t G = a.n_q / a.kv.n_kv;

@@ -227,6 +227,31 @@ def test_paged_attention_nonfinite_values_stay_in_their_rows(n):
     assert torch.isnan(got[n - 3:]).all()
 
 
+@pytest.mark.parametrize("n", [1, 200])
+def test_paged_attention_low_scores_and_nan_keys(n):
+    """Rows whose scores all lie far below zero keep their precision; a NaN key, wherever it is, shows in every row that sees it."""
+    L = 700
+    c = attn_case(81, [(n, L)], 4, 2, 128, 16, "f16", "head")
+    j = torch.arange(L, device="cuda")
+    pg, at = c["table"][0].long()[j // 16], j % 16
+    c["q"].view(n, 4, 128)[..., 0] = 30.0
+    keep = c["k"][pg, :, at].clone()
+    for low in (-20.0, -60.0, -400.0):                      # scores near -53, -160, -1060
+        k = keep.clone()
+        k[..., 0] = low
+        c["k"][pg, :, at] = k
+        check_attn(c, f"low {low}")
+    c["k"][pg, :, at] = keep
+    op = P().PagedAttention(P().PagedKV(c["k"], c["v"]), 4)
+    for key in list(range(8)) + [L - n, L - 1]:
+        k = keep.clone()
+        k[key] = float("nan")
+        c["k"][pg, :, at] = k
+        got = op(c["q"], c["table"], c["q_start"], c["kv_len"], c["max_new"])
+        sees = torch.arange(n, device="cuda") + L - n >= key
+        assert torch.isnan(got[sees]).all() and torch.isfinite(got[~sees]).all(), key
+
+
 def test_paged_attention_far_pages():
     """Element offsets beyond 32 bits: the last pages of a pool of 2^32 + elements."""
     page, n_kv, hd = 16, 8, 128
