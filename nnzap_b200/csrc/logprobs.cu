@@ -12,10 +12,10 @@
 //
 // Most probable tokens cost the stream nothing but a store: every thread's
 // maximum of each step (16 or 32 elements) goes to shared memory.  The k-th
-// largest of the 256 threads' overall maxima bounds the CTA's k best from
-// below; the steps whose maximum reaches it (about k of them) are read again,
-// 64 bytes each, and their elements collected as sorted 64-bit (value, index)
-// keys, 32 to a list, one per lane of a warp.
+// largest of 64 overall maxima (each of 4 threads) bounds the CTA's k best
+// from below; the steps whose maximum reaches it (about k of them) are read
+// again, 64 bytes each, and their elements that reach it sorted as 64-bit
+// (value, index) keys, 32 to a list, one per lane of a warp.
 //
 // A row is cut over a cluster of CTAs (1 to 16) whose triples and lists meet
 // in the first CTA's shared memory: no workspace, no atomics on memory, the
@@ -157,9 +157,12 @@ __device__ __forceinline__ void lp_unpack(const uint4& u, float* x) {
 
 constexpr int kLpSlots = 24;      // step maxima kept per thread; longer slices keep one per 2, 4, .. steps
 
+constexpr int kLpPool = kLpWarps * 64;
+
 struct LpShared {
   float smax[kLpSlots][kLpThreads];
-  unsigned long long buf[kLpWarps][64];                        // candidates of each warp
+  unsigned long long pool[kLpPool];                             // candidates
+  uint32_t count;
   unsigned long long list[kLpWarps][32];
   uint32_t tmax[kLpWarps][32];
   unsigned long long peer[kLpMaxCluster][32];                  // the cluster's lists (first CTA)
@@ -201,8 +204,11 @@ __device__ __forceinline__ void lp_tree(K (*lists)[32], K& mine, int warp, int l
   }
 }
 
+// CTAs per SM: 4 for f32 (512 rows in one wave: 61 us, with 3 and more
+// registers 84); 16-bit steps hold twice the elements and want the registers
+// (64 rows: 14.2 us, with 4 CTAs and spills 17.5).
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
+__global__ void __launch_bounds__(kLpThreads, sizeof(T) == 4 ? 4 : 3) logprobs_kernel(const LpArgs a) {
   constexpr int EPV = 16 / (int)sizeof(T);
   constexpr int E = kLpVec * EPV;
   __shared__ std::conditional_t<TOP, LpShared, LpSharedNoTop> sh;
@@ -289,66 +295,96 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LpArgs a) {
   if (lane == 0) sh.stat[warp] = st;
   unsigned long long best = 0;          // lane i: the i-th best so far
   if constexpr (TOP) {
-    // the k-th largest of the threads' maxima
-    uint32_t tk = lp_sort32(float_key(thread_max + 0.f), lane);
-    lp_tree(sh.tmax, tk, warp, lane);
-    const float floor_ = lp_value((unsigned long long)sh.tmax[0][a.top_k - 1] << 32);
+    // The k-th largest of 64 maxima, each over 4 threads (every warp finds it
+    // for itself: two sorts side by side and a merge).
+    sh.tmax[warp][lane] = float_key(thread_max + 0.f);
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    const uint32_t g0 = lp_sort32(max(max(sh.tmax[0][lane], sh.tmax[1][lane]), max(sh.tmax[2][lane], sh.tmax[3][lane])), lane);
+    const uint32_t g1 = lp_sort32(max(max(sh.tmax[4][lane], sh.tmax[5][lane]), max(sh.tmax[6][lane], sh.tmax[7][lane])), lane);
+    const uint32_t tk = __shfl_sync(0xffffffffu, lp_merge32(g0, g1, lane), (int)a.top_k - 1);
+    const float floor_ = lp_value((unsigned long long)tk << 32);
 
     // The steps of this warp's threads that reach it are read again, four
     // loads at a time; lane: vector lane / EPV of the step, element lane % EPV.
+    // f(value, index): one call per lane and element, the warp together.
     const uint32_t slots = (steps + (1u << shift) - 1) >> shift;
-    uint32_t mine = 0;                   // slots of this thread
-    for (uint32_t sl = 0; sl < slots; ++sl) {
-      const float v = sh.smax[sl][threadIdx.x];
-      if (v >= floor_ && v > -INFINITY) mine |= 1u << sl;
-    }
-    uint32_t cnt = 0;                    // candidates waiting in the buffer (warp-uniform)
-    unsigned long long kth = 0;           // the list's k-th key
-    auto flush = [&]() {                 // the first 32 of the buffer into the list
-      __syncwarp();
-      const unsigned long long k = (uint32_t)lane < cnt ? sh.buf[warp][lane] : 0ull;
-      const unsigned long long rest = (uint32_t)lane + 32 < cnt ? sh.buf[warp][lane + 32] : 0ull;
-      __syncwarp();
-      sh.buf[warp][lane] = rest;
-      cnt = cnt > 32 ? cnt - 32 : 0;
-      best = lp_merge32(best, lp_sort32(k, lane), lane);
-      kth = __shfl_sync(0xffffffffu, best, (int)a.top_k - 1);
-      __syncwarp();
-    };
-    uint32_t src = 0, sl = 0, sub = 0;   // thread (lane), slot and step of the next load
-    uint32_t owners = __ballot_sync(0xffffffffu, mine != 0);
-    while (owners || sub) {
-      float xv[4];
-      uint32_t idx[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        xv[q] = -INFINITY;
-        idx[q] = 0;
-        if (!(owners || sub)) continue;
-        if (sub == 0) {
-          src = (uint32_t)__ffs(owners) - 1;
-          sl = (uint32_t)__ffs(__shfl_sync(0xffffffffu, mine, (int)src)) - 1;
-          if ((uint32_t)lane == src) mine &= mine - 1;
-          owners = __ballot_sync(0xffffffffu, mine != 0);
-        }
-        const uint32_t gr = gb + ((sl << shift) + sub) * STEP + (lane / EPV) * kLpThreads + warp * 32 + src;
-        const int64_t e = (int64_t)gr * EPV + lane % EPV - skew;
-        if (lane < E && gr < ge && e >= 0 && e < (int64_t)a.n) xv[q] = lp_load1(xr + e);
-        idx[q] = (uint32_t)e;
-        sub = (sub + 1) & ((1u << shift) - 1);
+    auto again = [&](auto f) {
+      uint32_t mine = 0;                 // slots of this thread
+      for (uint32_t sl = 0; sl < slots; ++sl) {
+        const float v = sh.smax[sl][threadIdx.x];
+        if (v >= floor_ && v > -INFINITY) mine |= 1u << sl;
       }
+      uint32_t src = 0, sl = 0, sub = 0;   // thread (lane), slot and step of the next load
+      uint32_t owners = __ballot_sync(0xffffffffu, mine != 0);
+      while (owners || sub) {
+        float xv[4];
+        uint32_t idx[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const unsigned long long key = xv[q] >= floor_ && xv[q] > -INFINITY ? lp_key(xv[q], idx[q]) : 0ull;
+        for (int q = 0; q < 4; ++q) {
+          xv[q] = -INFINITY;
+          idx[q] = 0;
+          if (!(owners || sub)) continue;
+          if (sub == 0) {
+            src = (uint32_t)__ffs(owners) - 1;
+            sl = (uint32_t)__ffs(__shfl_sync(0xffffffffu, mine, (int)src)) - 1;
+            if ((uint32_t)lane == src) mine &= mine - 1;
+            owners = __ballot_sync(0xffffffffu, mine != 0);
+          }
+          const uint32_t gr = gb + ((sl << shift) + sub) * STEP + (lane / EPV) * kLpThreads + warp * 32 + src;
+          const int64_t e = (int64_t)gr * EPV + lane % EPV - skew;
+          if (lane < E && gr < ge && e >= 0 && e < (int64_t)a.n) xv[q] = lp_load1(xr + e);
+          idx[q] = (uint32_t)e;
+          sub = (sub + 1) & ((1u << shift) - 1);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f(xv[q], idx[q]);
+      }
+    };
+    // They are few (about k for any but contrived rows): one pool for the CTA.
+    again([&](float v, uint32_t i) {
+      if (v >= floor_ && v > -INFINITY) {
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < (uint32_t)kLpPool) sh.pool[at] = lp_key(v, i);
+      }
+    });
+    __syncthreads();
+    const uint32_t count = sh.count;
+    if (count <= (uint32_t)kLpPool) {
+      if (warp == 0) {
+        best = lp_sort32((uint32_t)lane < count ? sh.pool[lane] : 0ull, lane);
+        for (uint32_t at = 32; at < count; at += 32)
+          best = lp_merge32(best, lp_sort32(at + lane < count ? sh.pool[at + lane] : 0ull, lane), lane);
+      }
+    } else {
+      // many equal or nearly equal largest logits: a list per warp, 32
+      // candidates at a time, those that beat its k-th
+      __syncthreads();                   // the pool becomes the warps' buffers
+      unsigned long long* buf = sh.pool + warp * 64;
+      uint32_t cnt = 0;
+      unsigned long long kth = 0;
+      auto flush = [&]() {
+        __syncwarp();
+        const unsigned long long k = (uint32_t)lane < cnt ? buf[lane] : 0ull;
+        const unsigned long long rest = (uint32_t)lane + 32 < cnt ? buf[lane + 32] : 0ull;
+        __syncwarp();
+        buf[lane] = rest;
+        cnt = cnt > 32 ? cnt - 32 : 0;
+        best = lp_merge32(best, lp_sort32(k, lane), lane);
+        kth = __shfl_sync(0xffffffffu, best, (int)a.top_k - 1);
+        __syncwarp();
+      };
+      again([&](float v, uint32_t i) {
+        const unsigned long long key = v >= floor_ && v > -INFINITY ? lp_key(v, i) : 0ull;
         const bool take = key > kth;
         const uint32_t b = __ballot_sync(0xffffffffu, take);
-        if (take) sh.buf[warp][cnt + __popc(b & ((1u << lane) - 1u))] = key;
+        if (take) buf[cnt + __popc(b & ((1u << lane) - 1u))] = key;
         cnt += __popc(b);
         if (cnt >= 32) flush();
-      }
+      });
+      if (cnt) flush();
+      lp_tree(sh.list, best, warp, lane);
     }
-    if (cnt) flush();
-    lp_tree(sh.list, best, warp, lane);
   } else {
     __syncthreads();
   }
@@ -412,10 +448,13 @@ cudaError_t logprobs_go(const LpArgs& a, int sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     ready.store(true, std::memory_order_relaxed);
   }
-  // enough CTAs to fill the SMs, but at least a few steps of work for each
+  // CTAs per row: as many as keep the row's CTAs within two per SM, each with
+  // a step of work or more (a CTA's sorts and merges cost it 3 - 4 us: 64 rows
+  // of 151669 bf16 take 14.5 us with 4, 17.8 with 8, 16.9 with 2; 512 rows of
+  // 151936 f32 60.9 us with 1, 69.8 with 2; one row 8.3 us with 16, 11.2 with 4)
   const uint64_t bytes = (uint64_t)a.n * sizeof(T);
   uint32_t C = 1;
-  while (C < kLpMaxCluster && (uint64_t)a.rows * C < (uint64_t)sms * 6 && bytes / (2 * C) >= kLpThreads * kLpVec * 16) C *= 2;
+  while (C < kLpMaxCluster && (uint64_t)a.rows * 2 * C <= (uint64_t)sms * 2 && bytes / (2 * C) >= kLpThreads * kLpVec * 16) C *= 2;
   if ((uint64_t)a.rows * C > 0x7FFFFFFFull) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.rows * C);
