@@ -355,7 +355,8 @@ typedef struct nnz_paged_attn_args {
   float scale;                    /* 0: 1 / sqrt(head_dim) */
   void* out;                      /* [tokens][out_stride] */
   int64_t out_stride;             /* elements, multiple of 8 */
-  void* workspace;                /* nnz_paged_attn_workspace bytes, 256-byte aligned; one call at a time */
+  void* workspace;                /* nnz_paged_attn_workspace bytes, 256-byte aligned, zeroed by the caller
+                                   * before its first use (calls leave it as they found it); one call at a time */
   size_t workspace_bytes;
 } nnz_paged_attn_args;
 

@@ -231,117 +231,12 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(const PagedAttnArgs
   for (int e = 0; e < EPL; e += 2) *reinterpret_cast<uint32_t*>(op + e) = T16<T>::pack(o[e] * r, o[e + 1] * r);
 }
 
-// ---------------------------------------------------------------------------
-// merge of split tasks
-// ---------------------------------------------------------------------------
-// Parts k (max m_k, sum l_k, o_k) of a row: M = max m_k, out = sum 2^(m_k - M)
-// o_k / sum 2^(m_k - M) l_k.  A block looks at `span` workers' headers and
-// takes 16 rows of each split task; its 8 warps share the rows, and the parts
-// of a row where there are fewer than 8 of them.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a, const PartWs ws, uint32_t workers, uint32_t span) {
-  constexpr int E = HD / 32;
-  __shared__ float red[8][HD + 2];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t G = a.n_q / a.kv.n_kv;
-  pdl_wait();
-  const uint32_t w0 = blockIdx.x * span, w1 = min(w0 + span, workers);
-  for (uint32_t w = w0; w < w1; ++w) {
-    const PartHeader h = ws.head[w];
-    if (h.parts == 0) continue;
-    const int rbase = blockIdx.y * 16, rows = min(16, (int)h.rows - rbase);
-    if (rows <= 0) continue;
-    const int sw = rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;   // warps to a row
-    const int split = warp % sw;
-    for (int r0 = 0; r0 < rows; r0 += 8 / sw) {
-      const int row = rbase + r0 + warp / sw;
-      const bool live = row < rbase + rows;
-      float m = -INFINITY, l = 0.f, o[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-      if (live) {
-        for (uint32_t k0 = split; k0 < h.parts; k0 += 4 * sw) {
-          float pm[4], pl[4], po[4][E];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t k = k0 + i * sw;
-            pm[i] = -INFINITY;
-            pl[i] = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) po[i][e] = 0.f;
-            if (k < h.parts) {
-              const float* p = ws.slot((uint64_t)w + k, k == 0 ? 1 : 0, HD);
-              pm[i] = __ldcg(p + row);
-              pl[i] = __ldcg(p + ws.R + row);
-              const float* po_ = p + 2 * ws.R + (size_t)row * HD + lane * E;
-              if constexpr (E == 4) {
-                const float4 f = __ldcg(reinterpret_cast<const float4*>(po_));
-                po[i][0] = f.x; po[i][1] = f.y; po[i][2] = f.z; po[i][3] = f.w;
-              } else {
-                const float2 f = __ldcg(reinterpret_cast<const float2*>(po_));
-                po[i][0] = f.x; po[i][1] = f.y;
-              }
-            }
-          }
-          float mn = m;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mn = fmaxf(mn, pm[i]);
-          const float ms = mn == -INFINITY ? 0.f : mn;
-          const float c = exp2f(m - ms);
-          m = mn;
-          l *= c;
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] *= c;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float f = exp2f(pm[i] - ms);
-            l = fmaf(f, pl[i], l);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(f, po[i][e], o[e]);
-          }
-        }
-      }
-      if (sw > 1) {
-        if (lane == 0) {
-          red[warp][HD] = m;
-          red[warp][HD + 1] = l;
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) red[warp][lane * E + e] = o[e];
-        __syncthreads();
-        if (split == 0) {
-          float mn = m;
-          for (int i = 1; i < sw; ++i) mn = fmaxf(mn, red[warp + i][HD]);
-          const float ms = mn == -INFINITY ? 0.f : mn;
-          const float c = exp2f(m - ms);
-          l *= c;
-#pragma unroll
-          for (int e = 0; e < E; ++e) o[e] *= c;
-          for (int i = 1; i < sw; ++i) {
-            const float f = exp2f(red[warp + i][HD] - ms);
-            l = fmaf(f, red[warp + i][HD + 1], l);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(f, red[warp + i][lane * E + e], o[e]);
-          }
-        }
-        __syncthreads();
-      }
-      if (live && split == 0) {
-        const float il = l == 0.f ? 0.f : 1.f / l;
-        uint16_t* op = a.out + ((int64_t)h.row0 + row / G) * a.out_stride + ((int64_t)h.kvh * G + row % G) * HD + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(op + e) = T16<T>::pack(o[e] * il, o[e + 1] * il);
-      }
-    }
-  }
-}
-
 }  // namespace
 
 namespace {
 
-// The tiled kernel's parts, [HD / 4][R][4]: a block takes 32 rows of one
-// split task, lane = row, a warp HD / 8 dims, so every load is 512 bytes in
+// The tiled kernel's parts, [HD / 4][R][4] (128 KB each: one CTA alone would
+// need 13 us for four of them): a block takes 32 rows of one split task, lane = row, a warp HD / 8 dims, so every load is 512 bytes in
 // a row and a lane's output whole sectors.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) paged_merge_tile_kernel(const PagedAttnArgs a, const PartWs ws) {
@@ -368,7 +263,7 @@ __global__ void __launch_bounds__(256) paged_merge_tile_kernel(const PagedAttnAr
 #pragma unroll
       for (int i = 0; i < N4; ++i) po[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k < h.parts) {
-        const float* p = ws.slot((uint64_t)blockIdx.x + k, k == 0 ? 1 : 0, HD);
+        const float* p = ws.slot(blockIdx.x + k, k == 0 ? 1 : 0, HD);
         pm[j] = __ldcg(p + row);
         pl[j] = __ldcg(p + ws.R + row);
         const float4* q = reinterpret_cast<const float4*>(p + 2 * ws.R) + row;
@@ -415,24 +310,6 @@ cudaError_t paged_merge_tile_launch(const PagedAttnArgs& a, const PartWs& ws, ui
                      : cudaLaunchKernelEx(&cfg, &paged_merge_tile_kernel<__half, 64>, a, ws);
   return hd == 128 ? cudaLaunchKernelEx(&cfg, &paged_merge_tile_kernel<__nv_bfloat16, 128>, a, ws)
                    : cudaLaunchKernelEx(&cfg, &paged_merge_tile_kernel<__nv_bfloat16, 64>, a, ws);
-}
-
-cudaError_t paged_merge_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  const uint32_t span = std::max(1u, workers / (uint32_t)a.num_sms);
-  cfg.gridDim = dim3((workers + span - 1) / span, (ws.R + 15) / 16);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  if (dtype == RD_F16)
-    return hd == 128 ? cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__half, 128>, a, ws, workers, span)
-                     : cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__half, 64>, a, ws, workers, span);
-  return hd == 128 ? cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__nv_bfloat16, 128>, a, ws, workers, span)
-                   : cudaLaunchKernelEx(&cfg, &paged_merge_kernel<__nv_bfloat16, 64>, a, ws, workers, span);
 }
 
 namespace {
@@ -613,8 +490,7 @@ size_t nnz_paged_attn_workspace(const nnz_paged_kv* kv, uint32_t num_query_heads
   int* err = nullptr;
   int sms = 0;
   if (op_device(&err, &sms)) sms = 148;   // no device: the size for a full B200
-  return std::max(part_ws_bytes(paged_stream_workers(sms), kStreamRows, kv->head_dim),
-                  part_ws_bytes((uint32_t)sms, kUmmaRows, kv->head_dim));
+  return std::max(paged_stream_ws(sms, (int)kv->head_dim), paged_umma_ws(sms, (int)kv->head_dim));
 }
 
 int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* stream) {

@@ -6,11 +6,10 @@
 // Worker w takes units [w per, (w + 1) per) of the concatenation in task
 // order: whatever the mix of lengths, all workers finish together, and a
 // worker splits at most two tasks (its first and its last).  A worker that
-// holds a whole task writes its output; of a split task every worker leaves a
-// partial (max, sum, sum p v) in the workspace, the task's first part in slot
-// 1 of its worker, the others in slot 0 of theirs, and the first part's
-// worker leaves a header that the merge kernel goes by.  The cut depends on
-// the lengths alone, so results do not change from call to call.
+// holds a whole task writes its output; the parts of a split task (max, sum,
+// sum p v) meet in the workspace and are merged by whoever finishes last.  The
+// cut and the order of the merge depend on the lengths alone, so results do
+// not change from call to call.
 #pragma once
 #include "paged.cuh"
 
@@ -205,47 +204,127 @@ __device__ __forceinline__ void warp_find(const PagedAttnArgs& a, int QT, int KT
   }
 }
 
-// ---- workspace: headers, then two slots of partials per worker ----------
-struct PartHeader {
-  uint32_t row0;    // first q / out row of the task
-  uint32_t kvh;
-  uint32_t rows;    // (token, head) rows, head fastest
-  uint32_t parts;   // 0: the worker holds no first part of a split task
+// One part of one task per CTA, for few tasks: parts of at most q units, the
+// smallest q of q0 .. q1 (in steps of 1/16) that makes at most `ctas` of them.
+// Lanes hold the (sequence, tile) pairs 32 i + lane, i < N.
+struct PartRun {
+  uint32_t part, parts;    // 0 parts: none for this CTA
+  uint32_t end;            // of the part within the task (its start: c.unit)
 };
 
+template <int N>
+__device__ __forceinline__ bool warp_parts(const PagedAttnArgs& a, int QT, int KT, int lane, uint32_t ctas, uint32_t q0, uint32_t q1,
+                                           uint32_t cta, Cursor& c, PartRun& run) {
+  const SeqInfo mine = (uint32_t)lane < a.num_seqs ? seq_info(a, (uint32_t)lane) : SeqInfo{0, 0, 0, 0, 0};
+  const int nt = (mine.rows + QT - 1) / QT, inc = warp_scan(nt, lane), D = __shfl_sync(0xffffffffu, inc, 31);
+  if (D > 32 * N) return false;
+  uint32_t eu[N], es[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = lane + 32 * i;
+    eu[i] = es[i] = 0;
+    if (32 * i >= D) continue;
+    int s = 0;        // its sequence: those before it end at or before j
+    for (uint32_t l = 0; l < a.num_seqs; ++l) s += __shfl_sync(0xffffffffu, inc, (int)l) <= j ? 1 : 0;
+    const int first = __shfl_sync(0xffffffffu, inc - nt, s & 31);
+    if (j < D) {
+      es[i] = (uint32_t)s;
+      eu[i] = tile_units(seq_info(a, (uint32_t)s), j - first, QT, KT);
+    }
+  }
+  const uint32_t cap = ctas / a.kv.n_kv;      // parts of all pairs, per kv head
+  for (uint32_t q = q0; q <= q1; q += max(1u, q / 16)) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += 32 * i < D ? (eu[i] + q - 1) / q : 0;
+    if (__reduce_add_sync(0xffffffffu, n) > cap) continue;
+    run = {0, 0, 0};
+    uint32_t before = 0;                      // parts in order of pair, kv head, part
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (32 * i >= D) continue;
+      const uint32_t np = (eu[i] + q - 1) / q, all = np * a.kv.n_kv;
+      const uint32_t incl = before + warp_scan(all, lane);
+      const uint32_t hit = __ballot_sync(0xffffffffu, cta < incl && cta >= incl - all);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        const uint32_t rel = cta - __shfl_sync(0xffffffffu, incl - all, l);
+        run.parts = __shfl_sync(0xffffffffu, np, l);
+        c.units = __shfl_sync(0xffffffffu, eu[i], l);
+        c.s = __shfl_sync(0xffffffffu, es[i], l);
+        c.kvh = rel / run.parts;
+        run.part = rel % run.parts;
+        c.qt = l + 32 * i - (int)__shfl_sync(0xffffffffu, inc - nt, (int)c.s);
+        c.unit = (uint32_t)((uint64_t)c.units * run.part / run.parts);
+        run.end = (uint32_t)((uint64_t)c.units * (run.part + 1) / run.parts);
+        c.q = seq_info(a, c.s);
+      }
+      before = __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return true;
+  }
+  return false;
+}
+
+// ---- workspace: a header, a counter and two slots of partials per CTA ----
+// A CTA's part of a split task goes to slot 1 of the CTA if it is the task's
+// first, else to slot 0.
+// Streaming kernel: the counter of the first part's CTA counts the parts that
+// are there, and the CTA that completes it merges them, in order, and sets it
+// back to 0: the workspace is zeroed once by its owner and every call leaves
+// it as it found it.  Tiled kernel: the first part's CTA leaves a header, which
+// a merge kernel goes by.
+//
 // One slot: R maxima (log2 domain), R sums, R x HD sums of p v (row by row
 // from the streaming kernel, [HD / 4][R][4] from the tiled one).
 __host__ __device__ constexpr size_t slot_floats(uint32_t R, uint32_t hd) { return (size_t)R * (hd + 2); }
 
+struct PartHeader {
+  uint32_t row0;    // first q / out row of the task
+  uint32_t kvh;
+  uint32_t rows;    // (token, head) rows, head fastest
+  uint32_t parts;   // 0: the CTA holds no first part of a split task
+};
+
 struct PartWs {
   PartHeader* head;
+  uint32_t* count;
   float* slots;
   uint32_t R;
-  __device__ __forceinline__ float* slot(uint64_t worker, int which, uint32_t hd) const {
-    return slots + (worker * 2 + which) * slot_floats(R, hd);
+  __device__ __forceinline__ float* slot(uint32_t cta, int which, uint32_t hd) const {
+    return slots + ((size_t)cta * 2 + which) * slot_floats(R, hd);
   }
 };
 
-inline size_t part_ws_bytes(uint32_t workers, uint32_t R, uint32_t hd) {
-  return (((size_t)workers * sizeof(PartHeader) + 255) & ~(size_t)255) + (size_t)workers * 2 * slot_floats(R, hd) * 4;
+inline size_t part_ws_bytes(uint32_t ctas, uint32_t R, uint32_t hd) {
+  return (((size_t)ctas * 20 + 255) & ~(size_t)255) + (size_t)ctas * 2 * slot_floats(R, hd) * 4;
 }
-inline PartWs part_ws(void* ws, uint32_t workers, uint32_t R) {
-  return {static_cast<PartHeader*>(ws),
-          reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + (((size_t)workers * sizeof(PartHeader) + 255) & ~(size_t)255)), R};
+inline PartWs part_ws(void* ws, uint32_t ctas, uint32_t R) {
+  uint8_t* b = static_cast<uint8_t*>(ws);     // counters first: both kernels' workspaces begin with them
+  return {reinterpret_cast<PartHeader*>(b + (size_t)ctas * 4), reinterpret_cast<uint32_t*>(b),
+          reinterpret_cast<float*>(b + (((size_t)ctas * 20 + 255) & ~(size_t)255)), R};
 }
 
-// Merges the parts of split tasks into the output (paged.cu); launched with
-// programmatic dependent launch behind the kernel that left them.
-cudaError_t paged_merge_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st);
+// One thread, after its CTA's (or warp's) stores to a slot have been made
+// visible: counts the part; true for the last one.
+__device__ __forceinline__ bool part_done(const PartWs& ws, uint32_t first_cta, uint32_t parts) {
+  __threadfence();
+  if (atomicAdd(ws.count + first_cta, 1u) != parts - 1) return false;
+  ws.count[first_cta] = 0;
+  __threadfence();
+  return true;
+}
+
 cudaError_t paged_merge_tile_launch(const PagedAttnArgs& a, const PartWs& ws, uint32_t workers, int dtype, int hd, cudaStream_t st);
 
 // Few query rows per kv head and sequence (at most 16): keys streamed by
 // independent warps (paged_stream.cu).
 constexpr uint32_t kStreamRows = 16;
-uint32_t paged_stream_workers(int num_sms);
+size_t paged_stream_ws(int num_sms, int hd);      // bytes of workspace
 cudaError_t paged_stream_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st);
 // Many query rows: 2 x 128 to a CTA, tcgen05 (paged_umma.cu).
 constexpr uint32_t kUmmaRows = 256;
+size_t paged_umma_ws(int num_sms, int hd);
 cudaError_t paged_umma_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st);
 
 }  // namespace nnz

@@ -2,7 +2,9 @@
 // and kv head: single tokens, drafts of a few tokens): bound by the bytes of
 // K and V.
 //
-// Every warp is a worker of the shared cut (paged_sched.cuh): it streams its
+// Every warp is a worker of the shared cut (paged_sched.cuh), 8 to a CTA and a
+// CTA to an SM; the parts of a split task meet first within the CTA, then
+// (where it spans CTAs) in the workspace.  A warp streams its
 // run of 16-key units through a private ring of shared memory, each unit four
 // (or, with pages whose size is only a multiple of 8, eight) TMA copies of K
 // and V halves with the 128-byte swizzle, issued one per lane, so a unit's
@@ -26,7 +28,7 @@ namespace nnz {
 
 namespace {
 
-constexpr int kStWarps = 4;
+constexpr int kStWarps = 8;
 constexpr int kStKeys = 16;
 
 template <int HD>
@@ -39,11 +41,19 @@ struct StShape {
   static constexpr int kSmem = kStWarps * kWarpB + 1024;       // + alignment
 };
 
+// A warp's part of a task that it does not hold whole.
+struct StPart {
+  unsigned long long t0;   // the task's first unit
+  const float* sums;       // a slot (paged_sched.cuh), shared or global memory
+  uint32_t units;          // 0: no part
+  uint32_t row0, kvh, rows;
+};
+
 struct StArgs {
   CUtensorMap tmK, tmV;
   PagedAttnArgs a;
   PartWs ws;
-  uint32_t workers, min_per;
+  float* park;         // a slot per warp
   uint32_t box;        // keys per copy: 16 or 8
   float sl2;           // scale * log2(e)
 };
@@ -83,6 +93,26 @@ __device__ __forceinline__ bool finite16(uint32_t w, bool bf16) {
   return (w & e & 0xFFFFu) != (e & 0xFFFFu) && (w & e & 0xFFFF0000u) != (e & 0xFFFF0000u);
 }
 
+// (m, l, o) of a row plus one more part of it; lane: HD / 32 dims.
+template <int HD>
+__device__ __forceinline__ void merge_part(float pm, float pl, const float* po, float& m, float& l, float (&o)[HD / 32]) {
+  const float mn = fmaxf(m, pm), ms = mn == -INFINITY ? 0.f : mn;
+  const float c = exp2f(m - ms), f = exp2f(pm - ms);
+  m = mn;
+  l = l * c + pl * f;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d) o[d] = o[d] * c + po[d] * f;
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void merge_out(const PagedAttnArgs& a, uint32_t row0, uint32_t kvh, uint32_t row, int G, int lane, float l,
+                                          const float (&o)[HD / 32]) {
+  const float il = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* op = a.out + ((int64_t)row0 + row / G) * a.out_stride + ((int64_t)kvh * G + row % G) * HD + lane * (HD / 32);
+#pragma unroll
+  for (int d = 0; d < HD / 32; d += 2) *reinterpret_cast<uint32_t*>(op + d) = T16<T>::pack(o[d] * il, o[d + 1] * il);
+}
+
 // ROWS8: at most 8 query rows (the lower half of every fragment is absent).
 template <typename T, int HD, bool ROWS8>
 __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __grid_constant__ StArgs t) {
@@ -91,6 +121,9 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   constexpr int KS = HD / 16;              // K steps of S
   constexpr int NT = HD / 8;               // n tiles of O
   extern __shared__ uint8_t smem_raw[];
+  __shared__ StPart parts[kStWarps][2];     // that start before the warp's run or within it
+  __shared__ StPart merge[2];                // split tasks whose last part is this CTA's
+  __shared__ float red[kStWarps][HD + 2];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PagedAttnArgs& a = t.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -104,20 +137,35 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   __syncwarp();
   const int G = (int)(a.n_q / a.kv.n_kv);
   const int QT = (int)a.max_new;           // one tile holds all rows
-  pdl_wait();
-  pdl_launch();
-  const uint64_t worker = (uint64_t)blockIdx.x * kStWarps + warp;
-  uint64_t mine = 0;
-  const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine, nullptr);
-  const uint32_t per = max((uint32_t)((total + t.workers - 1) / t.workers), t.min_per);
-  const uint64_t u0 = worker * per, u1 = min(u0 + per, total);
-  PartHeader hdr{0, 0, 0, 0};
-  if (u0 >= u1) {
-    if (lane == 0) t.ws.head[worker] = hdr;
-    return;
-  }
+  // The run of this warp: of a part of one task that the CTA has for itself
+  // where there are few tasks (64 units to a CTA or more: a task that fits one
+  // CTA is cheaper there than split), else of the even cut.  Positions of
+  // units: within the task, or in all tasks' concatenation.
+  const uint32_t worker = blockIdx.x * kStWarps + warp;
+  uint64_t mine = 0, tasks = 0;
+  const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine, &tasks);
+  const uint32_t per_cta = max(1u, (uint32_t)((total + gridDim.x - 1) / gridDim.x)), per = (per_cta + kStWarps - 1) / kStWarps;
   Cursor c;
-  warp_find(a, QT, kStKeys, lane, u0, mine, c);
+  PartRun run{0, 0, 0};
+  const uint32_t q0 = max(per_cta, 64u);
+  const bool even = !(tasks <= gridDim.x && a.num_seqs <= 32 && warp_parts<1>(a, QT, kStKeys, lane, gridDim.x, q0, q0 + q0 / 4 + 32, blockIdx.x, c, run));
+  uint64_t u0 = (uint64_t)worker * per, u1 = min(u0 + per, total);
+  if (!even) {
+    const uint32_t n = run.parts ? run.end - c.unit : 0, b = c.unit;
+    u0 = run.parts ? b + n * warp / kStWarps : 0;
+    u1 = run.parts ? b + n * (warp + 1) / kStWarps : 0;
+    c.unit = (uint32_t)u0;
+  }
+  // CTAs that hold parts of the task that begins at unit t0
+  const uint64_t cta_units = (uint64_t)per * kStWarps;
+  auto first_cta = [&](uint64_t t0) -> uint32_t { return even ? (uint32_t)(t0 / cta_units) : blockIdx.x - run.part; };
+  auto num_parts = [&](uint64_t t0, uint32_t units) -> uint32_t {
+    return even ? (uint32_t)((t0 + units - 1) / cta_units - t0 / cta_units + 1) : run.parts;
+  };
+  if (lane < 2) parts[warp][lane].units = 0;
+  __syncwarp();
+  if (u0 < u1) {
+  if (even) warp_find(a, QT, kStKeys, lane, u0, mine, c);
 
   // ---- producer: copies of one unit, one per lane ----
   Cursor pc = c;
@@ -338,7 +386,6 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
-    const uint64_t t0 = u - c.unit, t1 = t0 + c.units;       // the task's units
     if (take == c.units) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
@@ -350,8 +397,10 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
         for (int j = 0; j < NT; ++j) *reinterpret_cast<uint32_t*>(op + 8 * j) = T16<T>::pack(o[j][2 * r] * il, o[j][2 * r + 1] * il);
       }
     } else {
-      const bool first = c.unit == 0;
-      float* slot = t.ws.slot(worker, first ? 1 : 0, HD);
+      // the last part of the run goes to the ring, which nothing fills any
+      // more; one before it, with copies under way, to global memory
+      const int which = c.unit == 0 ? 1 : 0;
+      float* slot = u + take == u1 ? reinterpret_cast<float*>(ring) : t.park + (size_t)worker * slot_floats(kStreamRows, HD);
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const int row = g + 8 * r;
@@ -364,14 +413,102 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
 #pragma unroll
         for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(op + 8 * j) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
       }
-      if (first) hdr = {(uint32_t)c.q.row0, c.kvh, (uint32_t)nrow, (uint32_t)((t1 - 1) / per - worker + 1)};
+      if (lane == 0) parts[warp][which] = {u - c.unit, slot, c.units, (uint32_t)c.q.row0, c.kvh, (uint32_t)nrow};
     }
     u += take;
     c.unit += take;
     if (u >= u1) break;
     cursor_next_task(a, c, QT, kStKeys);
   }
-  if (lane == 0) t.ws.head[worker] = hdr;
+  }
+
+  // ---- the CTA's parts: groups of one task each, a warp per group ----
+  if (threadIdx.x < 2) merge[threadIdx.x].units = 0;
+  __syncthreads();
+  {
+    // lane i < 16: part i, in order; a group starts where the task changes
+    const StPart* all = &parts[0][0];
+    const bool have = lane < 2 * kStWarps && all[lane].units != 0;
+    const unsigned long long t0 = have ? all[lane].t0 : 0;
+    const uint32_t valid = __ballot_sync(0xffffffffu, have), below = valid & ((1u << lane) - 1u);
+    const unsigned long long prev = __shfl_sync(0xffffffffu, t0, below ? 31 - __clz(below) : 0);
+    uint32_t starts = __ballot_sync(0xffffffffu, have && (!below || prev != t0));
+    for (int n = 0; n < warp && starts; ++n) starts &= starts - 1;      // the group of this warp ..
+    while (starts) {
+      const int i = __ffs(starts) - 1;
+      const uint32_t later = starts & (starts - 1);
+      const uint32_t members = valid & ~((1u << i) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : 0xFFFFFFFFu);
+      const StPart p = all[i];
+      const uint32_t c0 = first_cta(p.t0), np = num_parts(p.t0, p.units);
+      float* slot = t.ws.slot(blockIdx.x, c0 == blockIdx.x ? 1 : 0, HD);
+      for (uint32_t row = 0; row < p.rows; ++row) {
+        float m = -INFINITY, l = 0.f, o[HD / 32];
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
+        for (uint32_t k = members; k; k &= k - 1) {
+          const float* q = all[__ffs(k) - 1].sums;
+          merge_part<HD>(q[row], q[kStreamRows + row], q + 2 * kStreamRows + row * HD + lane * (HD / 32), m, l, o);
+        }
+        if (np == 1) {
+          merge_out<T, HD>(a, p.row0, p.kvh, row, G, lane, l, o);
+        } else {
+          if (lane == 0) {
+            slot[row] = m;
+            slot[kStreamRows + row] = l;
+          }
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d) slot[2 * kStreamRows + row * HD + lane * (HD / 32) + d] = o[d];
+        }
+      }
+      if (np > 1) {
+        __threadfence();
+        __syncwarp();
+        if (lane == 0 && part_done(t.ws, c0, np)) merge[c0 == blockIdx.x ? 1 : 0] = p;
+      }
+      for (int n = 0; n < kStWarps && starts; ++n) starts &= starts - 1;   // .. and every eighth after it
+    }
+  }
+  __syncthreads();
+  // ---- split tasks that this CTA completed ----
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const StPart p = merge[i];
+    if (!p.units) continue;
+    const uint32_t c0 = first_cta(p.t0), n = num_parts(p.t0, p.units);
+    const int sw = p.rows > 4 ? 1 : p.rows > 2 ? 2 : p.rows > 1 ? 4 : 8;   // warps to a row
+    const int split = warp % sw;
+    for (uint32_t r0 = 0; r0 < p.rows; r0 += kStWarps / sw) {
+      const uint32_t row = r0 + warp / sw;
+      const bool live = row < p.rows;
+      float m = -INFINITY, l = 0.f, o[HD / 32];
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
+      if (live) {
+#pragma unroll 4
+        for (uint32_t k = split; k < n; k += sw) {
+          const float* q = t.ws.slot(c0 + k, k == 0 ? 1 : 0, HD);
+          float po[HD / 32];      // another SM's stores: from L2
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d) po[d] = __ldcg(q + 2 * kStreamRows + row * HD + lane * (HD / 32) + d);
+          merge_part<HD>(__ldcg(q + row), __ldcg(q + kStreamRows + row), po, m, l, o);
+        }
+      }
+      if (sw > 1) {
+        if (lane == 0) {
+          red[warp][HD] = m;
+          red[warp][HD + 1] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) red[warp][lane * (HD / 32) + d] = o[d];
+        __syncthreads();
+        if (split == 0)
+          for (int k = 1; k < sw; ++k)
+            merge_part<HD>(red[warp + k][HD], red[warp + k][HD + 1], &red[warp + k][lane * (HD / 32)], m, l, o);
+        __syncthreads();
+      }
+      if (live && split == 0) merge_out<T, HD>(a, p.row0, p.kvh, row, G, lane, l, o);
+    }
+  }
 }
 
 template <typename T, int HD, bool ROWS8>
@@ -380,7 +517,7 @@ cudaError_t stream_go(const StArgs& t, cudaStream_t st) {
   const cudaError_t e = raise_smem((const void*)&paged_stream_kernel<T, HD, ROWS8>, StShape<HD>::kSmem, ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(t.workers / kStWarps);
+  cfg.gridDim = dim3((uint32_t)t.a.num_sms);
   cfg.blockDim = dim3(kStWarps * 32);
   cfg.dynamicSmemBytes = StShape<HD>::kSmem;
   cfg.stream = st;
@@ -396,21 +533,21 @@ cudaError_t stream_t(const StArgs& t, int hd, cudaStream_t st) {
 
 }  // namespace
 
-uint32_t paged_stream_workers(int num_sms) { return (uint32_t)num_sms * 2 * kStWarps; }
+size_t paged_stream_ws(int num_sms, int hd) {
+  return part_ws_bytes((uint32_t)num_sms, kStreamRows, (uint32_t)hd) +
+         (size_t)num_sms * kStWarps * slot_floats(kStreamRows, (uint32_t)hd) * 4;
+}
 
 cudaError_t paged_stream_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st) {
   StArgs t;
   t.a = a;
-  t.workers = paged_stream_workers(a.num_sms);
-  t.ws = part_ws(a.ws, t.workers, kStreamRows);
-  t.min_per = 1;
+  t.ws = part_ws(a.ws, (uint32_t)a.num_sms, kStreamRows);
+  t.park = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + part_ws_bytes((uint32_t)a.num_sms, kStreamRows, (uint32_t)hd));
   t.box = a.kv.page_size % 16 ? 8 : 16;
   t.sl2 = a.scale * 1.4426950408889634f;
   if (!paged_tensor_map(&t.tmK, a.kv, a.kv.k, hd, t.box) || !paged_tensor_map(&t.tmV, a.kv, a.kv.v, hd, t.box))
     return cudaErrorInvalidValue;
-  const cudaError_t e = dtype == RD_F16 ? stream_t<__half>(t, hd, st) : stream_t<__nv_bfloat16>(t, hd, st);
-  if (e != cudaSuccess) return e;
-  return paged_merge_launch(a, t.ws, t.workers, dtype, hd, st);
+  return dtype == RD_F16 ? stream_t<__half>(t, hd, st) : stream_t<__nv_bfloat16>(t, hd, st);
 }
 
 }  // namespace nnz

@@ -327,26 +327,13 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_MISC + 128);
   const uint32_t G = a.n_q / a.kv.n_kv;
   const int PT = (int)t.pt, QT = 2 * PT;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 2);     // the products and warp 11
-    }
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
-      mbar_init(pv_done + i, 1);
-    }
-    for (int i = 0; i < kPres; ++i) {
-      mbar_init(v_ready + i, 1);
-      mbar_init(pres_full + i, 1);
-    }
-    for (int i = 0; i < kSegs; ++i) {
-      mbar_init(seg_full + i, 1);
-      mbar_init(seg_empty + i, 10);
-    }
+  pdl_launch();       // the merge kernel may be set up (it waits for this one's end)
+  // every barrier by its own thread; arrivals: 2 for a free stage (the products
+  // and warp 11), 4 for P (a warp each), 10 for a part's end, else 1
+  static_assert(S::kBars <= kUmThreads);
+  if (threadIdx.x < (uint32_t)S::kBars) {
+    uint64_t* b = kv_full + threadIdx.x;
+    mbar_init(b, b >= kv_empty && b < q_full ? 2 : b == p_full || b == p_full + 1 ? 4 : b >= seg_empty ? 10 : 1);
     fence_barrier_init();
   }
   if (warp == 8 && lane < 3) {
@@ -357,8 +344,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tslot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_wait();
-  pdl_launch();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -388,72 +373,13 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     const uint64_t total = warp_total(a, QT, kUmKeys, lane, blockIdx.x == 0, mine, &tasks);
     const uint32_t P = t.workers, per = max(1u, (uint32_t)((total + P - 1) / P));
     // One part per CTA where that costs no more than kPartCost units over the
-    // even cut: with at most P tasks, the smallest q that cuts them into parts
-    // of at most q units, P of them or fewer.
+    // even cut.
     Cursor c;
-    uint32_t part = 0, parts = 0, end = 0;     // one-part runs: part of c's task, its end
-    uint64_t u = 0, u1 = 0;                    // even runs: units [u, u1)
-    bool more = false, even = true;
-    if (tasks <= P && a.num_seqs <= 32) {
-      const SeqInfo q = (uint32_t)lane < a.num_seqs ? seq_info(a, (uint32_t)lane) : SeqInfo{0, 0, 0, 0, 0};
-      const int nt = (q.rows + QT - 1) / QT, inc = warp_scan(nt, lane), D = __shfl_sync(0xffffffffu, inc, 31);
-      // entry j (a tile of one sequence, for every kv head): lanes hold j = lane + 32 i
-      constexpr int kPer = 5;                  // P <= 160
-      uint32_t eu[kPer], es[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int j = lane + 32 * i;
-        eu[i] = es[i] = 0;
-        if (32 * i >= D) continue;
-        // its sequence: the lanes whose tiles end at or before j
-        int s = 0;
-        for (uint32_t l = 0; l < a.num_seqs; ++l) s += __shfl_sync(0xffffffffu, inc, (int)l) <= j ? 1 : 0;
-        const int first = __shfl_sync(0xffffffffu, inc - nt, s & 31);
-        if (j < D) {
-          es[i] = (uint32_t)s;
-          eu[i] = tile_units(seq_info(a, (uint32_t)s), j - first, QT, kUmKeys);
-        }
-      }
-      const uint32_t cap = P / a.kv.n_kv;      // parts of all entries, per kv head
-      for (uint32_t q_ = per; q_ <= per + kPartCost && D <= 32 * kPer; ++q_) {
-        uint32_t n = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) n += 32 * i < D ? (eu[i] + q_ - 1) / q_ : 0;
-        if (__reduce_add_sync(0xffffffffu, n) > cap) continue;
-        // parts in order of entry, kv head, part
-        even = false;
-        uint32_t before = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if (32 * i >= D) continue;
-          const uint32_t np = (eu[i] + q_ - 1) / q_, all = np * a.kv.n_kv;
-          const uint32_t incl = before + warp_scan(all, lane);
-          const uint32_t hit = __ballot_sync(0xffffffffu, blockIdx.x < incl && blockIdx.x >= incl - all);
-          if (hit) {
-            const int l = __ffs(hit) - 1;
-            const uint32_t rel = blockIdx.x - __shfl_sync(0xffffffffu, incl - all, l);
-            parts = __shfl_sync(0xffffffffu, np, l);
-            c.units = __shfl_sync(0xffffffffu, eu[i], l);
-            c.s = __shfl_sync(0xffffffffu, es[i], l);
-            c.kvh = rel / parts;
-            part = rel % parts;
-            c.qt = l + 32 * i - (int)__shfl_sync(0xffffffffu, inc - nt, (int)c.s);
-            c.unit = c.units * part / parts;
-            end = c.units * (part + 1) / parts;
-            more = true;
-          }
-          before = __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (more) c.q = seq_info(a, c.s);
-        break;
-      }
-    }
-    if (even) {
-      u = (uint64_t)blockIdx.x * per;
-      u1 = min(u + per, total);
-      more = u < u1;
-      if (more) warp_find(a, QT, kUmKeys, lane, u, mine, c);
-    }
+    PartRun run{0, 0, 0};
+    uint64_t u = (uint64_t)blockIdx.x * per, u1 = min(u + per, total);     // even cut
+    const bool even = !(tasks <= P && a.num_seqs <= 32 && warp_parts<5>(a, QT, kUmKeys, lane, P, per, per + kPartCost, blockIdx.x, c, run));
+    bool more = even ? u < u1 : run.parts != 0;
+    if (even && more) warp_find(a, QT, kUmKeys, lane, u, mine, c);
 
     const uint32_t nb = kUmKeys / t.box;
     const uint32_t bi = (uint32_t)lane % nb, half = (uint32_t)lane / nb;
@@ -463,7 +389,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       // ---- the next part: to the other warps ----
       Segment o{};
       if (more) {
-        o.take = even ? (uint32_t)min((uint64_t)(c.units - c.unit), u1 - u) : end - c.unit;
+        o.take = even ? (uint32_t)min((uint64_t)(c.units - c.unit), u1 - u) : run.end - c.unit;
         o.unit = c.unit;
         o.s = c.s;
         o.kvh = c.kvh;
@@ -479,7 +405,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
             o.n[i] = un > c.unit ? min(un - c.unit, o.take) : 0;
           }
         if (!even) {
-          o.parts = parts > 1 ? parts : 0;
+          o.parts = run.parts > 1 ? run.parts : 0;
         } else if (o.take != c.units) {
           const uint64_t t0 = u - c.unit;
           o.parts = (uint32_t)((t0 + c.units - 1) / per - t0 / per + 1);
@@ -737,11 +663,11 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         uint16_t* op = a.out + (int64_t)(g.row0 + tok) * a.out_stride + (int64_t)(g.kvh * G + r % G) * HD;
         float* slot = t.ws.slot(blockIdx.x, first ? 1 : 0, HD);
         float* part = slot + 2 * t.ws.R + (size_t)rr * 4;   // [HD / 4][R][4]: lanes side by side
+        if (first && !whole) hdr = {(uint32_t)g.row0, g.kvh, (uint32_t)g.rows * G, g.parts};
         if (live && !whole) {
           slot[rr] = l == 0.f ? -INFINITY : m;
           slot[t.ws.R + rr] = l;
         }
-        if (first && !whole) hdr = {(uint32_t)g.row0, g.kvh, (uint32_t)g.rows * G, g.parts};
         if (g.n[x]) {
           wait(pv_done + x, ns - 1);
           tc_fence_after();
@@ -797,6 +723,8 @@ cudaError_t umma_go(const UmArgs& t, cudaStream_t st) {
 }
 
 }  // namespace
+
+size_t paged_umma_ws(int num_sms, int hd) { return part_ws_bytes((uint32_t)num_sms, kUmmaRows, (uint32_t)hd); }
 
 cudaError_t paged_umma_launch(const PagedAttnArgs& a, int dtype, int hd, cudaStream_t st) {
   UmArgs t;
