@@ -16,6 +16,7 @@
 //
 // Absent pages and keys past the length are not loaded or not trusted: their
 // scores are masked, their V rows zeroed in shared memory.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -23,6 +24,8 @@
 
 #include "paged_sched.cuh"
 #include "paged_tma.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace nnz {
 
@@ -54,6 +57,8 @@ struct StArgs {
   PagedAttnArgs a;
   PartWs ws;
   float* park;         // a slot per warp
+  uint32_t cluster;    // > 1: one sequence, CTAs in clusters
+  uint32_t clusters;   // of a kv head (used as its length asks)
   uint32_t box;        // keys per copy: 16 or 8
   float sl2;           // scale * log2(e)
 };
@@ -123,7 +128,8 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   extern __shared__ uint8_t smem_raw[];
   __shared__ StPart parts[kStWarps][2];     // that start before the warp's run or within it
   __shared__ StPart merge[2];                // split tasks whose last part is this CTA's
-  __shared__ float red[kStWarps][HD + 2];
+  __shared__ __align__(16) float gather[kStreamRows * (HD + 2)];     // a CTA's sums in a cluster; warps' in a merge
+  float (*red)[HD + 2] = reinterpret_cast<float (*)[HD + 2]>(gather);
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PagedAttnArgs& a = t.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -137,24 +143,52 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   __syncwarp();
   const int G = (int)(a.n_q / a.kv.n_kv);
   const int QT = (int)a.max_new;           // one tile holds all rows
-  // The run of this warp: of a part of one task that the CTA has for itself
-  // where there are few tasks (64 units to a CTA or more: a task that fits one
-  // CTA is cheaper there than split), else of the even cut.  Positions of
-  // units: within the task, or in all tasks' concatenation.
+  // The run of this warp.  One sequence: its part of the head that the cluster
+  // has.  Few tasks: of a part of one task that the CTA has for itself.  Else:
+  // of the even cut.  Positions of units: within the task, or (even cut) in
+  // all tasks' concatenation.
   const uint32_t worker = blockIdx.x * kStWarps + warp;
-  uint64_t mine = 0, tasks = 0;
-  const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine, &tasks);
-  const uint32_t per_cta = max(1u, (uint32_t)((total + gridDim.x - 1) / gridDim.x)), per = (per_cta + kStWarps - 1) / kStWarps;
   Cursor c;
   PartRun run{0, 0, 0};
-  const uint32_t q0 = max(per_cta, 64u);
-  const bool even = !(tasks <= gridDim.x && a.num_seqs <= 32 && warp_parts<1>(a, QT, kStKeys, lane, gridDim.x, q0, q0 + q0 / 4 + 32, blockIdx.x, c, run));
-  uint64_t u0 = (uint64_t)worker * per, u1 = min(u0 + per, total);
-  if (!even) {
-    const uint32_t n = run.parts ? run.end - c.unit : 0, b = c.unit;
-    u0 = run.parts ? b + n * warp / kStWarps : 0;
-    u1 = run.parts ? b + n * (warp + 1) / kStWarps : 0;
-    c.unit = (uint32_t)u0;
+  bool even = false;
+  uint64_t mine = 0, u0 = 0, u1 = 0;
+  uint32_t per = 1;
+  if (t.cluster > 1) {
+    const uint32_t id = blockIdx.x / t.cluster;
+    c.s = 0;
+    c.kvh = id / t.clusters;
+    c.qt = 0;
+    c.q = seq_info(a, 0);
+    if (worker == 0 && lane == 0 && seq_bad(a, c.q)) atomicOr(a.err, ERR_BAD_PAGE);
+    if (c.q.rows > 0) {
+      c.units = tile_units(c.q, 0, QT, kStKeys);
+      // as many clusters as get four units to a warp
+      const uint32_t warps = t.cluster * kStWarps;
+      run.parts = min(t.clusters, max(1u, c.units / (4 * warps)));
+      run.part = id % t.clusters;
+      if (run.part < run.parts) {
+        const uint32_t n = run.parts * warps, w = run.part * warps + blockIdx.x % t.cluster * kStWarps + warp;
+        u0 = (uint64_t)c.units * w / n;
+        u1 = (uint64_t)c.units * (w + 1) / n;
+        c.unit = (uint32_t)u0;
+      }
+    }
+  } else {
+    uint64_t tasks = 0;
+    const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine, &tasks);
+    const uint32_t per_cta = max(1u, (uint32_t)((total + gridDim.x - 1) / gridDim.x));
+    per = (per_cta + kStWarps - 1) / kStWarps;
+    even = !(tasks <= gridDim.x && a.num_seqs <= 32 &&
+             warp_parts<1>(a, QT, kStKeys, lane, gridDim.x, per_cta, per_cta + per_cta / 4 + 8, blockIdx.x, c, run));
+    if (even) {
+      u0 = (uint64_t)worker * per;
+      u1 = min(u0 + per, total);
+    } else if (run.parts) {
+      const uint32_t n = run.end - c.unit;
+      u0 = c.unit + n * warp / kStWarps;
+      u1 = c.unit + n * (warp + 1) / kStWarps;
+      c.unit = (uint32_t)u0;
+    }
   }
   // CTAs that hold parts of the task that begins at unit t0
   const uint64_t cta_units = (uint64_t)per * kStWarps;
@@ -386,7 +420,7 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
-    if (take == c.units) {
+    if (take == c.units && t.cluster <= 1) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const int row = g + 8 * r;
@@ -420,6 +454,78 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
     if (u >= u1) break;
     cursor_next_task(a, c, QT, kStKeys);
   }
+  }
+
+  if (t.cluster > 1) {
+    // ---- one task: the CTA's parts, then the cluster's in its first CTA ----
+    cg::cluster_group cl = cg::this_cluster();
+    if (run.part >= run.parts) return;                    // the whole cluster
+    __syncthreads();
+    const uint32_t rows = (uint32_t)(c.q.rows * G), rank = blockIdx.x % t.cluster, id = blockIdx.x / t.cluster;
+    for (uint32_t row = warp; row < rows; row += kStWarps) {
+      float m = -INFINITY, l = 0.f, o[HD / 32];
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
+      for (int k = 0; k < 2 * kStWarps; ++k) {
+        const StPart& p = parts[k >> 1][k & 1];
+        if (!p.units) continue;
+        merge_part<HD>(p.sums[row], p.sums[kStreamRows + row], p.sums + 2 * kStreamRows + row * HD + lane * (HD / 32), m, l, o);
+      }
+      float* q = gather + row * (HD + 2);
+      if (lane == 0) {
+        q[HD] = m;
+        q[HD + 1] = l;
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d) q[lane * (HD / 32) + d] = o[d];
+    }
+    cl.sync();
+    // CTA r of the cluster sums rows r, r + cluster, ..
+    for (uint32_t row = rank + t.cluster * warp; row < rows; row += t.cluster * kStWarps) {
+      float m = -INFINITY, l = 0.f, o[HD / 32];
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
+#pragma unroll 4
+      for (uint32_t k = 0; k < t.cluster; ++k) {
+        const float* q = cl.map_shared_rank(gather, k) + row * (HD + 2);
+        float po[HD / 32];
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) po[d] = q[lane * (HD / 32) + d];
+        merge_part<HD>(q[HD], q[HD + 1], po, m, l, o);
+      }
+      if (run.parts == 1) {
+        merge_out<T, HD>(a, (uint32_t)c.q.row0, c.kvh, row, G, lane, l, o);
+      } else {
+        float* slot = t.ws.slot(id, 0, HD);
+        if (lane == 0) {
+          slot[row] = m;
+          slot[kStreamRows + row] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) slot[2 * kStreamRows + row * HD + lane * (HD / 32) + d] = o[d];
+      }
+    }
+    if (run.parts > 1) __threadfence();
+    cl.sync();      // the CTAs' sums have been read, the cluster's are stored
+    if (run.parts == 1 || rank != 0) return;
+    if (threadIdx.x == 0) merge[0].units = part_done(t.ws, id - run.part, run.parts) ? 1u : 0u;
+    __syncthreads();
+    if (!merge[0].units) return;
+    for (uint32_t row = warp; row < rows; row += kStWarps) {
+      float m = -INFINITY, l = 0.f, o[HD / 32];
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d) o[d] = 0.f;
+#pragma unroll 4
+      for (uint32_t k = 0; k < run.parts; ++k) {
+        const float* q = t.ws.slot(id - run.part + k, 0, HD);
+        float po[HD / 32];
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) po[d] = __ldcg(q + 2 * kStreamRows + row * HD + lane * (HD / 32) + d);
+        merge_part<HD>(__ldcg(q + row), __ldcg(q + kStreamRows + row), po, m, l, o);
+      }
+      merge_out<T, HD>(a, (uint32_t)c.q.row0, c.kvh, row, G, lane, l, o);
+    }
+    return;
   }
 
   // ---- the CTA's parts: groups of one task each, a warp per group ----
@@ -511,17 +617,65 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   }
 }
 
+// Clusters for one sequence (its parts then meet through distributed shared
+// memory; through the workspace they take 5 us longer): 8 CTAs to a head where
+// the page table holds at most 4096 keys, else as many clusters of 4 as the
+// device runs at once.  One row, 16 / 8 heads of 128, us by length:
+//   keys       515   2048   8192   32767
+//   8 x 1      6.7    8.7   18.1    51.5
+//   4 x 4      8.2   11.5   16.4    32.8
+//   even cut  11.5   12.8   20.9    36.1
+template <typename K>
+void stream_clusters(K* fn, StArgs& t, cudaLaunchConfig_t cfg, std::atomic<int> (&fits)[9]) {
+  t.cluster = t.clusters = 1;
+  if (t.a.num_seqs != 1) return;
+  const uint64_t keys = (uint64_t)t.a.table_stride * t.a.kv.page_size;
+  for (uint32_t C = keys <= 4096 ? 8 : 4; C >= 4; C /= 2) {
+    // clusters of C that the device runs at once (asked once)
+    int n = fits[C].load(std::memory_order_relaxed);
+    if (n == 0) {
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = C;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(C);
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = -1;
+      }
+      fits[C].store(n, std::memory_order_relaxed);
+    }
+    const uint32_t n_kv = t.a.kv.n_kv;
+    if (n >= (int)n_kv) {
+      t.cluster = C;
+      t.clusters = C == 8 ? 1u : (uint32_t)n / n_kv;
+      return;
+    }
+  }
+}
+
 template <typename T, int HD, bool ROWS8>
-cudaError_t stream_go(const StArgs& t, cudaStream_t st) {
+cudaError_t stream_go(StArgs t, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
-  const cudaError_t e = raise_smem((const void*)&paged_stream_kernel<T, HD, ROWS8>, StShape<HD>::kSmem, ready);
+  static std::atomic<int> fits[9];
+  const auto fn = &paged_stream_kernel<T, HD, ROWS8>;
+  const cudaError_t e = raise_smem((const void*)fn, StShape<HD>::kSmem, ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((uint32_t)t.a.num_sms);
   cfg.blockDim = dim3(kStWarps * 32);
   cfg.dynamicSmemBytes = StShape<HD>::kSmem;
   cfg.stream = st;
-  return cudaLaunchKernelEx(&cfg, &paged_stream_kernel<T, HD, ROWS8>, t);
+  stream_clusters(fn, t, cfg, fits);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = t.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(t.cluster > 1 ? t.cluster * t.clusters * t.a.kv.n_kv : (uint32_t)t.a.num_sms);
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, t);
 }
 
 template <typename T>
