@@ -205,7 +205,6 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   Cursor pc = c;
   uint32_t left = (uint32_t)(u1 - u0);      // units still to be issued
   const uint32_t nb = kStKeys / t.box;       // copies along the keys of a unit
-  const uint32_t ncopy = nb * 2 * S::kHalves;
   uint32_t page0 = 0, npage = 0;             // key boxes whose page numbers the lanes hold
   int my_page = -1;
   uint32_t my_at = 0;
@@ -227,20 +226,23 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
         }
       }
     }
-    // lane i copies box i % nb of part i / nb (K halves, then V halves)
-    const uint32_t bi = (uint32_t)lane % nb, part = (uint32_t)lane / nb;
-    const int pg = __shfl_sync(0xffffffffu, my_page, (int)(b0 - page0 + bi));
-    const uint32_t at = __shfl_sync(0xffffffffu, my_at, (int)(b0 - page0 + bi));
-    const bool go = (uint32_t)lane < ncopy && pg >= 0;
-    const uint32_t mask = __ballot_sync(0xffffffffu, go);
-    if (lane == 0) {
-      there[stg] = mask & ((1u << nb) - 1u);
-      mbar_arrive_expect_tx(&bars[stg], (uint32_t)__popc(mask) * t.box * 128);
+    // one elected lane issues (a lane each takes the compiler's loop over
+    // divergent operands, about 100 cycles a copy)
+    const int i0 = (int)(b0 - page0), i1 = (int)(i0 + nb - 1);
+    const int p0 = __shfl_sync(0xffffffffu, my_page, i0), p1 = __shfl_sync(0xffffffffu, my_page, i1);
+    const int a0 = (int)__shfl_sync(0xffffffffu, my_at, i0), a1 = (int)__shfl_sync(0xffffffffu, my_at, i1);
+    uint8_t* dst = ring + stg * S::kStageB;
+    if (elect_one()) {
+      const uint32_t have = (p0 >= 0 ? 1u : 0u) | (nb == 2 && p1 >= 0 ? 2u : 0u);
+      there[stg] = have;
+      mbar_arrive_expect_tx(&bars[stg], (uint32_t)__popc(have) * 2 * S::kHalves * t.box * 128);
+#pragma unroll
+      for (int part = 0; part < 2 * S::kHalves; ++part) {
+        const CUtensorMap* tm = part < S::kHalves ? &t.tmK : &t.tmV;
+        if (p0 >= 0) tma_load_4d(dst + part * S::kBoxB, tm, part % S::kHalves * 64, a0, (int)pc.kvh, p0, &bars[stg]);
+        if (nb == 2 && p1 >= 0) tma_load_4d(dst + part * S::kBoxB + 8 * 128, tm, part % S::kHalves * 64, a1, (int)pc.kvh, p1, &bars[stg]);
+      }
     }
-    __syncwarp();
-    if (go)
-      tma_load_4d(ring + stg * S::kStageB + part * S::kBoxB + bi * t.box * 128, part < S::kHalves ? &t.tmK : &t.tmV,
-                  (int)(part % S::kHalves) * 64, (int)at, (int)pc.kvh, pg, &bars[stg]);
     __syncwarp();
     --left;
     if (++pc.unit == pc.units) {
@@ -321,35 +323,40 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
         }
       }
       uint32_t pa[2][2];       // [key half][row half]
-      float pv[NR][4];
+      float pv[NR][4], mx[NR];
+      const bool masked = !all_there || key0 + kStKeys > seen_all;
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        float mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int k = (e >> 1) * 8 + 2 * q4 + (e & 1);
-          const float x = s[e >> 1][2 * r + (e & 1)] * t.sl2;
-          pv[r][e] = key0 + k < limit[r] && present(k) ? x : -INFINITY;
-          mx = fmaxf(mx, pv[r][e]);
+          pv[r][e] = s[e >> 1][2 * r + (e & 1)] * t.sl2;
+          if (masked && !(key0 + k < limit[r] && present(k))) pv[r][e] = -INFINITY;
         }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[r], mx);
-        const float ms = mn == -INFINITY ? 0.f : mn;      // nothing seen yet: every p is exp2(-inf) = 0
-        const float al = exp2f(m[r] - ms);
-        m[r] = mn;
-        float sum = 0.f;
+        mx[r] = fmaxf(fmaxf(pv[r][0], pv[r][1]), fmaxf(pv[r][2], pv[r][3]));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[NR - 1] > m[NR - 1])) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pv[r][e] = exp2f(pv[r][e] - ms);
-          sum += pv[r][e];
-        }
-        l[r] = l[r] * al + sum;
+        for (int r = 0; r < NR; ++r) {
+          const float mn = fmaxf(m[r], mx[r]);
+          const float al = m[r] == mn ? 1.f : ex2(m[r] - mn);     // 0 at the first key seen
+          m[r] = mn;
+          l[r] *= al;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          o[j][2 * r] *= al;
-          o[j][2 * r + 1] *= al;
+          for (int j = 0; j < NT; ++j) {
+            o[j][2 * r] *= al;
+            o[j][2 * r + 1] *= al;
+          }
         }
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float ms = m[r] == -INFINITY ? 0.f : m[r];      // nothing seen yet: every p is 2^-inf = 0
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[r][e] = ex2(pv[r][e] - ms);
+        l[r] += (pv[r][0] + pv[r][1]) + (pv[r][2] + pv[r][3]);
         pa[0][r] = T16<T>::pack(pv[r][0], pv[r][1]);
         pa[1][r] = T16<T>::pack(pv[r][2], pv[r][3]);
       }

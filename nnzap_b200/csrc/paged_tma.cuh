@@ -10,6 +10,21 @@
 
 namespace nnz {
 
+// One lane of the warp, known as such to the compiler: behind a plain test of
+// the lane it takes every tcgen05.mma for divergent code (S: 900 -> 585 cycles
+// for its 8 instructions, P V: 1900 -> 700).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // x: dim (0 or 64), y: token within the page.
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tm, int x, int y, int head, int page, uint64_t* bar) {
   asm volatile(

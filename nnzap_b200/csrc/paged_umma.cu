@@ -127,11 +127,6 @@ __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[31])
       : "memory");
 }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 
 // Two f32 at a time (one instruction each).
 __device__ __forceinline__ uint64_t pair2(float x, float y) {
@@ -238,15 +233,6 @@ __device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32
   const float2 t = split2(add2(acc[0], acc[1]));
   sum = t.x + t.y;
   top = fmaxf(mx[0], mx[1]);
-}
-
-// One lane of the warp, known as such to the compiler: behind a plain test of
-// the lane it takes every tcgen05.mma for divergent code (S: 900 -> 585 cycles
-// for its 8 instructions, P V: 1900 -> 700).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
-  return p != 0;
 }
 
 template <bool BF16>
