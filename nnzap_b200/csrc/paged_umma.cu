@@ -18,15 +18,17 @@
 // m, rescale O and compute the unit again, which after the first units is
 // rare.  P up to 256 costs no precision, the sums are f32.
 //
-// Roles: warps 0-3 and 4-7 softmax and epilogue of row tiles 0 and 1 (thread =
-// TMEM lane = row), warp 8 finds the CTA's run of units, hands its parts to the
-// others and loads them (Q, then K and V tiles into one ring, boxes of one page
-// each, one per lane), warp 9 MMA issue, warp 11 cleans the V tiles at the
-// diagonal and at the end (10 only makes the third warpgroup whole).  Boxes of absent pages and past the length are
+// Roles: warps 0-7 and 8-15 softmax and epilogue of row tiles 0 and 1 (TMEM lane
+// = row; warps 0-3 of a tile have keys 0-63 of a unit and the lower half of the
+// output's dims, 4-7 the others), warp 16 finds the CTA's run of units, hands
+// its parts to the others and loads them (Q, then K and V tiles into one ring,
+// boxes of one page each, one per lane), warp 17 MMA issue, warp 19 cleans the
+// V tiles at the diagonal and at the end.  Boxes of absent pages and past the length are
 // loaded from beyond the pool's last page: the copy engine fills them with
 // zeros, so no stale byte meets the product.
 //
-// TMEM: S / P of the two row tiles at columns 0 and 128, O at 256 and 384.
+// TMEM: S of the two row tiles at columns 0 and 128, O at 256 and 384; P of keys
+// 0-63 and 64-127 over the first 32 columns of their halves of S.
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -42,11 +44,12 @@ namespace nnz {
 namespace {
 
 constexpr int kUmKeys = 128;
-constexpr int kUmThreads = 384;
-// Registers a thread: 384 x 168 at launch; the two softmax warpgroups take 216
-// each (a unit's P and two quarters of S), the third goes down to 72: 2 x 128
-// x 216 + 128 x 72 = 64512.
-constexpr int kUmRegsSoftmax = 216, kUmRegsIssue = 72;
+constexpr int kUmThreads = 640;
+// Registers a thread: 640 x 96 at launch; the four softmax warpgroups take 104
+// each (32 words of P, two eighths of S), the fifth goes down to 64: 4 x 128 x
+// 104 + 128 x 64 = 61440.
+constexpr int kUmRegsSoftmax = 104, kUmRegsIssue = 64;
+constexpr int kWTma = 16, kWMma = 17, kWClean = 19;      // warps (18 only makes the fifth warpgroup whole)
 constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
 constexpr uint32_t kPartCost = 3;                 // what a part costs besides its units, in units (queries, epilogue, merge)
@@ -61,7 +64,8 @@ struct UmShape {
   static constexpr uint32_t OFF_BAR = OFF_KV + kStages * kTileB;
   static constexpr int kBars = 2 * kStages + 8 + 2 * kPres + 2 * kSegs;
   static constexpr uint32_t OFF_MISC = OFF_BAR + kBars * 8;
-  static constexpr uint32_t kSmem = OFF_MISC + 128 + kSegs * 128 + 1024;
+  static constexpr uint32_t OFF_SEG = OFF_MISC + 64, OFF_XT = OFF_SEG + kSegs * 80;
+  static constexpr uint32_t kSmem = OFF_XT + 1024 + 1024;
 };
 
 struct UmArgs {
@@ -104,6 +108,20 @@ __device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
         "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
+}
+__device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
 }
 // Waits for this thread's TMEM loads; v is tied to the wait so that no use of
 // it can be scheduled before.
@@ -175,13 +193,13 @@ __device__ __forceinline__ float2 ex2_fma(float a, float b) {
   return split2(mul2(p, pair2(__int_as_float((__float_as_int(k.x) << 23) + 0x3F800000), __int_as_float((__float_as_int(k.y) << 23) + 0x3F800000))));
 }
 
-// Sets the scores of a row's 128 keys that it does not see to -infinity, in
+// Sets the scores of 64 keys of a row that it does not see to -infinity, in
 // TMEM: it sees the first `end`, on pages whose bit is set (one bit per 2^sh
 // keys).  (Rolled: this runs a few times per task, and instructions have to
 // be fetched.)
 __device__ __forceinline__ void um_mask(uint32_t tS, int end, uint32_t bits, uint32_t sh) {
 #pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
     uint32_t see = end >= 32 * c + 32 ? 0xFFFFFFFFu : end <= 32 * c ? 0u : (1u << (end - 32 * c)) - 1u;
     const uint32_t pg = bits >> ((32 * c) >> sh);          // first page bit of this quarter
     if (sh >= 5) {
@@ -200,22 +218,22 @@ __device__ __forceinline__ void um_mask(uint32_t tS, int end, uint32_t bits, uin
   }
 }
 
-// P = 2^(S sl2 - ms) of a row's 128 keys as 64 words of the pool's type, their
-// f32 sum, and the largest score.  The next quarter of S is on its way while
-// one is worked on.
+// P = 2^(S sl2 - ms) of 64 keys of a row as 32 words of the pool's type, their
+// f32 sum, and the largest score.  The next 16 of S are on their way while some
+// are worked on.
 template <typename T>
-__device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32_t (&w)[64], float& sum, float& top) {
+__device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32_t (&w)[32], float& sum, float& top) {
   const uint64_t k2 = pair2(sl2, sl2), m2 = pair2(-ms, -ms);
   uint64_t acc[2] = {0ull, 0ull};
   float mx[2] = {-INFINITY, -INFINITY};
-  uint32_t v[2][32];
-  tm_ld32(tS, v[0]);
+  uint32_t v[2][16];
+  tm_ld16(tS, v[0]);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     tm_wait_ld(v[c & 1]);
-    if (c < 3) tm_ld32(tS + 32 * (c + 1), v[(c + 1) & 1]);
+    if (c < 3) tm_ld16(tS + 16 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
+    for (int e = 0; e < 16; e += 2) {
       const float a = __uint_as_float(v[c & 1][e]), b = __uint_as_float(v[c & 1][e + 1]);
       mx[(e >> 1) & 1] = fmaxf(fmaxf(mx[(e >> 1) & 1], a), b);
       const float2 y = split2(fma2(pair2(a, b), k2, m2));
@@ -223,17 +241,28 @@ __device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32
       // special-function units alone take 2 x 1024 cycles per unit
       const float2 q = ((e >> 1) & 3) == 3 ? ex2_fma(y.x, y.y) : make_float2(ex2(y.x), ex2(y.y));
       acc[(e >> 1) & 1] = add2(acc[(e >> 1) & 1], pair2(q.x, q.y));
-      w[16 * c + e / 2] = T16<T>::pack(q.x, q.y);
+      w[8 * c + e / 2] = T16<T>::pack(q.x, q.y);
     }
-    // the quarter's work stays before the wait for the next one
-    uint32_t* q = w + 16 * c;
-    asm volatile("" : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]), "+r"(q[8]),
-                      "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15]));
+    // the words stay before the wait for the next ones
+    uint32_t* q = w + 8 * c;
+    asm volatile("" : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]));
   }
   const float2 t = split2(add2(acc[0], acc[1]));
   sum = t.x + t.y;
   top = fmaxf(mx[0], mx[1]);
 }
+
+// The two warps that share 32 rows: whether any of their 64 threads says so.
+__device__ __forceinline__ bool pair_any(int bar, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred a, b;\n setp.ne.u32 a, %2, 0;\n bar.red.or.pred b, %1, 64, a;\n selp.u32 %0, 1, 0, b;\n}\n"
+      : "=r"(r)
+      : "r"(bar), "r"((uint32_t)p)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void pair_sync(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
 
 template <bool BF16>
 __host__ __device__ constexpr uint32_t um_idesc(int M, int N) {
@@ -247,7 +276,7 @@ __device__ __forceinline__ uint32_t bad_mask(uint32_t w) {
   return ((w & e) == e ? 0xFFFFu : 0u) | (((w >> 16) & e) == e ? 0xFFFF0000u : 0u);
 }
 
-// The part of one task in a CTA's run, as warp 8 hands it to the others.
+// The part of one task in a CTA's run, as warp 16 hands it to the others.
 struct Segment {
   uint32_t take;       // units (0: the run is over)
   uint32_t unit;       // first unit within the task
@@ -302,31 +331,35 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint64_t* q_full = kv_empty + S::kStages;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;        // [2] S of a row tile complete
-  uint64_t* p_full = s_full + 2;         // [2] P written, O rescaled (4 warps)
+  uint64_t* p_full = s_full + 2;         // [2] P written, O rescaled (8 warps)
   uint64_t* pv_done = p_full + 2;        // [2] P V complete
   uint64_t* v_ready = pv_done + 2;       // [kPres] a unit's V tile is ready for the product
   uint64_t* pres_full = v_ready + kPres; // [kPres] page mask of a unit written
   uint64_t* seg_full = pres_full + kPres;   // [kSegs]
-  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 10 other warps are done with it
+  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 18 other warps are done with it
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + S::OFF_MISC);
+  volatile uint32_t* absent = tslot + 1 + kPres;   // an absent page was met
   volatile uint32_t* pres = tslot + 1;   // [kPres] one bit per box of the unit: page present
-  Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_MISC + 128);
+  Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_SEG);
+  static_assert(sizeof(Segment) <= 80 && S::kSmem <= 232448);
+  uint32_t* xt = reinterpret_cast<uint32_t*>(sm + S::OFF_XT);     // [2][128] what the two threads of a row tell each other
   const uint32_t G = a.n_q / a.kv.n_kv;
   const int PT = (int)t.pt, QT = 2 * PT;
   pdl_launch();       // the merge kernel may be set up (it waits for this one's end)
   // every barrier by its own thread; arrivals: 2 for a free stage (the products
-  // and warp 11), 4 for P (a warp each), 10 for a part's end, else 1
+  // and warp 19), 8 for P (a warp each), 18 for a part's end, else 1
   static_assert(S::kBars <= kUmThreads);
+  if (threadIdx.x == 0) *absent = 0;
   if (threadIdx.x < (uint32_t)S::kBars) {
     uint64_t* b = kv_full + threadIdx.x;
-    mbar_init(b, b >= kv_empty && b < q_full ? 2 : b == p_full || b == p_full + 1 ? 4 : b >= seg_empty ? 10 : 1);
+    mbar_init(b, b >= kv_empty && b < q_full ? 2 : b == p_full || b == p_full + 1 ? 8 : b >= seg_empty ? 18 : 1);
     fence_barrier_init();
   }
-  if (warp == 8 && lane < 3) {
+  if (warp == kWTma && lane < 3) {
     const CUtensorMap* tm = lane == 0 ? &t.tmQ : lane == 1 ? &t.tmK : &t.tmV;
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
   }
-  if (warp == 9) {
+  if (warp == kWMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tslot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -340,7 +373,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     if (!failed) failed = !mbar_wait(bar, parity & 1u, a.err);
   };
 
-  // part k of the run; warps 0-7, 9 and 11 take them in order from warp 8
+  // part k of the run; warps 0-15, 17 and 19 take them in order from warp 16
   auto segment = [&](uint32_t k, Segment& g) -> bool {
     wait(seg_full + k % kSegs, k / kSegs);
     g = segs[k % kSegs];
@@ -351,9 +384,9 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     if (lane == 0) mbar_arrive1(seg_empty + k % kSegs);
   };
 
-  if (warp >= 8) {
+  if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUmRegsIssue));
-  if (warp == 8) {
+  if (warp == kWTma) {
     // ---------------- the run, and its TMA ----------------
     uint64_t mine = 0, tasks = 0;
     const uint64_t total = warp_total(a, QT, kUmKeys, lane, blockIdx.x == 0, mine, &tasks);
@@ -418,11 +451,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         const uint32_t pi = key / a.kv.page_size;
         at = key - pi * a.kv.page_size;
         const int p = __ldg(pages + pi);
-        if (p >= 0 && (uint32_t)p >= a.kv.num_pages) {
-          atomicOr(a.err, ERR_BAD_PAGE);
-          return -1;
-        }
-        return p;
+        if ((uint32_t)p < a.kv.num_pages) return p;
+        if (p >= 0) atomicOr(a.err, ERR_BAD_PAGE);
+        *absent = 1;
+        return -1;
       };
       uint32_t at, nat = 0;
       int pg = page_of(0, at), npg = -1;
@@ -467,7 +499,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         ++unit_no;
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kWMma) {
     // ---------------- MMA ----------------
     constexpr uint32_t id_s = um_idesc<BF>(128, 128), id_o = um_idesc<BF>(128, HD) | (1u << 16);
     uint32_t stage_use = 0, np[2] = {0, 0}, unit_no = 0;
@@ -488,7 +520,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kUmKeys / 16; ++kk)
-          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + kk * 8, smem_desc_sw128_mn(sm + S::OFF_KV + st * S::kTileB + kk * 16 * 128), id_o,
+          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + (kk < 4 ? kk * 8 : 32 + kk * 8), smem_desc_sw128_mn(sm + S::OFF_KV + st * S::kTileB + kk * 16 * 128), id_o,
                   acc || kk != 0);
         umma_commit(pv_done + x);
       }
@@ -507,7 +539,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         if (i < g.take) wait(kv_full + ks, ku / S::kStages);
         if (i > 0) {
           wait(kv_full + vs, vu / S::kStages);
-          wait(v_ready + unit_no % kPres, unit_no / kPres);   // warp 11 has seen to it
+          wait(v_ready + unit_no % kPres, unit_no / kPres);   // warp 19 has seen to it
           ++unit_no;
         }
 #pragma unroll
@@ -531,7 +563,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       segment_done(seg);
     }
     if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
-  } else if (warp == 11) {
+  } else if (warp == kWClean) {
     // ---------------- V tiles with keys that not every row sees ----------------
     // A V row past the length is zeroed (its box holds earlier keys), and so is
     // every non-finite element of a row that some rows see and others do not,
@@ -579,10 +611,11 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUmRegsSoftmax));
     // ---------------- softmax and epilogue of row tile x ----------------
-    const int x = warp >> 2;
+    const int x = warp >> 3, half = (warp >> 2) & 1, bar = 1 + 4 * x + (warp & 3);
     const uint32_t r = 32u * (warp & 3) + lane;
     const uint32_t tl = tmem + ((32u * (warp & 3)) << 16);
-    const uint32_t tS = tl + x * 128, tO = tl + 256 + x * 128;
+    const uint32_t tS = tl + x * 128 + half * 64, tO = tl + 256 + x * 128 + half * (HD / 2);
+    volatile uint32_t* xr = xt + x * 128 + r;
     uint32_t ns = 0, unit_no = 0;       // units of this row tile, units of the run
     PartHeader hdr{0, 0, 0, 0};
     for (uint32_t seg = 0; segment(seg, g); ++seg) {
@@ -591,37 +624,54 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       const int limit = live ? g.seen(tok) : 0;
       const bool tile = x * PT < g.rows;
       const int seen_all = g.seen(x * PT);
-      float m = 0.f, l = 0.f, scale = 1.f;
+      float m = 0.f, l = 0.f;
+      bool fresh = true;              // no visible key among this thread's yet
       for (uint32_t i = 0; i < g.n[x]; ++i) {
-        const uint32_t un = unit_no + i;
         wait(s_full + x, ns);
         tc_fence_after();
-        wait(pres_full + un % kPres, un / kPres);   // written before the unit's K was asked for
-        const uint32_t mask = pres[un % kPres];
+        // page masks only once some page was absent (written before the unit's
+        // K was asked for)
+        uint32_t mask = 0xFFFFu;
+        const uint32_t sh = 31 - __clz(t.box);
+        const bool gaps = *absent != 0;
+        if (gaps) {
+          const uint32_t un = unit_no + i;
+          wait(pres_full + un % kPres, un / kPres);
+          mask = pres[un % kPres];
+        }
         const int key0 = (int)((g.unit + i) * kUmKeys);
-        const bool masked = mask != (1u << (kUmKeys / t.box)) - 1u || key0 + kUmKeys > seen_all;
-        uint32_t w[64];
+        uint32_t w[32];
         float sum, top;
-        if (masked) um_mask(tS, limit - key0, mask, 31 - __clz(t.box));
-        for (;;) {
+        if (gaps || key0 + kUmKeys > seen_all)
+          um_mask(tS, limit - key0 - 64 * half, mask >> ((64 * half) >> sh), sh);
+        for (bool first = true;; first = false) {
           um_pass<T>(tS, t.sl2, m, w, sum, top);
           top *= t.sl2;
           // (NaN scores are no maximum; they make the row's sum NaN.)  The
-          // first unit's maximum may not lie far below m either, or P would
-          // leave the 16-bit type's normal range.
-          const bool off = live && (top > m + kLag || (l == 0.f && top < m - kUnder && top > -INFINITY));
-          if (!__any_sync(0xffffffffu, off)) break;
-          if (off) {
-            const float f = l == 0.f ? 1.f : ex2(m - top);   // nothing to rescale yet
-            m = top;
-            l *= f;
-            scale = f;
+          // first maximum may not lie far below m either, or P would leave
+          // the 16-bit type's normal range.
+          const bool off = live && (top > m + kLag || (fresh && top < m - kUnder && top > -INFINITY));
+          if (!first || !pair_any(bar, off)) break;
+          // both threads of the row: the same m from both halves' maxima (as
+          // bf16, which is as good; the lowest bit says fresh)
+          reinterpret_cast<volatile uint16_t*>(xr)[half] =
+              (uint16_t)((__bfloat16_as_ushort(__float2bfloat16_rn(top)) & 0xFFFEu) | (fresh ? 1u : 0u));
+          pair_sync(bar);
+          const uint32_t both = *xr;
+          pair_sync(bar);
+          const float tp = fmaxf(__uint_as_float((both << 16) & 0xFFFE0000u), __uint_as_float(both & 0xFFFE0000u));
+          const bool all_fresh = (both & 0x10001u) == 0x10001u;
+          float scale = 1.f;
+          if (live && (tp > m + kLag || (all_fresh && tp < m - kUnder && tp > -INFINITY))) {
+            if (!all_fresh) scale = ex2(m - tp);     // else there is nothing to rescale
+            m = tp;
+            l *= scale;
           }
           if (i > 0) {
             wait(pv_done + x, ns - 1);
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
+            for (int c = 0; c < HD / 64; ++c) {
               uint32_t o[32];
               tm_ld32(tO + 32 * c, o);
               tm_wait_ld(o);
@@ -630,12 +680,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
               tmem_st32(tO + 32 * c, o);
             }
           }
-          scale = 1.f;
         }
+        if (top > -INFINITY) fresh = false;
         l += sum;
-        tm_st32(tS, w);
-        tm_st32(tS + 32, w + 32);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tmem_st32(tS, w);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive1(p_full + x);
@@ -643,14 +691,24 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       }
       unit_no += g.take;
       if (tile) {
+        // the row's sum: both halves', in one order
+        if (half == 1) *xr = __float_as_uint(l);
+        pair_sync(bar);
+        if (half == 0) {
+          l += __uint_as_float(*xr);
+          *xr = __float_as_uint(l);
+        }
+        pair_sync(bar);
+        if (half == 1) l = __uint_as_float(*xr);
+        pair_sync(bar);
         const bool whole = g.parts == 0, first = g.unit == 0;
         const float il = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         const uint32_t rr = (uint32_t)x * PT * G + r;
-        uint16_t* op = a.out + (int64_t)(g.row0 + tok) * a.out_stride + (int64_t)(g.kvh * G + r % G) * HD;
+        uint16_t* op = a.out + (int64_t)(g.row0 + tok) * a.out_stride + (int64_t)(g.kvh * G + r % G) * HD + half * (HD / 2);
         float* slot = t.ws.slot(blockIdx.x, first ? 1 : 0, HD);
-        float* part = slot + 2 * t.ws.R + (size_t)rr * 4;   // [HD / 4][R][4]: lanes side by side
+        float* part = slot + 2 * t.ws.R + (size_t)rr * 4 + (size_t)half * (HD / 2) * t.ws.R;   // [HD / 4][R][4]: lanes side by side
         if (first && !whole) hdr = {(uint32_t)g.row0, g.kvh, (uint32_t)g.rows * G, g.parts};
-        if (live && !whole) {
+        if (live && !whole && half == 0) {
           slot[rr] = l == 0.f ? -INFINITY : m;
           slot[t.ws.R + rr] = l;
         }
@@ -663,7 +721,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         if (g.n[x])
           for (int w = 0; w < 8; ++w) marks |= mk[w];
 #pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
+        for (int c = 0; c < HD / 64; ++c) {
           uint32_t w[32];
           float o[32];
           if (g.n[x]) {
@@ -672,7 +730,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           }
 #pragma unroll
           for (int d = 0; d < 32; ++d) o[d] = g.n[x] ? __uint_as_float(w[d]) * il : 0.f;
-          if (marks) add_nonfinite<BF>(a, g, mk, limit, 32 * c, o);
+          if (marks) add_nonfinite<BF>(a, g, mk, limit, half * (HD / 2) + 32 * c, o);
           if (live && whole) {
 #pragma unroll
             for (int d = 0; d < 32; d += 8)
@@ -692,7 +750,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  if (warp == kWMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 template <typename T, int HD>
