@@ -134,18 +134,6 @@ __device__ __forceinline__ void tm_wait_ld(uint32_t (&v)[32]) {
   asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
                     "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
-// 32 columns of this thread's TMEM lane; complete after tcgen05.wait::st.
-__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
-      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
-      "r"(v[31])
-      : "memory");
-}
-
 // Two f32 at a time (one instruction each).
 __device__ __forceinline__ uint64_t pair2(float x, float y) {
   uint64_t r;
@@ -367,17 +355,18 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tslot;
-  Segment g;
   bool failed = false;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (!failed) failed = !mbar_wait(bar, parity & 1u, a.err);
   };
 
   // part k of the run; warps 0-15, 17 and 19 take them in order from warp 16
-  auto segment = [&](uint32_t k, Segment& g) -> bool {
+  // (fields are read into registers one by one: a copy indexed by the row tile
+  // would live in local memory, which with this much shared memory means L2)
+  auto segment = [&](uint32_t k) -> const Segment* {
     wait(seg_full + k % kSegs, k / kSegs);
-    g = segs[k % kSegs];
-    return g.take != 0 && !failed;
+    const Segment* g = segs + k % kSegs;
+    return g->take != 0 && !failed ? g : nullptr;
   };
   auto segment_done = [&](uint32_t k) {
     __syncwarp();
@@ -530,13 +519,16 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       if (elect_one()) umma_commit(bar);
       __syncwarp();
     };
-    for (uint32_t seg = 0; segment(seg, g); ++seg) {
+    for (uint32_t seg = 0;; ++seg) {
+      const Segment* g = segment(seg);
+      if (!g) break;
+      const uint32_t take = g->take, n0 = g->n[0], n1 = g->n[1];
       wait(q_full, seg);
-      for (uint32_t i = 0; i <= g.take; ++i) {
+      for (uint32_t i = 0; i <= take; ++i) {
         // K of unit i, V of unit i - 1 (the ring holds K0 V0 K1 V1 ...)
         const uint32_t ku = stage_use + 2 * i, vu = stage_use + 2 * i - 1;
         const uint32_t ks = ku % S::kStages, vs = vu % S::kStages;
-        if (i < g.take) wait(kv_full + ks, ku / S::kStages);
+        if (i < take) wait(kv_full + ks, ku / S::kStages);
         if (i > 0) {
           wait(kv_full + vs, vu / S::kStages);
           wait(v_ready + unit_no % kPres, unit_no / kPres);   // warp 19 has seen to it
@@ -544,22 +536,22 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          if (i > 0 && i - 1 < g.n[x]) {
+          if (i > 0 && i - 1 < (x ? n1 : n0)) {
             wait(p_full + x, np[x]);
             ++np[x];
             tc_fence_after();
             issue_o(x, vs, i > 1);
           }
-          if (i < g.n[x]) {
+          if (i < (x ? n1 : n0)) {
             tc_fence_after();
             issue_s(x, ks);
           }
         }
         if (i > 0) release(kv_empty + vs);
-        if (i < g.take) release(kv_empty + ks);
-        if (i + 1 == g.take) release(q_empty);
+        if (i < take) release(kv_empty + ks);
+        if (i + 1 == take) release(q_empty);
       }
-      stage_use += 2 * g.take;
+      stage_use += 2 * take;
       segment_done(seg);
     }
     if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
@@ -569,15 +561,18 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     // every non-finite element of a row that some rows see and others do not,
     // or 0 * V would reach the others; the epilogue adds it to those that do.
     uint32_t stage_use = 0, unit_no = 0;
-    for (uint32_t seg = 0; segment(seg, g); ++seg) {
-      const int seen_all = g.seen(0), seen_any = g.seen(g.rows - 1);
+    for (uint32_t seg = 0;; ++seg) {
+      const Segment* g = segment(seg);
+      if (!g) break;
+      const int seen_all = g->seen(0), seen_any = g->seen(g->rows - 1);
+      const uint32_t take = g->take, unit = g->unit;
       const int base = max(0, seen_any - 256);   // key of the first mark
-      for (uint32_t i = 0; i < g.take; ++i) {
+      for (uint32_t i = 0; i < take; ++i) {
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv, ++stage_use) {
           const uint32_t st = stage_use % S::kStages;
           wait(kv_full + st, stage_use / S::kStages);
-          const int key0 = (int)((g.unit + i) * kUmKeys);
+          const int key0 = (int)((unit + i) * kUmKeys);
           if (kv && key0 + kUmKeys > seen_all) {
             const int r0 = max(0, seen_all - key0);
             constexpr int CH = HD / 8;           // 16-byte chunks of a row
@@ -618,15 +613,19 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     volatile uint32_t* xr = xt + x * 128 + r;
     uint32_t ns = 0, unit_no = 0;       // units of this row tile, units of the run
     PartHeader hdr{0, 0, 0, 0};
-    for (uint32_t seg = 0; segment(seg, g); ++seg) {
+    for (uint32_t seg = 0;; ++seg) {
+      const Segment* g = segment(seg);
+      if (!g) break;
+      const int rows = g->rows, row0 = g->row0;
+      const uint32_t take = g->take, unit = g->unit, units = g->n[x], seg_parts = g->parts, kvh = g->kvh;
       const int tok = x * PT + (int)(r / G);         // token of the task
-      const bool live = r < (uint32_t)PT * G && tok < g.rows;
-      const int limit = live ? g.seen(tok) : 0;
-      const bool tile = x * PT < g.rows;
-      const int seen_all = g.seen(x * PT);
+      const bool live = r < (uint32_t)PT * G && tok < rows;
+      const int limit = live ? g->seen(tok) : 0;
+      const bool tile = x * PT < rows;
+      const int seen_all = g->seen(x * PT);
       float m = 0.f, l = 0.f;
       bool fresh = true;              // no visible key among this thread's yet
-      for (uint32_t i = 0; i < g.n[x]; ++i) {
+      for (uint32_t i = 0; i < units; ++i) {
         wait(s_full + x, ns);
         tc_fence_after();
         // page masks only once some page was absent (written before the unit's
@@ -639,7 +638,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           wait(pres_full + un % kPres, un / kPres);
           mask = pres[un % kPres];
         }
-        const int key0 = (int)((g.unit + i) * kUmKeys);
+        const int key0 = (int)((unit + i) * kUmKeys);
         uint32_t w[32];
         float sum, top;
         if (gaps || key0 + kUmKeys > seen_all)
@@ -689,7 +688,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         if (lane == 0) mbar_arrive1(p_full + x);
         ++ns;
       }
-      unit_no += g.take;
+      unit_no += take;
       if (tile) {
         // the row's sum: both halves', in one order
         if (half == 1) *xr = __float_as_uint(l);
@@ -701,36 +700,36 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         pair_sync(bar);
         if (half == 1) l = __uint_as_float(*xr);
         pair_sync(bar);
-        const bool whole = g.parts == 0, first = g.unit == 0;
+        const bool whole = seg_parts == 0, first = unit == 0;
         const float il = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         const uint32_t rr = (uint32_t)x * PT * G + r;
-        uint16_t* op = a.out + (int64_t)(g.row0 + tok) * a.out_stride + (int64_t)(g.kvh * G + r % G) * HD + half * (HD / 2);
+        uint16_t* op = a.out + (int64_t)(row0 + tok) * a.out_stride + (int64_t)(kvh * G + r % G) * HD + half * (HD / 2);
         float* slot = t.ws.slot(blockIdx.x, first ? 1 : 0, HD);
         float* part = slot + 2 * t.ws.R + (size_t)rr * 4 + (size_t)half * (HD / 2) * t.ws.R;   // [HD / 4][R][4]: lanes side by side
-        if (first && !whole) hdr = {(uint32_t)g.row0, g.kvh, (uint32_t)g.rows * G, g.parts};
+        if (first && !whole) hdr = {(uint32_t)row0, kvh, (uint32_t)rows * G, seg_parts};
         if (live && !whole && half == 0) {
           slot[rr] = l == 0.f ? -INFINITY : m;
           slot[t.ws.R + rr] = l;
         }
-        if (g.n[x]) {
+        if (units) {
           wait(pv_done + x, ns - 1);
           tc_fence_after();
         }
-        const volatile uint32_t* mk = segs[seg % kSegs].marks;
+        const volatile uint32_t* mk = g->marks;
         uint32_t marks = 0;      // some key of the segment has a non-finite V
-        if (g.n[x])
+        if (units)
           for (int w = 0; w < 8; ++w) marks |= mk[w];
 #pragma unroll 1
         for (int c = 0; c < HD / 64; ++c) {
           uint32_t w[32];
           float o[32];
-          if (g.n[x]) {
+          if (units) {
             tm_ld32(tO + 32 * c, w);
             tm_wait_ld(w);
           }
 #pragma unroll
-          for (int d = 0; d < 32; ++d) o[d] = g.n[x] ? __uint_as_float(w[d]) * il : 0.f;
-          if (marks) add_nonfinite<BF>(a, g, mk, limit, half * (HD / 2) + 32 * c, o);
+          for (int d = 0; d < 32; ++d) o[d] = units ? __uint_as_float(w[d]) * il : 0.f;
+          if (marks) add_nonfinite<BF>(a, *g, mk, limit, half * (HD / 2) + 32 * c, o);
           if (live && whole) {
 #pragma unroll
             for (int d = 0; d < 32; d += 8)
