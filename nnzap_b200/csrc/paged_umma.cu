@@ -11,12 +11,13 @@
 //                       the pool's type over the S it came from
 //   O += P V            tcgen05.mma, P from TMEM, V as stored (MN-major B)
 // so while one row tile's softmax runs, the tensor cores work for the other.
-// m only follows the row's maximum from afar: it starts at 0, a unit's P is
-// computed with the m that the row has, in one pass over S, and only if a
-// score turns out to be more than 8 (in log2) above it (in the row's first
-// unit also: the maximum more than 4 below) does the row take its maximum for
-// m, rescale O and compute the unit again, which after the first units is
-// rare.  P up to 256 costs no precision, the sums are f32.
+// m need not be the row's maximum: any m gives the same quotient as long as no
+// P overflows or leaves the 16-bit type's normal range.  It starts at 0, a
+// unit's P is computed with the m that the row has, in one pass over S without
+// looking for a maximum, and only if the sum of 64 P turns out to be 2^15 or
+// more (or, among the first keys that a row sees, less than 1/4) does the row
+// take its maximum for m, rescale O and compute the unit again, which after
+// the first units is rare.  Sums are f32.
 //
 // Roles: warps 0-7 and 8-15 softmax and epilogue of row tiles 0 and 1 (TMEM lane
 // = row; warps 0-3 of a tile have keys 0-63 of a unit and the lower half of the
@@ -54,7 +55,7 @@ constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
 constexpr uint32_t kPartCost = 3;                 // what a part costs besides its units, in units (queries, epilogue, merge)
 constexpr int kPres = 8;                          // units whose page masks are kept
-constexpr float kLag = 8.f, kUnder = 4.f;         // how far (log2) a row's maximum may lie above / at first below its m
+constexpr float kMost = 32768.f, kLeast = 0.25f;  // sum of 64 P: below kMost (no P overflows), at first kLeast at least
 
 template <int HD>
 struct UmShape {
@@ -206,14 +207,26 @@ __device__ __forceinline__ void um_mask(uint32_t tS, int end, uint32_t bits, uin
   }
 }
 
-// P = 2^(S sl2 - ms) of 64 keys of a row as 32 words of the pool's type, their
-// f32 sum, and the largest score.  The next 16 of S are on their way while some
-// are worked on.
+// The largest of 64 scores of a row.
+__device__ __forceinline__ float um_top(uint32_t tS) {
+  float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
+    uint32_t v[32];
+    tm_ld32(tS + 32 * c, v);
+    tm_wait_ld(v);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(v[e]));
+  }
+  return fmaxf(mx[0], mx[1]);
+}
+
+// P = 2^(S sl2 - ms) of 64 keys of a row as 32 words of the pool's type; their
+// f32 sum.  The next 16 of S are on their way while some are worked on.
 template <typename T>
-__device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32_t (&w)[32], float& sum, float& top) {
+__device__ __forceinline__ float um_pass(uint32_t tS, float sl2, float ms, uint32_t (&w)[32]) {
   const uint64_t k2 = pair2(sl2, sl2), m2 = pair2(-ms, -ms);
   uint64_t acc[2] = {0ull, 0ull};
-  float mx[2] = {-INFINITY, -INFINITY};
   uint32_t v[2][16];
   tm_ld16(tS, v[0]);
 #pragma unroll
@@ -222,9 +235,7 @@ __device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32
     if (c < 3) tm_ld16(tS + 16 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-      const float a = __uint_as_float(v[c & 1][e]), b = __uint_as_float(v[c & 1][e + 1]);
-      mx[(e >> 1) & 1] = fmaxf(fmaxf(mx[(e >> 1) & 1], a), b);
-      const float2 y = split2(fma2(pair2(a, b), k2, m2));
+      const float2 y = split2(fma2(pair2(__uint_as_float(v[c & 1][e]), __uint_as_float(v[c & 1][e + 1])), k2, m2));
       // a quarter of the exponentials on the FMA pipe: both row tiles' on the
       // special-function units alone take 2 x 1024 cycles per unit
       const float2 q = ((e >> 1) & 3) == 3 ? ex2_fma(y.x, y.y) : make_float2(ex2(y.x), ex2(y.y));
@@ -236,8 +247,7 @@ __device__ __forceinline__ void um_pass(uint32_t tS, float sl2, float ms, uint32
     asm volatile("" : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]));
   }
   const float2 t = split2(add2(acc[0], acc[1]));
-  sum = t.x + t.y;
-  top = fmaxf(mx[0], mx[1]);
+  return t.x + t.y;
 }
 
 // The two warps that share 32 rows: whether any of their 64 threads says so.
@@ -251,6 +261,14 @@ __device__ __forceinline__ bool pair_any(int bar, bool p) {
   return r != 0;
 }
 __device__ __forceinline__ void pair_sync(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
+// The value of the row's thread of half `from`.
+__device__ __forceinline__ float pair_tell(int bar, volatile uint32_t* at, int half, int from, float v) {
+  if (half == from) *at = __float_as_uint(v);
+  pair_sync(bar);
+  const float r = __uint_as_float(*at);
+  pair_sync(bar);
+  return r;
+}
 
 template <bool BF16>
 __host__ __device__ constexpr uint32_t um_idesc(int M, int N) {
@@ -270,6 +288,7 @@ struct Segment {
   uint32_t unit;       // first unit within the task
   uint32_t n[2];       // units that each row tile looks at (from the first)
   uint32_t parts;      // 0: the whole task; else the parts it is split into
+  uint32_t gaps;       // a page of its keys is absent
   uint32_t s, kvh;
   int row0;            // q / out row of the task's first token
   int rows;            // tokens of the task
@@ -326,7 +345,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint64_t* seg_full = pres_full + kPres;   // [kSegs]
   uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 18 other warps are done with it
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + S::OFF_MISC);
-  volatile uint32_t* absent = tslot + 1 + kPres;   // an absent page was met
   volatile uint32_t* pres = tslot + 1;   // [kPres] one bit per box of the unit: page present
   Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_SEG);
   static_assert(sizeof(Segment) <= 80 && S::kSmem <= 232448);
@@ -337,7 +355,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   // every barrier by its own thread; arrivals: 2 for a free stage (the products
   // and warp 19), 8 for P (a warp each), 18 for a part's end, else 1
   static_assert(S::kBars <= kUmThreads);
-  if (threadIdx.x == 0) *absent = 0;
   if (threadIdx.x < (uint32_t)S::kBars) {
     uint64_t* b = kv_full + threadIdx.x;
     mbar_init(b, b >= kv_empty && b < q_full ? 2 : b == p_full || b == p_full + 1 ? 8 : b >= seg_empty ? 18 : 1);
@@ -419,6 +436,13 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           o.parts = (uint32_t)((t0 + c.units - 1) / per - t0 / per + 1);
         }
       }
+      if (more) {     // (softmax warps ask per part, not per unit: shared memory is slow to answer while MMAs read it)
+        const uint32_t k0 = o.unit * kUmKeys, k1 = min((o.unit + o.take) * kUmKeys, (uint32_t)o.seen(o.rows - 1));
+        const uint32_t p0 = k0 / a.kv.page_size, p1 = k1 > k0 ? (k1 - 1) / a.kv.page_size + 1 : p0;
+        bool gap = false;
+        for (uint32_t p = p0 + lane; p < p1; p += 32) gap |= (uint32_t)__ldg(a.page_table + (size_t)o.s * a.table_stride + p) >= a.kv.num_pages;
+        o.gaps = __any_sync(0xffffffffu, gap) ? 1u : 0u;
+      }
       if (seg >= kSegs) wait(seg_empty + seg % kSegs, seg / kSegs - 1);
       __syncwarp();
       if (lane == 0) {
@@ -442,7 +466,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         const int p = __ldg(pages + pi);
         if ((uint32_t)p < a.kv.num_pages) return p;
         if (p >= 0) atomicOr(a.err, ERR_BAD_PAGE);
-        *absent = 1;
         return -1;
       };
       uint32_t at, nat = 0;
@@ -618,6 +641,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       if (!g) break;
       const int rows = g->rows, row0 = g->row0;
       const uint32_t take = g->take, unit = g->unit, units = g->n[x], seg_parts = g->parts, kvh = g->kvh;
+      const bool gaps = g->gaps != 0;
       const int tok = x * PT + (int)(r / G);         // token of the task
       const bool live = r < (uint32_t)PT * G && tok < rows;
       const int limit = live ? g->seen(tok) : 0;
@@ -628,11 +652,9 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       for (uint32_t i = 0; i < units; ++i) {
         wait(s_full + x, ns);
         tc_fence_after();
-        // page masks only once some page was absent (written before the unit's
-        // K was asked for)
+        // page masks only where the part has absent pages
         uint32_t mask = 0xFFFFu;
         const uint32_t sh = 31 - __clz(t.box);
-        const bool gaps = *absent != 0;
         if (gaps) {
           const uint32_t un = unit_no + i;
           wait(pres_full + un % kPres, un / kPres);
@@ -640,28 +662,23 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         }
         const int key0 = (int)((unit + i) * kUmKeys);
         uint32_t w[32];
-        float sum, top;
+        float sum;
         if (gaps || key0 + kUmKeys > seen_all)
           um_mask(tS, limit - key0 - 64 * half, mask >> ((64 * half) >> sh), sh);
         for (bool first = true;; first = false) {
-          um_pass<T>(tS, t.sl2, m, w, sum, top);
-          top *= t.sl2;
-          // (NaN scores are no maximum; they make the row's sum NaN.)  The
-          // first maximum may not lie far below m either, or P would leave
-          // the 16-bit type's normal range.
-          const bool off = live && (top > m + kLag || (fresh && top < m - kUnder && top > -INFINITY));
+          sum = um_pass<T>(tS, t.sl2, m, w);
+          // Out of range: a sum of 2^15 or more (or NaN), or of less than 1/4
+          // among the first keys that the row sees.
+          const bool off = live && (!(sum < kMost) || (fresh && sum < kLeast));
           if (!first || !pair_any(bar, off)) break;
-          // both threads of the row: the same m from both halves' maxima (as
-          // bf16, which is as good; the lowest bit says fresh)
-          reinterpret_cast<volatile uint16_t*>(xr)[half] =
-              (uint16_t)((__bfloat16_as_ushort(__float2bfloat16_rn(top)) & 0xFFFEu) | (fresh ? 1u : 0u));
-          pair_sync(bar);
-          const uint32_t both = *xr;
-          pair_sync(bar);
-          const float tp = fmaxf(__uint_as_float((both << 16) & 0xFFFE0000u), __uint_as_float(both & 0xFFFE0000u));
-          const bool all_fresh = (both & 0x10001u) == 0x10001u;
+          // both threads of a row: the same m, from both halves' maxima
+          const float top = um_top(tS) * t.sl2;
+          const float tp = fmaxf(pair_tell(bar, xr, half, 0, top), pair_tell(bar, xr, half, 1, top));
+          const float say = (off ? 2.f : 0.f) + (fresh ? 1.f : 0.f);
+          const float s0 = pair_tell(bar, xr, half, 0, say), s1 = pair_tell(bar, xr, half, 1, say);
+          const bool all_fresh = s0 != 0.f && s0 != 2.f && s1 != 0.f && s1 != 2.f;
           float scale = 1.f;
-          if (live && (tp > m + kLag || (all_fresh && tp < m - kUnder && tp > -INFINITY))) {
+          if (live && (s0 >= 2.f || s1 >= 2.f) && (tp > m || (all_fresh && tp > -INFINITY))) {
             if (!all_fresh) scale = ex2(m - tp);     // else there is nothing to rescale
             m = tp;
             l *= scale;
@@ -679,8 +696,9 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
               tmem_st32(tO + 32 * c, o);
             }
           }
+          if (top > -INFINITY) fresh = false;
         }
-        if (top > -INFINITY) fresh = false;
+        if (sum > 0.f) fresh = false;
         l += sum;
         tmem_st32(tS, w);
         tc_fence_before();
@@ -691,15 +709,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       unit_no += take;
       if (tile) {
         // the row's sum: both halves', in one order
-        if (half == 1) *xr = __float_as_uint(l);
-        pair_sync(bar);
-        if (half == 0) {
-          l += __uint_as_float(*xr);
-          *xr = __float_as_uint(l);
-        }
-        pair_sync(bar);
-        if (half == 1) l = __uint_as_float(*xr);
-        pair_sync(bar);
+        l = pair_tell(bar, xr, half, 0, l) + pair_tell(bar, xr, half, 1, l);
         const bool whole = seg_parts == 0, first = unit == 0;
         const float il = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         const uint32_t rr = (uint32_t)x * PT * G + r;
