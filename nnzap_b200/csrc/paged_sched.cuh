@@ -67,8 +67,13 @@ __device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t x
     }
     const uint64_t last = (uint64_t)x * n + y;
     if (last < m) return sum;
-    n = (uint32_t)(last / m);
-    y = (uint32_t)(last % m);
+    if (last >> 32) {
+      n = (uint32_t)(last / m);
+      y = (uint32_t)(last % m);
+    } else {                       // 32-bit division
+      n = (uint32_t)last / m;
+      y = (uint32_t)last % m;
+    }
     const uint32_t t = m;
     m = x;
     x = t;
@@ -255,8 +260,9 @@ __device__ __forceinline__ bool warp_parts(const PagedAttnArgs& a, int QT, int K
         c.kvh = rel / run.parts;
         run.part = rel % run.parts;
         c.qt = l + 32 * i - (int)__shfl_sync(0xffffffffu, inc - nt, (int)c.s);
-        c.unit = (uint32_t)((uint64_t)c.units * run.part / run.parts);
-        run.end = (uint32_t)((uint64_t)c.units * (run.part + 1) / run.parts);
+        const uint32_t each = c.units / run.parts, more = c.units % run.parts;     // the first `more` have one unit more
+        c.unit = each * run.part + min(run.part, more);
+        run.end = c.unit + each + (run.part < more ? 1u : 0u);
         c.q = seq_info(a, c.s);
       }
       before = __shfl_sync(0xffffffffu, incl, 31);
@@ -264,6 +270,10 @@ __device__ __forceinline__ bool warp_parts(const PagedAttnArgs& a, int QT, int K
     return true;
   }
   return false;
+}
+
+__device__ __forceinline__ uint64_t div_up(uint64_t x, uint32_t y) {
+  return x >> 32 ? (x + y - 1) / y : ((uint32_t)x + (y - 1)) >= y - 1 ? ((uint32_t)x + (y - 1)) / y : (x + y - 1) / y;
 }
 
 // ---- workspace: a header, a counter and two slots of partials per CTA ----

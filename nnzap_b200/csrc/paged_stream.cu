@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   } else {
     uint64_t tasks = 0;
     const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine, &tasks);
-    const uint32_t per_cta = max(1u, (uint32_t)((total + gridDim.x - 1) / gridDim.x));
+    const uint32_t per_cta = max(1u, (uint32_t)div_up(total, gridDim.x));
     per = (per_cta + kStWarps - 1) / kStWarps;
     even = !(tasks <= gridDim.x && a.num_seqs <= 32 &&
              warp_parts<1>(a, QT, kStKeys, lane, gridDim.x, per_cta, per_cta + per_cta / 4 + 8, blockIdx.x, c, run));

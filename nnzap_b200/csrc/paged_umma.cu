@@ -372,9 +372,15 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tslot;
-  bool failed = false;
+  // Bounded waits: one that gives up leaves no tries to the later ones, and the
+  // error is reported at the end (nothing but the poll stands in the loop).
+  uint32_t tries = kSpinLimit;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!failed) failed = !mbar_wait(bar, parity & 1u, a.err);
+    for (uint32_t n = 0; !mbar_try_wait(bar, parity & 1u);)
+      if (++n > tries) {
+        tries = 0;
+        break;
+      }
   };
 
   // part k of the run; warps 0-15, 17 and 19 take them in order from warp 16
@@ -383,7 +389,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   auto segment = [&](uint32_t k) -> const Segment* {
     wait(seg_full + k % kSegs, k / kSegs);
     const Segment* g = segs + k % kSegs;
-    return g->take != 0 && !failed ? g : nullptr;
+    return g->take != 0 && tries ? g : nullptr;
   };
   auto segment_done = [&](uint32_t k) {
     __syncwarp();
@@ -394,18 +400,22 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUmRegsIssue));
   if (warp == kWTma) {
     // ---------------- the run, and its TMA ----------------
-    uint64_t mine = 0, tasks = 0;
-    const uint64_t total = warp_total(a, QT, kUmKeys, lane, blockIdx.x == 0, mine, &tasks);
-    const uint32_t P = t.workers, per = max(1u, (uint32_t)((total + P - 1) / P));
-    // One part per CTA where that costs no more than kPartCost units over the
-    // even cut.
     Cursor c;
     PartRun run{0, 0, 0};
-    uint64_t u = (uint64_t)blockIdx.x * per, u1 = min(u + per, total);     // even cut
-    const bool even = !(tasks <= P && a.num_seqs <= 32 && warp_parts<5>(a, QT, kUmKeys, lane, P, per, per + kPartCost, blockIdx.x, c, run));
-    bool more = even ? u < u1 : run.parts != 0;
+    uint64_t u = 0, u1 = 0;
+    uint32_t per = 1;
+    bool even = true, more = false;
+    uint64_t mine = 0, tasks = 0;
+    const uint64_t total = warp_total(a, QT, kUmKeys, lane, blockIdx.x == 0, mine, &tasks);
+    const uint32_t P = t.workers;
+    per = max(1u, (uint32_t)div_up(total, P));
+    // One part per CTA where that costs no more than kPartCost units over the
+    // even cut.
+    u = (uint64_t)blockIdx.x * per;
+    u1 = min(u + per, total);     // even cut
+    even = !(tasks <= P && a.num_seqs <= 32 && warp_parts<5>(a, QT, kUmKeys, lane, P, per, per + kPartCost, blockIdx.x, c, run));
+    more = even ? u < u1 : run.parts != 0;
     if (even && more) warp_find(a, QT, kUmKeys, lane, u, mine, c);
-
     const uint32_t nb = kUmKeys / t.box;
     const uint32_t bi = (uint32_t)lane % nb, half = (uint32_t)lane / nb;
     const bool copies = half < (uint32_t)NH;
@@ -436,20 +446,24 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           o.parts = (uint32_t)((t0 + c.units - 1) / per - t0 / per + 1);
         }
       }
-      if (more) {     // (softmax warps ask per part, not per unit: shared memory is slow to answer while MMAs read it)
-        const uint32_t k0 = o.unit * kUmKeys, k1 = min((o.unit + o.take) * kUmKeys, (uint32_t)o.seen(o.rows - 1));
-        const uint32_t p0 = k0 / a.kv.page_size, p1 = k1 > k0 ? (k1 - 1) / a.kv.page_size + 1 : p0;
-        bool gap = false;
-        for (uint32_t p = p0 + lane; p < p1; p += 32) gap |= (uint32_t)__ldg(a.page_table + (size_t)o.s * a.table_stride + p) >= a.kv.num_pages;
-        o.gaps = __any_sync(0xffffffffu, gap) ? 1u : 0u;
-      }
-      if (seg >= kSegs) wait(seg_empty + seg % kSegs, seg / kSegs - 1);
-      __syncwarp();
-      if (lane == 0) {
-        segs[seg % kSegs] = o;
-        mbar_arrive1(seg_full + seg % kSegs);
-      }
-      if (o.take == 0 || failed) break;
+      auto publish = [&] {
+        if (o.take) {     // (softmax warps ask per part, not per unit: shared memory is slow to answer while MMAs read it)
+          const uint32_t k0 = o.unit * kUmKeys, k1 = min((o.unit + o.take) * kUmKeys, (uint32_t)o.seen(o.rows - 1));
+          const uint32_t p0 = k0 / a.kv.page_size, p1 = k1 > k0 ? (k1 - 1) / a.kv.page_size + 1 : p0;
+          bool gap = false;
+          for (uint32_t p = p0 + lane; p < p1; p += 32) gap |= (uint32_t)__ldg(a.page_table + (size_t)o.s * a.table_stride + p) >= a.kv.num_pages;
+          o.gaps = __any_sync(0xffffffffu, gap) ? 1u : 0u;
+        }
+        if (seg >= kSegs) wait(seg_empty + seg % kSegs, seg / kSegs - 1);
+        __syncwarp();
+        if (lane == 0) {
+          segs[seg % kSegs] = o;
+          mbar_arrive1(seg_full + seg % kSegs);
+        }
+      };
+      // (the first part's loads go first: nobody can use it before they land)
+      if (seg || !o.take) publish();
+      if (o.take == 0 || !tries) break;
       u += o.take;
       more = even && u < u1 && cursor_next_task(a, c, QT, kUmKeys);
 
@@ -504,7 +518,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
             tma_load_4d(sm + S::OFF_KV + st * S::kTileB + half * kHalfB + bi * t.box * 128, kv ? &t.tmV : &t.tmK, (int)half * 64, (int)at,
                         (int)o.kvh, pg >= 0 ? pg : (int)a.kv.num_pages, kv_full + st);
           ++stage_use;
-          if (kv == 0 && i == 0 && seg) queries();
+          if (kv == 0 && i == 0) {
+            if (seg) queries();
+            else publish();
+          }
         }
         pg = npg;
         at = nat;
@@ -757,6 +774,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     }
     if (threadIdx.x == 0) t.ws.head[blockIdx.x] = hdr;
   }
+  if (!tries && lane == 0) atomicOr(a.err, ERR_MBAR_TIMEOUT);
   tc_fence_before();
   __syncthreads();
   if (warp == kWMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
