@@ -41,45 +41,64 @@ __global__ void rope_table_kernel(double l2theta, uint32_t half, uint32_t positi
 // token; a thread asks for all its chunks (up to kNrUnroll) before it waits
 // for the position, the table row that depends on it, or the slot, so a CTA
 // pays two memory latencies and the 8 CTAs of an SM keep 128 KB in flight.
+// A lane holds four pairs of a head whole: 8 elements in a row (pairwise), or 4
+// of each half (half split: two 8-byte chunks; with 16-byte chunks the pairs
+// would meet by 8 shuffles more per chunk).
 constexpr int kNrThreads = 128, kNrUnroll = 4;
+
+template <int STYLE>
+__device__ __forceinline__ uint4 nr_load(const uint16_t* head, uint32_t hl, int hd) {
+  if constexpr (STYLE == ROPE_PAIRWISE) return __ldcs(reinterpret_cast<const uint4*>(head) + hl);
+  const uint2 a = __ldcs(reinterpret_cast<const uint2*>(head) + hl), b = __ldcs(reinterpret_cast<const uint2*>(head + hd / 2) + hl);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <int STYLE>
+__device__ __forceinline__ void nr_store(uint16_t* head, uint32_t hl, int hd, const uint4& v) {
+  if constexpr (STYLE == ROPE_PAIRWISE) {
+    reinterpret_cast<uint4*>(head)[hl] = v;
+  } else {
+    reinterpret_cast<uint2*>(head)[hl] = make_uint2(v.x, v.y);
+    reinterpret_cast<uint2*>(head + hd / 2)[hl] = make_uint2(v.z, v.w);
+  }
+}
 
 template <typename T, int HD, int STYLE>
 __global__ void __launch_bounds__(kNrThreads, 8) norm_rope_kernel(const NormRopeArgs a) {
   constexpr int LPH = HD / 8;                          // lanes per head
-  constexpr int NCS = STYLE == ROPE_PAIRWISE ? 4 : 8;   // (cos, sin) of a lane's 8 elements
   constexpr uint32_t HPS = kNrThreads / LPH;            // heads per step of the CTA
   const uint32_t tok = blockIdx.x;
   const uint32_t hl = threadIdx.x % LPH, hg = threadIdx.x / LPH;
   const uint32_t n_kv = a.kv.n_kv, heads = a.n_q + 2 * n_kv;
-  const uint4* src = reinterpret_cast<const uint4*>(a.qkv + (int64_t)tok * a.qkv_stride);
+  const uint16_t* src = a.qkv + (int64_t)tok * a.qkv_stride;
   uint4 u[kNrUnroll];
 #pragma unroll
   for (int i = 0; i < kNrUnroll; ++i) {
     const uint32_t h = hg + i * HPS;
-    u[i] = h < heads ? __ldcs(src + h * LPH + hl) : make_uint4(0u, 0u, 0u, 0u);
+    u[i] = h < heads ? nr_load<STYLE>(src + h * HD, hl, HD) : make_uint4(0u, 0u, 0u, 0u);
   }
   const int pos = a.positions[tok];
   const long long slot = a.slots[tok];
+  // element e of the lane: 8 hl + e, or 4 hl + e of the first (e < 4) or second half
   float4 wq[2], wk[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    wq[i] = __ldg(reinterpret_cast<const float4*>(a.q_norm + hl * 8) + i);
-    wk[i] = __ldg(reinterpret_cast<const float4*>(a.k_norm + hl * 8) + i);
+    const uint32_t at = STYLE == ROPE_PAIRWISE ? hl * 8 + 4 * i : hl * 4 + i * (HD / 2);
+    wq[i] = __ldg(reinterpret_cast<const float4*>(a.q_norm + at));
+    wk[i] = __ldg(reinterpret_cast<const float4*>(a.k_norm + at));
   }
   const bool bad_pos = pos < 0 || (uint32_t)pos >= a.table_positions;
   const bool bad_slot = slot >= (long long)a.kv.num_pages * a.kv.page_size;
   const bool bad = bad_pos || bad_slot;
   if (bad && threadIdx.x == 0) atomicOr(a.err, bad_pos ? ERR_BAD_POS : ERR_BAD_PAGE);
-  float2 cs[NCS];
+  float4 cs[2];             // (cos, sin) of the lane's pairs 4 hl .. 4 hl + 3
   {
-    const float2* tab = a.table + (size_t)(bad_pos ? 0 : pos) * (HD / 2);
-    const uint32_t i0 = STYLE == ROPE_PAIRWISE ? hl * 4 : (hl % (LPH / 2)) * 8;
-#pragma unroll
-    for (int i = 0; i < NCS; ++i) cs[i] = __ldg(tab + i0 + i);
+    const float4* tab = reinterpret_cast<const float4*>(a.table + (size_t)(bad_pos ? 0 : pos) * (HD / 2)) + hl * 2;
+    cs[0] = __ldg(tab);
+    cs[1] = __ldg(tab + 1);
   }
   int64_t page_off = 0;
   if (!bad && slot >= 0) {
-    const long long pg = slot / a.kv.page_size;
+    const long long pg = slot >> 32 ? slot / a.kv.page_size : (long long)((uint32_t)slot / a.kv.page_size);
     page_off = pg * a.kv.page_stride + (slot - pg * a.kv.page_size) * a.kv.token_stride;
   }
   for (uint32_t h0 = 0; h0 < heads; h0 += kNrUnroll * HPS) {
@@ -87,61 +106,50 @@ __global__ void __launch_bounds__(kNrThreads, 8) norm_rope_kernel(const NormRope
     for (int i = 0; i < kNrUnroll; ++i) {
       const uint32_t h = h0 + i * HPS + hg;
       if (h0 + i * HPS >= heads) break;               // the same for every thread
-      const bool live = h < heads;
-      // every lane takes the shuffles (value heads too: their result is not used)
-      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-      float x[8], ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = T16<T>::to_f2(w[e]);
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
-        ss = fmaf(f.x, f.x, ss);
-        ss = fmaf(f.y, f.y, ss);
-      }
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(ss / (float)HD + a.eps);
-      const bool is_q = h < a.n_q;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float4 nw = is_q ? wq[e] : wk[e];
-        x[4 * e] *= r * nw.x;
-        x[4 * e + 1] *= r * nw.y;
-        x[4 * e + 2] *= r * nw.z;
-        x[4 * e + 3] *= r * nw.w;
-      }
-      if constexpr (STYLE == ROPE_PAIRWISE) {
+      const bool is_q = h < a.n_q, is_v = h >= a.n_q + n_kv;
+      uint4 y = u[i];
+      if (!__all_sync(0xffffffffu, is_v)) {            // a query or key head among the warp's
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        float x[8], ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = x[2 * e], q = x[2 * e + 1];
-          x[2 * e] = p * cs[e].x - q * cs[e].y;
-          x[2 * e + 1] = p * cs[e].y + q * cs[e].x;
+          const float2 f = T16<T>::to_f2(w[e]);
+          x[2 * e] = f.x;
+          x[2 * e + 1] = f.y;
+          ss = fmaf(f.x, f.x, ss);
+          ss = fmaf(f.y, f.y, ss);
         }
-      } else {
-        // element e of the first half pairs with element e of the second,
-        // LPH / 2 lanes away
-        const bool second = hl >= LPH / 2;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float other = __shfl_xor_sync(0xffffffffu, x[e], LPH / 2);
-          x[e] = second ? other * cs[e].y + x[e] * cs[e].x : x[e] * cs[e].x - other * cs[e].y;
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = rsqrtf(ss * (1.f / HD) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float4 nw = is_q ? wq[e] : wk[e];
+          x[4 * e] *= r * nw.x;
+          x[4 * e + 1] *= r * nw.y;
+          x[4 * e + 2] *= r * nw.z;
+          x[4 * e + 3] *= r * nw.w;
         }
+        const float c[4] = {cs[0].x, cs[0].z, cs[1].x, cs[1].z}, s[4] = {cs[0].y, cs[0].w, cs[1].y, cs[1].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int ia = STYLE == ROPE_PAIRWISE ? 2 * e : e, ib = STYLE == ROPE_PAIRWISE ? 2 * e + 1 : e + 4;
+          const float p = x[ia], q = x[ib];
+          x[ia] = p * c[e] - q * s[e];
+          x[ib] = p * s[e] + q * c[e];
+        }
+        if (!is_v)
+          y = make_uint4(T16<T>::pack(x[0], x[1]), T16<T>::pack(x[2], x[3]), T16<T>::pack(x[4], x[5]), T16<T>::pack(x[6], x[7]));
       }
-      uint4 y = u[i];
-      if (h < a.n_q + n_kv)   // a query or key head
-        y = make_uint4(T16<T>::pack(x[0], x[1]), T16<T>::pack(x[2], x[3]), T16<T>::pack(x[4], x[5]), T16<T>::pack(x[6], x[7]));
       if (is_q) {
         if (bad) y = make_uint4(0u, 0u, 0u, 0u);
-        reinterpret_cast<uint4*>(a.q_out + (int64_t)tok * a.q_stride)[h * LPH + hl] = y;
-      } else if (live && !bad && slot >= 0) {
-        const bool is_k = h < a.n_q + n_kv;
-        const uint32_t kh = h - a.n_q - (is_k ? 0u : n_kv);
-        uint16_t* base = is_k ? a.kv.k : a.kv.v;
-        *reinterpret_cast<uint4*>(base + page_off + (int64_t)kh * a.kv.head_stride + hl * 8) = y;
+        nr_store<STYLE>(a.q_out + (int64_t)tok * a.q_stride + h * HD, hl, HD, y);
+      } else if (h < heads && !bad && slot >= 0) {
+        const uint32_t kh = h - a.n_q - (is_v ? n_kv : 0u);
+        nr_store<STYLE>((is_v ? a.kv.v : a.kv.k) + page_off + (int64_t)kh * a.kv.head_stride, hl, HD, y);
       }
       const uint32_t hn = h + kNrUnroll * HPS;
-      if (hn < heads) u[i] = __ldcs(src + hn * LPH + hl);
+      if (hn < heads) u[i] = nr_load<STYLE>(src + hn * HD, hl, HD);
     }
   }
 }
@@ -462,7 +470,7 @@ int nnz_qk_norm_rope_paged(const nnz_paged_kv* kv, const nnz_norm_rope_args* p, 
       p->q_stride < p->num_query_heads * hd)
     return refuse(NNZ_EINVAL, "nnz_qk_norm_rope_paged: row strides must be multiples of 8 elements that hold the heads");
   if (!aligned16(p->qkv) || !aligned16(p->q_out) || !aligned16(p->q_norm) || !aligned16(p->k_norm) ||
-      (reinterpret_cast<uintptr_t>(p->rope_table) & 7))
+      (reinterpret_cast<uintptr_t>(p->rope_table) & 15))
     return refuse(NNZ_EINVAL, "nnz_qk_norm_rope_paged: pointers must be 16-byte aligned");
   NormRopeArgs a{};
   int sms = 0;

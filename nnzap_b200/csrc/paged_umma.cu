@@ -157,31 +157,6 @@ __device__ __forceinline__ float2 split2(uint64_t a) {
   return r;
 }
 
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-// 2^a, 2^b on the FMA pipe: a = n + f with n the nearest integer (adding 1.5 x
-// 2^23 leaves it in the low mantissa bits), |f| <= 1/2, 2^f by its degree-4
-// polynomial of least largest relative error (2.6e-6, fitted by reweighted
-// least squares), 2^n from its exponent bits.  Below -127: 0; NaN: NaN.
-__device__ __forceinline__ float2 ex2_fma(float a, float b) {
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));     // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
-  const uint64_t y = pair2(a, b);
-  const uint64_t t = add2(y, pair2(12582912.f, 12582912.f));
-  const uint64_t n = add2(t, pair2(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, pair2(-1.f, -1.f), y);
-  uint64_t p = fma2(f, pair2(0.0095701011f, 0.0095701011f), pair2(0.0559178591f, 0.0559178591f));
-  p = fma2(p, f, pair2(0.2402474433f, 0.2402474433f));
-  p = fma2(p, f, pair2(0.6931217909f, 0.6931217909f));
-  p = fma2(p, f, pair2(0.9999992847f, 0.9999992847f));
-  const float2 k = split2(t);
-  return split2(mul2(p, pair2(__int_as_float((__float_as_int(k.x) << 23) + 0x3F800000), __int_as_float((__float_as_int(k.y) << 23) + 0x3F800000))));
-}
-
 // Sets the scores of 64 keys of a row that it does not see to -infinity, in
 // TMEM: it sees the first `end`, on pages whose bit is set (one bit per 2^sh
 // keys).  (Rolled: this runs a few times per task, and instructions have to
@@ -236,9 +211,9 @@ __device__ __forceinline__ float um_pass(uint32_t tS, float sl2, float ms, uint3
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
       const float2 y = split2(fma2(pair2(__uint_as_float(v[c & 1][e]), __uint_as_float(v[c & 1][e + 1])), k2, m2));
-      // a quarter of the exponentials on the FMA pipe: both row tiles' on the
-      // special-function units alone take 2 x 1024 cycles per unit
-      const float2 q = ((e >> 1) & 3) == 3 ? ex2_fma(y.x, y.y) : make_float2(ex2(y.x), ex2(y.y));
+      // (all on the special-function units: a polynomial for every fourth on
+      // the FMA pipe made it 235 instead of 229 us for 4096 tokens)
+      const float2 q = make_float2(ex2(y.x), ex2(y.y));
       acc[(e >> 1) & 1] = add2(acc[(e >> 1) & 1], pair2(q.x, q.y));
       w[8 * c + e / 2] = T16<T>::pack(q.x, q.y);
     }
