@@ -20,7 +20,6 @@ runs in the CUDA library; this module checks and marshals arguments.
 from __future__ import annotations
 
 import ctypes as C
-import typing
 
 import torch
 
@@ -174,12 +173,36 @@ class PagedAttention:
         return out
 
 
-class TokenLogprobs(typing.NamedTuple):
-    logprob: torch.Tensor | None        # float32, the given tokens' shape
-    entropy: torch.Tensor               # float32 [rows]
-    logsumexp: torch.Tensor             # float32 [rows]
-    top_ids: torch.Tensor | None        # int32 [rows][top_k]
-    top_logprobs: torch.Tensor | None   # float32 [rows][top_k]
+class TokenLogprobs:
+    """What :func:`token_logprobs` returns: views of one allocation, made when they are asked for."""
+    __slots__ = ("_f", "_shape", "_rows", "_m", "_k", "top_ids")
+
+    def __init__(self, f, shape, rows, m, k, top_ids):
+        self._f, self._shape, self._rows, self._m, self._k, self.top_ids = f, shape, rows, m, k, top_ids
+
+    @property
+    def entropy(self) -> torch.Tensor:
+        """float32 [rows]"""
+        return self._f.as_strided((self._rows,), (1,), 0)
+
+    @property
+    def logsumexp(self) -> torch.Tensor:
+        """float32 [rows]"""
+        return self._f.as_strided((self._rows,), (1,), self._rows)
+
+    @property
+    def logprob(self) -> torch.Tensor | None:
+        """float32, the given tokens' shape"""
+        if self._shape is None:
+            return None
+        return self._f.as_strided(self._shape, (1,) if len(self._shape) == 1 else (self._m, 1), 2 * self._rows)
+
+    @property
+    def top_logprobs(self) -> torch.Tensor | None:
+        """float32 [rows][top_k]; ``top_ids`` int32 alike (both None for top_k 0)"""
+        if not self._k:
+            return None
+        return self._f.as_strided((self._rows, self._k), (self._k, 1), (2 + self._m) * self._rows)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0) -> TokenLogprobs:
@@ -200,22 +223,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     else:
         m = 1 if tokens.dim() == 1 else tokens.shape[1]
         a.tokens = _index(tokens, torch.int32, (rows,) if tokens.dim() == 1 else (rows, m), dev, "tokens")
-    f32 = {"dtype": torch.float32, "device": dev}
-    lp = None if tokens is None else torch.empty(tokens.shape, **f32)
-    ent, lse = torch.empty(rows, **f32), torch.empty(rows, **f32)
-    ids = top = None
-    if top_k:
-        ids, top = torch.empty((rows, top_k), dtype=torch.int32, device=dev), torch.empty((rows, top_k), **f32)
-        a.top_k, a.top_ids, a.top_logprobs = top_k, ids.data_ptr(), top.data_ptr()
+    f = torch.empty(rows * (2 + m + top_k), dtype=torch.float32, device=dev)     # entropy | logsumexp | logprob | top
+    p, ids = f.data_ptr(), None
+    a.entropy, a.logsumexp = p, p + 4 * rows
     if m:
-        a.num_tokens, a.logprob = m, lp.data_ptr()
+        a.num_tokens, a.logprob = m, p + 8 * rows
+    if top_k:
+        ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+        a.top_k, a.top_ids, a.top_logprobs = top_k, ids.data_ptr(), p + 4 * rows * (2 + m)
     a.logits, a.dtype, a.rows, a.n = logits.data_ptr(), _DTYPES[logits.dtype], rows, n
     a.stride = logits.stride(0) if rows > 1 else n
-    a.entropy, a.logsumexp = ent.data_ptr(), lse.data_ptr()
     rc = lib().nnz_token_logprobs(C.byref(a), _stream(dev.index))
     if rc:
         check(rc)
-    return TokenLogprobs(lp, ent, lse, ids, top)
+    return TokenLogprobs(f, None if tokens is None else tuple(tokens.shape), rows, m, top_k, ids)
 
 
 def stream_check() -> None:
