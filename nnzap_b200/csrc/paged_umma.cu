@@ -7,7 +7,7 @@
 // runs, one per CTA and SM (paged_sched.cuh).  Per unit, for each of the two
 // row tiles:
 //   S = Q K^T           tcgen05.mma, operands in shared memory, f32 in TMEM
-//   P = 2^(S c - m)     one thread per row: online softmax out of TMEM, P in
+//   P = 2^(S c - m)     two threads per row: online softmax out of TMEM, P in
 //                       the pool's type over the S it came from
 //   O += P V            tcgen05.mma, P from TMEM, V as stored (MN-major B)
 // so while one row tile's softmax runs, the tensor cores work for the other.
@@ -21,12 +21,12 @@
 //
 // Roles: warps 0-7 and 8-15 softmax and epilogue of row tiles 0 and 1 (TMEM lane
 // = row; warps 0-3 of a tile have keys 0-63 of a unit and the lower half of the
-// output's dims, 4-7 the others), warp 16 finds the CTA's run of units, hands
-// its parts to the others and loads them (Q, then K and V tiles into one ring,
-// boxes of one page each, one per lane), warp 17 MMA issue, warp 19 cleans the
-// V tiles at the diagonal and at the end.  Boxes of absent pages and past the length are
-// loaded from beyond the pool's last page: the copy engine fills them with
-// zeros, so no stale byte meets the product.
+// output's dims, 4-7 the others; together they clean the V tiles at the
+// diagonal and at the end), warp 16 finds the CTA's run of units, hands its
+// parts to the others and loads them (Q, then K and V tiles into one ring,
+// boxes of one page each, one per lane), warp 17 MMA issue.  Boxes of absent
+// pages and past the length are loaded from beyond the pool's last page: the
+// copy engine fills them with zeros, so no stale byte meets the product.
 //
 // TMEM: S of the two row tiles at columns 0 and 128, O at 256 and 384; P of keys
 // 0-63 and 64-127 over the first 32 columns of their halves of S.
@@ -50,7 +50,7 @@ constexpr int kUmThreads = 640;
 // each (32 words of P, two eighths of S), the fifth goes down to 64: 4 x 128 x
 // 104 + 128 x 64 = 61440.
 constexpr int kUmRegsSoftmax = 104, kUmRegsIssue = 64;
-constexpr int kWTma = 16, kWMma = 17, kWClean = 19;      // warps (18 only makes the fifth warpgroup whole)
+constexpr int kWTma = 16, kWMma = 17;             // warps (18 and 19 only make the fifth warpgroup whole)
 constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
 constexpr uint32_t kPartCost = 3;                 // what a part costs besides its units, in units (queries, epilogue, merge)
@@ -257,6 +257,13 @@ __device__ __forceinline__ uint32_t bad_mask(uint32_t w) {
   return ((w & e) == e ? 0xFFFFu : 0u) | (((w >> 16) & e) == e ? 0xFFFF0000u : 0u);
 }
 
+// Not 0: a non-finite element among the two.
+template <bool BF16>
+__device__ __forceinline__ uint32_t bad_any(uint32_t w) {
+  constexpr uint32_t e = BF16 ? 0x7F807F80u : 0x7C007C00u, one = BF16 ? 0x00800080u : 0x04000400u;
+  return ((w & e) + one) & 0x80008000u;
+}
+
 // The part of one task in a CTA's run, as warp 16 hands it to the others.
 struct Segment {
   uint32_t take;       // units (0: the run is over)
@@ -267,7 +274,7 @@ struct Segment {
   uint32_t s, kvh;
   int row0;            // q / out row of the task's first token
   int rows;            // tokens of the task
-  uint32_t marks[8];   // keys with a non-finite V, among the task's last 256 (set by the MMA warp)
+  uint32_t marks[8];   // keys with a non-finite V, among the task's last 256
   int d, e;            // token i of the task sees keys [0, clamp(d + i, 0, e))
 
   __device__ __forceinline__ int seen(int i) const { return max(0, min(d + i, e)); }
@@ -315,10 +322,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint64_t* s_full = q_empty + 1;        // [2] S of a row tile complete
   uint64_t* p_full = s_full + 2;         // [2] P written, O rescaled (8 warps)
   uint64_t* pv_done = p_full + 2;        // [2] P V complete
-  uint64_t* v_ready = pv_done + 2;       // [kPres] a unit's V tile is ready for the product
+  uint64_t* v_ready = pv_done + 2;       // [kPres] a unit's V tile has been cleaned (units that need it; 16 warps)
   uint64_t* pres_full = v_ready + kPres; // [kPres] page mask of a unit written
   uint64_t* seg_full = pres_full + kPres;   // [kSegs]
-  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 18 other warps are done with it
+  uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 17 other warps are done with it
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + S::OFF_MISC);
   volatile uint32_t* pres = tslot + 1;   // [kPres] one bit per box of the unit: page present
   Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_SEG);
@@ -327,12 +334,12 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   const uint32_t G = a.n_q / a.kv.n_kv;
   const int PT = (int)t.pt, QT = 2 * PT;
   pdl_launch();       // the merge kernel may be set up (it waits for this one's end)
-  // every barrier by its own thread; arrivals: 2 for a free stage (the products
-  // and warp 19), 8 for P (a warp each), 18 for a part's end, else 1
+  // every barrier by its own thread; arrivals: a warp each for P (8), a clean V
+  // tile (16) and a part's end (17), else 1
   static_assert(S::kBars <= kUmThreads);
   if (threadIdx.x < (uint32_t)S::kBars) {
     uint64_t* b = kv_full + threadIdx.x;
-    mbar_init(b, b >= kv_empty && b < q_full ? 2 : b == p_full || b == p_full + 1 ? 8 : b >= seg_empty ? 18 : 1);
+    mbar_init(b, b == p_full || b == p_full + 1 ? 8 : b >= v_ready && b < pres_full ? 16 : b >= seg_empty ? 17 : 1);
     fence_barrier_init();
   }
   if (warp == kWTma && lane < 3) {
@@ -358,7 +365,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       }
   };
 
-  // part k of the run; warps 0-15, 17 and 19 take them in order from warp 16
+  // part k of the run; warps 0-15 and 17 take them in order from warp 16
   // (fields are read into registers one by one: a copy indexed by the row tile
   // would live in local memory, which with this much shared memory means L2)
   auto segment = [&](uint32_t k) -> const Segment* {
@@ -507,6 +514,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     // ---------------- MMA ----------------
     constexpr uint32_t id_s = um_idesc<BF>(128, 128), id_o = um_idesc<BF>(128, HD) | (1u << 16);
     uint32_t stage_use = 0, np[2] = {0, 0}, unit_no = 0;
+    uint32_t vphase = 0;      // bit s: parity of v_ready[s]
     auto issue_s = [&](int x, uint32_t st) {
       if (elect_one()) {
 #pragma unroll
@@ -538,6 +546,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       const Segment* g = segment(seg);
       if (!g) break;
       const uint32_t take = g->take, n0 = g->n[0], n1 = g->n[1];
+      const int mixed0 = g->seen(0) - (int)(g->unit * kUmKeys);      // from this key of the part on, not all rows see all
       wait(q_full, seg);
       for (uint32_t i = 0; i <= take; ++i) {
         // K of unit i, V of unit i - 1 (the ring holds K0 V0 K1 V1 ...)
@@ -546,7 +555,11 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         if (i < take) wait(kv_full + ks, ku / S::kStages);
         if (i > 0) {
           wait(kv_full + vs, vu / S::kStages);
-          wait(v_ready + unit_no % kPres, unit_no / kPres);   // warp 19 has seen to it
+          if ((int)(i * kUmKeys) > mixed0) {                    // (unit i - 1 ends there)
+            const uint32_t slot = unit_no % kPres;
+            wait(v_ready + slot, vphase >> slot);
+            vphase ^= 1u << slot;
+          }
           ++unit_no;
         }
 #pragma unroll
@@ -570,53 +583,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       segment_done(seg);
     }
     if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
-  } else if (warp == kWClean) {
-    // ---------------- V tiles with keys that not every row sees ----------------
-    // A V row past the length is zeroed (its box holds earlier keys), and so is
-    // every non-finite element of a row that some rows see and others do not,
-    // or 0 * V would reach the others; the epilogue adds it to those that do.
-    uint32_t stage_use = 0, unit_no = 0;
-    for (uint32_t seg = 0;; ++seg) {
-      const Segment* g = segment(seg);
-      if (!g) break;
-      const int seen_all = g->seen(0), seen_any = g->seen(g->rows - 1);
-      const uint32_t take = g->take, unit = g->unit;
-      const int base = max(0, seen_any - 256);   // key of the first mark
-      for (uint32_t i = 0; i < take; ++i) {
-#pragma unroll 1
-        for (int kv = 0; kv < 2; ++kv, ++stage_use) {
-          const uint32_t st = stage_use % S::kStages;
-          wait(kv_full + st, stage_use / S::kStages);
-          const int key0 = (int)((unit + i) * kUmKeys);
-          if (kv && key0 + kUmKeys > seen_all) {
-            const int r0 = max(0, seen_all - key0);
-            constexpr int CH = HD / 8;           // 16-byte chunks of a row
-#pragma unroll 4
-            for (int e = r0 * CH + lane; e < kUmKeys * CH; e += 32) {
-              const int r = e / CH, ch = e % CH;
-              uint4* p4 = reinterpret_cast<uint4*>(sm + S::OFF_KV + st * S::kTileB + (ch >> 3) * kHalfB + sw128_off((uint32_t)r, (uint32_t)(ch & 7)));
-              const bool gone = key0 + r >= seen_any;
-              const uint4 w = *p4;
-              const uint32_t b0 = bad_mask<BF>(w.x), b1 = bad_mask<BF>(w.y), b2 = bad_mask<BF>(w.z), b3 = bad_mask<BF>(w.w);
-              const bool bad = (b0 | b1 | b2 | b3) != 0;
-              if (gone || bad) *p4 = gone ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w.x & ~b0, w.y & ~b1, w.z & ~b2, w.w & ~b3);
-              if (bad && !gone) {
-                const uint32_t bit = (uint32_t)(key0 + r - base);
-                atomicOr(segs[seg % kSegs].marks + (bit >> 5), 1u << (bit & 31));
-              }
-            }
-            fence_async_smem();
-          }
-          __syncwarp();
-          if (lane == 0) {
-            if (kv) mbar_arrive1(v_ready + unit_no % kPres);
-            mbar_arrive1(kv_empty + st);
-          }
-        }
-        ++unit_no;
-      }
-      segment_done(seg);
-    }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUmRegsSoftmax));
@@ -639,6 +605,42 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       const int limit = live ? g->seen(tok) : 0;
       const bool tile = x * PT < rows;
       const int seen_all = g->seen(x * PT);
+      const int task_all = g->seen(0), task_any = g->seen(rows - 1);   // keys that all rows of the task see, that any sees
+      // A V row past the length is zeroed (its box holds earlier keys), and so
+      // is every non-finite element of a row that some rows see and others do
+      // not, or 0 * V would reach the others; the epilogue adds it to those
+      // that do.  The 16 warps share the tile: one alone, with 8 loads in
+      // flight beside the products', would need longer than a unit takes.
+      auto clean = [&](uint32_t i) {
+        constexpr int CH = HD / 8, N = 16 * 32;           // 16-byte chunks of a row; threads
+        const int key0 = (int)((unit + i) * kUmKeys);
+        const uint32_t use = 2 * (unit_no + i) + 1, st = use % S::kStages;
+        const int lo = max(0, task_all - key0) * CH, hi = min(kUmKeys, max(0, task_any - key0)) * CH;
+        const int base = max(0, task_any - 256);          // key of the first mark
+        auto chunk = [&](int e) {
+          return reinterpret_cast<uint4*>(sm + S::OFF_KV + st * S::kTileB + (e % CH >> 3) * kHalfB + sw128_off((uint32_t)(e / CH), (uint32_t)(e % CH & 7)));
+        };
+        wait(kv_full + st, use / S::kStages);
+        for (int e = hi + (int)threadIdx.x; e < kUmKeys * CH; e += N) *chunk(e) = make_uint4(0u, 0u, 0u, 0u);
+        uint4 v[kUmKeys * CH / N];
+#pragma unroll
+        for (int j = 0; j < kUmKeys * CH / N; ++j) {
+          const int e = lo + (int)threadIdx.x + j * N;
+          v[j] = e < hi ? *chunk(e) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int j = 0; j < kUmKeys * CH / N; ++j) {
+          if (!(bad_any<BF>(v[j].x) | bad_any<BF>(v[j].y) | bad_any<BF>(v[j].z) | bad_any<BF>(v[j].w))) continue;
+          const int e = lo + (int)threadIdx.x + j * N;
+          *chunk(e) = make_uint4(v[j].x & ~bad_mask<BF>(v[j].x), v[j].y & ~bad_mask<BF>(v[j].y), v[j].z & ~bad_mask<BF>(v[j].z),
+                                 v[j].w & ~bad_mask<BF>(v[j].w));
+          const uint32_t bit = (uint32_t)(key0 + e / CH - base);
+          atomicOr(segs[seg % kSegs].marks + (bit >> 5), 1u << (bit & 31));
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(v_ready + (unit_no + i) % kPres);
+      };
       float m = 0.f, l = 0.f;
       bool fresh = true;              // no visible key among this thread's yet
       for (uint32_t i = 0; i < units; ++i) {
@@ -697,6 +699,14 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive1(p_full + x);
         ++ns;
+        if (key0 + kUmKeys > task_all) clean(i);
+      }
+      // units that only the other row tile looks at (every tile of the ring is
+      // waited for in turn: a parity tells one phase from the next, not from
+      // the one after)
+      for (uint32_t i = units; i < take; ++i) {
+        for (uint32_t use = 2 * (unit_no + i), kv = 0; kv < 2; ++kv, ++use) wait(kv_full + use % S::kStages, use / S::kStages);
+        if ((int)((unit + i + 1) * kUmKeys) > task_all) clean(i);
       }
       unit_no += take;
       if (tile) {

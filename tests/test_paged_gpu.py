@@ -190,6 +190,36 @@ def test_paged_attention_long_and_many(lens, hd, page):
     check_attn(attn_case(3, lens, 8, 4, hd, page, "f16", "head"))
 
 
+# one sequence: its heads' keys are cut over clusters whose shape follows the page table's length
+@pytest.mark.parametrize("new,keys", [(1, 0), (1, 1), (1, 16), (1, 17), (1, 130), (1, 515), (2, 1), (4, 4), (3, 2049), (1, 4095), (2, 4097), (1, 9000)])
+@pytest.mark.parametrize("n_q,n_kv,hd,page,dtype,cols", [
+    (16, 8, 128, 16, "f16", 0), (16, 8, 128, 16, "bf16", 300), (8, 2, 64, 24, "bf16", 0), (4, 1, 64, 64, "f16", 80), (32, 32, 128, 8, "f16", 1),
+    (40, 40, 64, 16, "bf16", 300)])
+def test_paged_attention_one_sequence(new, keys, n_q, n_kv, hd, page, dtype, cols):
+    check_attn(attn_case(new + keys, [(new, keys)], n_q, n_kv, hd, page, dtype, "head", extra_cols=max(cols, 1 - keys)))
+
+
+@pytest.mark.parametrize("cols", [1, 300])
+@pytest.mark.parametrize("keys,absent", [(515, 0.5), (5000, 0.3), (5000, 1.0)])
+def test_paged_attention_one_sequence_with_absent_pages(keys, absent, cols):
+    check_attn(attn_case(21, [(2, keys)], 8, 4, 128, 16, "f16", "head", absent=absent, extra_cols=cols))
+
+
+# few rows over lengths that are split within a CTA, over two and over many, next to short ones
+@pytest.mark.parametrize("lens", [[(1, 515)] * 2, [(2, 2048)] * 4, [(1, 1), (1, 6000), (1, 17)], [(4, 33 * i) for i in range(1, 32)],
+                                  [(1, 61 * i) for i in range(70)], [(8, 900), (1, 901), (5, 5)]])
+@pytest.mark.parametrize("n_q,n_kv,hd,page", [(16, 8, 128, 16), (8, 4, 64, 40)])
+def test_paged_attention_small_batches(lens, n_q, n_kv, hd, page):
+    check_attn(attn_case(5, lens, n_q, n_kv, hd, page, "bf16", "both"))
+
+
+# chunks whose tiles end one short of, on and past the edges of 64 and 128 keys
+@pytest.mark.parametrize("new,keys", [(17, 17), (64, 65), (127, 128), (128, 1024), (129, 191), (255, 4099), (513, 513), (1025, 1153)])
+@pytest.mark.parametrize("n_q,n_kv,hd,page", [(16, 8, 128, 16), (8, 2, 64, 64)])
+def test_paged_attention_one_chunk(new, keys, n_q, n_kv, hd, page):
+    check_attn(attn_case(new, [(new, keys)], n_q, n_kv, hd, page, "f16", "token"))
+
+
 def test_paged_attention_padding_rows_and_scale():
     c = attn_case(9, [(3, 50), (9, 80)], 4, 2, 128, 16, "bf16", "head", gap=5, scale=0.25)
     got = check_attn(c)
