@@ -24,7 +24,7 @@
 // output's dims, 4-7 the others; together they clean the V tiles at the
 // diagonal and at the end), warp 16 finds the CTA's run of units, hands its
 // parts to the others and loads them (Q, then K and V tiles into one ring,
-// boxes of one page each, one per lane), warp 17 MMA issue.  Boxes of absent
+// boxes of one page each), warp 17 MMA issue.  Boxes of absent
 // pages and past the length are loaded from beyond the pool's last page: the
 // copy engine fills them with zeros, so no stale byte meets the product.
 //
@@ -333,7 +333,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint32_t* xt = reinterpret_cast<uint32_t*>(sm + S::OFF_XT);     // [2][128] what the two threads of a row tell each other
   const uint32_t G = a.n_q / a.kv.n_kv;
   const int PT = (int)t.pt, QT = 2 * PT;
-  pdl_launch();       // the merge kernel may be set up (it waits for this one's end)
   // every barrier by its own thread; arrivals: a warp each for P (8), a clean V
   // tile (16) and a part's end (17), else 1
   static_assert(S::kBars <= kUmThreads);
@@ -354,6 +353,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tslot;
+  pdl_launch();       // the merge kernel may be set up (it waits for this one's end)
   // Bounded waits: one that gives up leaves no tries to the later ones, and the
   // error is reported at the end (nothing but the poll stands in the loop).
   uint32_t tries = kSpinLimit;
@@ -399,8 +399,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     more = even ? u < u1 : run.parts != 0;
     if (even && more) warp_find(a, QT, kUmKeys, lane, u, mine, c);
     const uint32_t nb = kUmKeys / t.box;
-    const uint32_t bi = (uint32_t)lane % nb, half = (uint32_t)lane / nb;
-    const bool copies = half < (uint32_t)NH;
+    const uint32_t bi = (uint32_t)lane % nb;      // this lane's box of a unit
     uint32_t stage_use = 0, unit_no = 0;
     for (uint32_t seg = 0;; ++seg) {
       // ---- the next part: to the other warps ----
@@ -484,6 +483,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       for (uint32_t i = 0; i < o.take; ++i) {
         if (i + 1 < o.take) npg = page_of(i + 1, nat);
         const uint32_t mask = __ballot_sync(0xffffffffu, (uint32_t)lane < nb && pg >= 0);
+        if (pg < 0) pg = (int)a.kv.num_pages;
         const int slot = (int)(unit_no % kPres);
         if (lane == 0) {
           pres[slot] = mask;
@@ -496,9 +496,18 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           __syncwarp();
           if (lane == 0) mbar_arrive_expect_tx(kv_full + st, S::kTileB);
           __syncwarp();
-          if (copies)
-            tma_load_4d(sm + S::OFF_KV + st * S::kTileB + half * kHalfB + bi * t.box * 128, kv ? &t.tmV : &t.tmK, (int)half * 64, (int)at,
-                        (int)o.kvh, pg >= 0 ? pg : (int)a.kv.num_pages, kv_full + st);
+          // one elected lane issues (a lane each takes the compiler's loop over
+          // divergent operands, about 100 cycles a copy)
+          uint8_t* dst = sm + S::OFF_KV + st * S::kTileB;
+          const CUtensorMap* tm = kv ? &t.tmV : &t.tmK;
+#pragma unroll 4
+          for (uint32_t b = 0; b < nb; ++b, dst += t.box * 128) {
+            const int bp = __shfl_sync(0xffffffffu, pg, (int)b), bo = (int)__shfl_sync(0xffffffffu, at, (int)b);
+            if (elect_one())
+#pragma unroll
+              for (int h = 0; h < NH; ++h) tma_load_4d(dst + h * kHalfB, tm, h * 64, bo, (int)o.kvh, bp, kv_full + st);
+          }
+          __syncwarp();
           ++stage_use;
           if (kv == 0 && i == 0) {
             if (seg) queries();
