@@ -325,7 +325,8 @@ typedef struct nnz_norm_rope_args {
   const float* k_norm;
   float eps;
   int32_t rope_style;             /* NNZ_ROPE_* */
-  const float* rope_table;        /* f32 [table_positions][head_dim / 2][2] (cos, sin) */
+  const float* rope_table;        /* f32 [table_positions][head_dim / 2][2] (cos, sin), 16-byte aligned like
+                                   * q_norm, k_norm, qkv and q_out */
   uint32_t table_positions;
   const int32_t* positions;       /* [tokens] */
   const int64_t* slots;           /* [tokens] page * page_size + place in the page; negative: not written */
@@ -342,7 +343,7 @@ typedef struct nnz_norm_rope_args {
 int nnz_qk_norm_rope_paged(const nnz_paged_kv* kv, const nnz_norm_rope_args* args, void* stream);
 
 typedef struct nnz_paged_attn_args {
-  const void* q;                  /* [tokens][q_stride], the pool's dtype; normed and rotated */
+  const void* q;                  /* [tokens][q_stride], the pool's dtype; normed and rotated; 16-byte aligned */
   int64_t q_stride;               /* elements, multiple of 8 */
   uint32_t tokens;                /* rows of q and out */
   uint32_t num_query_heads;       /* multiple (<= 64x) of num_kv_heads */
@@ -353,7 +354,7 @@ typedef struct nnz_paged_attn_args {
   const int32_t* page_table;      /* [num_seqs][table_stride] pages in order; negative: absent (evicted) */
   uint32_t table_stride;          /* table_stride * page_size <= 2^31 - 2^16 */
   float scale;                    /* 0: 1 / sqrt(head_dim) */
-  void* out;                      /* [tokens][out_stride] */
+  void* out;                      /* [tokens][out_stride], 16-byte aligned */
   int64_t out_stride;             /* elements, multiple of 8 */
   void* workspace;                /* nnz_paged_attn_workspace bytes, 256-byte aligned, zeroed by the caller
                                    * before its first use (calls leave it as they found it); one call at a time */

@@ -5,7 +5,8 @@
 // of KT keys (one unit at least, so that rows without keys get their zeros).
 // Worker w takes units [w per, (w + 1) per) of the concatenation in task
 // order: whatever the mix of lengths, all workers finish together, and a
-// worker splits at most two tasks (its first and its last).  A worker that
+// worker splits at most two tasks (its first and its last).  Where there are
+// few tasks, a worker may take one part of one task instead (warp_parts).  A worker that
 // holds a whole task writes its output; the parts of a split task (max, sum,
 // sum p v) meet in the workspace and are merged by whoever finishes last.  The
 // cut and the order of the merge depend on the lengths alone, so results do

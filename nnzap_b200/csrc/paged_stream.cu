@@ -4,11 +4,13 @@
 //
 // Every warp is a worker of the shared cut (paged_sched.cuh), 8 to a CTA and a
 // CTA to an SM; the parts of a split task meet first within the CTA, then
-// (where it spans CTAs) in the workspace.  A warp streams its
-// run of 16-key units through a private ring of shared memory, each unit four
-// (or, with pages whose size is only a multiple of 8, eight) TMA copies of K
-// and V halves with the 128-byte swizzle, issued one per lane, so a unit's
-// page may lie anywhere and ldmatrix reads without conflicts.  S = Q K^T and
+// (where it spans CTAs) in the workspace, or, for one sequence, through the
+// distributed shared memory of a cluster.  A warp streams its run of 16-key
+// units through a private ring of shared memory, each unit four (or, with
+// pages whose size is only a multiple of 8, eight) TMA copies of K and V
+// halves with the 128-byte swizzle, so a unit's page may lie anywhere and
+// ldmatrix reads without conflicts.  16 keys and 8 warps: a page of 16 is one
+// unit, and 8 rings of 24 KB keep 190 KB of an SM's memory in flight.  S = Q K^T and
 // O += P V are mma.m16n8k16 with the G heads of every new token as rows; the
 // online softmax keeps its f32 maximum and sum in the score fragments' lanes.
 // The ring runs ahead across task boundaries.  Page numbers are read 32
@@ -16,6 +18,11 @@
 //
 // Absent pages and keys past the length are not loaded or not trusted: their
 // scores are masked, their V rows zeroed in shared memory.
+//
+// Measured (16 / 8 heads of 128, f16): 64 single tokens over 2017 .. 4032 keys
+// 133 to 140 us, 5.9 TB/s of K and V, 0.9 of a plain copy's rate; one token
+// over 32767 keys (bf16) 31.5 us, 4.3 TB/s, and over 515 keys 6.8 us, which is
+// the launch, two dependent loads, four units and the merge over the cluster.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -144,9 +151,11 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   const int G = (int)(a.n_q / a.kv.n_kv);
   const int QT = (int)a.max_new;           // one tile holds all rows
   // The run of this warp.  One sequence: its part of the head that the cluster
-  // has.  Few tasks: of a part of one task that the CTA has for itself.  Else:
-  // of the even cut.  Positions of units: within the task, or (even cut) in
-  // all tasks' concatenation.
+  // has.  Few tasks: of a part of one task that the CTA has for itself, if that
+  // makes no CTA's run longer than a quarter and 8 units (us, against the even
+  // cut: 2 x 515 keys 11.8 / 22.0, 8 x 2048 24.0 / 29.6, 16 x 4000 50.9 / 76.5).
+  // Else: of the even cut.  Positions of units: within the task, or (even cut)
+  // in all tasks' concatenation.
   const uint32_t worker = blockIdx.x * kStWarps + warp;
   Cursor c;
   PartRun run{0, 0, 0};
