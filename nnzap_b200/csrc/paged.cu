@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kNrThreads, 8) norm_rope_kernel(const NormRope
 // softmax in f32.  No tensor cores and no split over the keys: pages that the
 // tiled kernels cannot load (a size that is no multiple of 8) are served
 // right, not fast.  Bound by the latency of a key's loads and warp sum: 64
-// single tokens over 2017 .. 4032 keys 2629 us with pages of 12, against 136 us
+// single tokens over 2017 .. 4032 keys 2629 us with pages of 12, against 139 us
 // with pages of 8 in the streaming kernel.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) paged_attn_any_kernel(const PagedAttnArgs a) {
@@ -545,9 +545,9 @@ int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* s
   // The tiled kernels copy boxes of 8 keys or more of one page; a page whose
   // size is no multiple of 8 would end inside one.  Up to 16 rows of a kv head
   // fit one mma tile and are streamed by single warps (us, against the tcgen05
-  // kernel: 64 single tokens of 2017 .. 4032 keys 140 / 196, one of 515 7.2 /
-  // 22.5, 16 rows of 8000 keys 25.7 / 28.0, 32 x 16 rows of 1000 .. 4000 keys 84
-  // / 106); more rows need several such tiles, and go to tcgen05.
+  // kernel: 64 single tokens of 2017 .. 4032 keys 137 / 192, one of 515 7.2 /
+  // 17.7, 16 rows of 8000 keys 23.8 / 26.6, 32 x 16 rows of 1000 .. 4000 keys 85
+  // / 97); more rows need several such tiles, and go to tcgen05.
   const bool tiled = kv->page_size % 8 == 0;
   const uint64_t rows = (uint64_t)a.max_new * (a.n_q / a.kv.n_kv);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -147,22 +147,20 @@ __device__ __forceinline__ V warp_scan(V v, int lane) {
   return v;
 }
 
-// All units (and tasks), a lane per sequence; `mine`: the lane's units in the
+// All units, a lane per sequence; `mine`: the lane's units in the
 // last 32 sequences.  One lane of one warp of the grid reports lengths that
 // are out of range.
-__device__ __forceinline__ uint64_t warp_total(const PagedAttnArgs& a, int QT, int KT, int lane, bool report, uint64_t& mine, uint64_t* tasks) {
-  uint64_t total = 0, nt = 0;
+__device__ __forceinline__ uint64_t warp_total(const PagedAttnArgs& a, int QT, int KT, int lane, bool report, uint64_t& mine) {
+  uint64_t total = 0;
   for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += 32) {
     mine = 0;
     if (s0 + lane < a.num_seqs) {
       const SeqInfo q = seq_info(a, s0 + lane);
       if (report && seq_bad(a, q)) atomicOr(a.err, ERR_BAD_PAGE);
       mine = head_units(q, QT, KT) * a.kv.n_kv;
-      nt += (uint64_t)((q.rows + QT - 1) / QT) * a.kv.n_kv;
     }
     total += mine;
   }
-  if (tasks) *tasks = warp_sum64(nt);
   return warp_sum64(total);
 }
 
@@ -210,71 +208,86 @@ __device__ __forceinline__ void warp_find(const PagedAttnArgs& a, int QT, int KT
   }
 }
 
+__device__ __forceinline__ uint64_t div_up(uint64_t x, uint32_t y) {
+  return x >> 32 ? (x + y - 1) / y : ((uint32_t)x + (y - 1)) >= y - 1 ? ((uint32_t)x + (y - 1)) / y : (x + y - 1) / y;
+}
+
 // One part of one task per CTA, for few tasks: parts of at most q units, the
-// smallest q of q0 .. q1 (in steps of 1/16) that makes at most `ctas` of them.
-// Lanes hold the (sequence, tile) pairs 32 i + lane, i < N.
+// smallest q of the even cut's .. slack more (in steps of 1/16) that makes at
+// most `ctas` of them; false if there is none.  Lanes hold the (sequence, tile)
+// pairs 32 i + lane, i < N (N > 1: in `sm`, 32 N words, and in loops that are
+// not unrolled: every CTA starts with this, once, and waits for instructions).
 struct PartRun {
   uint32_t part, parts;    // 0 parts: none for this CTA
   uint32_t end;            // of the part within the task (its start: c.unit)
 };
 
-template <int N>
-__device__ __forceinline__ bool warp_parts(const PagedAttnArgs& a, int QT, int KT, int lane, uint32_t ctas, uint32_t q0, uint32_t q1,
-                                           uint32_t cta, Cursor& c, PartRun& run) {
-  const SeqInfo mine = (uint32_t)lane < a.num_seqs ? seq_info(a, (uint32_t)lane) : SeqInfo{0, 0, 0, 0, 0};
+template <int N, typename Slack>
+__device__ __forceinline__ bool warp_parts(const PagedAttnArgs& a, int QT, int KT, int lane, uint32_t ctas, Slack slack, bool report,
+                                           uint32_t cta, uint32_t* sm, Cursor& c, PartRun& run) {
+  if (a.num_seqs > 32) return false;
+  SeqInfo mine{0, 0, 0, 0, 0};
+  if ((uint32_t)lane < a.num_seqs) {
+    mine = seq_info(a, (uint32_t)lane);
+    if (report && seq_bad(a, mine)) atomicOr(a.err, ERR_BAD_PAGE);
+  }
   const int nt = (mine.rows + QT - 1) / QT, inc = warp_scan(nt, lane), D = __shfl_sync(0xffffffffu, inc, 31);
-  if (D > 32 * N) return false;
-  uint32_t eu[N], es[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int j = lane + 32 * i;
-    eu[i] = es[i] = 0;
-    if (32 * i >= D) continue;
+  if (D > 32 * N || (uint32_t)D * a.kv.n_kv > ctas) return false;
+  uint32_t reg = 0, sum = 0;                  // sequence << 27 | units (of 16 keys or more, and keys are below 2^31)
+#pragma unroll 1
+  for (int j0 = 0; j0 < D; j0 += 32) {
+    const int j = j0 + lane;
     int s = 0;        // its sequence: those before it end at or before j
     for (uint32_t l = 0; l < a.num_seqs; ++l) s += __shfl_sync(0xffffffffu, inc, (int)l) <= j ? 1 : 0;
     const int first = __shfl_sync(0xffffffffu, inc - nt, s & 31);
+    uint32_t v = 0;
     if (j < D) {
-      es[i] = (uint32_t)s;
-      eu[i] = tile_units(seq_info(a, (uint32_t)s), j - first, QT, KT);
+      const uint32_t u = tile_units(seq_info(a, (uint32_t)s), j - first, QT, KT);
+      sum += u;
+      v = (uint32_t)s << 27 | u;
     }
+    if constexpr (N > 1) sm[j] = v;
+    else reg = v;
   }
+  if (__any_sync(0xffffffffu, sum >> 26)) return false;      // (the sum over the lanes is 32-bit)
+  auto pair = [&](int j0) { return N > 1 ? sm[j0 + lane] : reg; };
+  constexpr uint32_t kUnits = (1u << 27) - 1;
+  const uint32_t per = max(1u, (uint32_t)div_up((uint64_t)__reduce_add_sync(0xffffffffu, sum) * a.kv.n_kv, ctas));
   const uint32_t cap = ctas / a.kv.n_kv;      // parts of all pairs, per kv head
-  for (uint32_t q = q0; q <= q1; q += max(1u, q / 16)) {
+  const uint32_t q1 = per + slack(per);
+#pragma unroll 1
+  for (uint32_t q = per; q <= q1; q += max(1u, q / 16)) {
     uint32_t n = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) n += 32 * i < D ? (eu[i] + q - 1) / q : 0;
+#pragma unroll 1
+    for (int j0 = 0; j0 < D; j0 += 32) n += ((pair(j0) & kUnits) + q - 1) / q;
     if (__reduce_add_sync(0xffffffffu, n) > cap) continue;
     run = {0, 0, 0};
     uint32_t before = 0;                      // parts in order of pair, kv head, part
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (32 * i >= D) continue;
-      const uint32_t np = (eu[i] + q - 1) / q, all = np * a.kv.n_kv;
+#pragma unroll 1
+    for (int j0 = 0; j0 < D; j0 += 32) {
+      const uint32_t v = pair(j0), np = ((v & kUnits) + q - 1) / q, all = np * a.kv.n_kv;
       const uint32_t incl = before + warp_scan(all, lane);
       const uint32_t hit = __ballot_sync(0xffffffffu, cta < incl && cta >= incl - all);
       if (hit) {
         const int l = __ffs(hit) - 1;
-        const uint32_t rel = cta - __shfl_sync(0xffffffffu, incl - all, l);
+        const uint32_t rel = cta - __shfl_sync(0xffffffffu, incl - all, l), w = __shfl_sync(0xffffffffu, v, l);
         run.parts = __shfl_sync(0xffffffffu, np, l);
-        c.units = __shfl_sync(0xffffffffu, eu[i], l);
-        c.s = __shfl_sync(0xffffffffu, es[i], l);
+        c.units = w & kUnits;
+        c.s = w >> 27;
         c.kvh = rel / run.parts;
-        run.part = rel % run.parts;
-        c.qt = l + 32 * i - (int)__shfl_sync(0xffffffffu, inc - nt, (int)c.s);
-        const uint32_t each = c.units / run.parts, more = c.units % run.parts;     // the first `more` have one unit more
+        run.part = rel - c.kvh * run.parts;
+        c.qt = l + j0 - (int)__shfl_sync(0xffffffffu, inc - nt, (int)c.s);
+        const uint32_t each = c.units / run.parts, more = c.units - each * run.parts;     // the first `more` have one unit more
         c.unit = each * run.part + min(run.part, more);
         run.end = c.unit + each + (run.part < more ? 1u : 0u);
         c.q = seq_info(a, c.s);
+        break;
       }
       before = __shfl_sync(0xffffffffu, incl, 31);
     }
     return true;
   }
   return false;
-}
-
-__device__ __forceinline__ uint64_t div_up(uint64_t x, uint32_t y) {
-  return x >> 32 ? (x + y - 1) / y : ((uint32_t)x + (y - 1)) >= y - 1 ? ((uint32_t)x + (y - 1)) / y : (x + y - 1) / y;
 }
 
 // ---- workspace: a header, a counter and two slots of partials per CTA ----

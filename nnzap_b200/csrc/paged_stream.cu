@@ -20,8 +20,8 @@
 // scores are masked, their V rows zeroed in shared memory.
 //
 // Measured (16 / 8 heads of 128, f16): 64 single tokens over 2017 .. 4032 keys
-// 133 to 140 us, 5.9 TB/s of K and V, 0.9 of a plain copy's rate; one token
-// over 32767 keys (bf16) 31.5 us, 4.3 TB/s, and over 515 keys 6.8 us, which is
+// 137 us, 5.8 TB/s of K and V, 0.88 of a plain copy's rate; one token
+// over 32767 keys (bf16) 30 us, 4.5 TB/s, and over 515 keys 6.7 us, which is
 // the launch, two dependent loads, four units and the merge over the cluster.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -127,7 +127,7 @@ __device__ __forceinline__ void merge_out(const PagedAttnArgs& a, uint32_t row0,
 
 // ROWS8: at most 8 query rows (the lower half of every fragment is absent).
 template <typename T, int HD, bool ROWS8>
-__global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __grid_constant__ StArgs t) {
+__global__ void __launch_bounds__(kStWarps * 32, 1) paged_stream_kernel(const __grid_constant__ StArgs t) {
   using S = StShape<HD>;
   constexpr int NR = ROWS8 ? 1 : 2;        // fragment row halves
   constexpr int KS = HD / 16;              // K steps of S
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
   // The run of this warp.  One sequence: its part of the head that the cluster
   // has.  Few tasks: of a part of one task that the CTA has for itself, if that
   // makes no CTA's run longer than a quarter and 8 units (us, against the even
-  // cut: 2 x 515 keys 11.8 / 22.0, 8 x 2048 24.0 / 29.6, 16 x 4000 50.9 / 76.5).
+  // cut: 2 x 515 keys 11.3 / 16.9, 8 x 2048 22.6 / 29.5, 16 x 4000 50.3 / 74.8).
   // Else: of the even cut.  Positions of units: within the task, or (even cut)
   // in all tasks' concatenation.
   const uint32_t worker = blockIdx.x * kStWarps + warp;
@@ -183,13 +183,10 @@ __global__ void __launch_bounds__(kStWarps * 32) paged_stream_kernel(const __gri
       }
     }
   } else {
-    uint64_t tasks = 0;
-    const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine, &tasks);
-    const uint32_t per_cta = max(1u, (uint32_t)div_up(total, gridDim.x));
-    per = (per_cta + kStWarps - 1) / kStWarps;
-    even = !(tasks <= gridDim.x && a.num_seqs <= 32 &&
-             warp_parts<1>(a, QT, kStKeys, lane, gridDim.x, per_cta, per_cta + per_cta / 4 + 8, blockIdx.x, c, run));
+    even = !warp_parts<1>(a, QT, kStKeys, lane, gridDim.x, [](uint32_t q) { return q / 4 + 8; }, worker == 0, blockIdx.x, nullptr, c, run);
     if (even) {
+      const uint64_t total = warp_total(a, QT, kStKeys, lane, worker == 0, mine);
+      per = (max(1u, (uint32_t)div_up(total, gridDim.x)) + kStWarps - 1) / kStWarps;
       u0 = (uint64_t)worker * per;
       u1 = min(u0 + per, total);
     } else if (run.parts) {

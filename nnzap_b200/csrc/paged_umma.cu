@@ -29,13 +29,13 @@
 // copy engine fills them with zeros, so no stale byte meets the product.
 //
 // Measured (16 / 8 heads of 128): 4096 tokens behind 4096 keys 223 us, 920
-// TFLOP/s of the visible pairs' products; 512 behind 4096 39.6 us.  A unit
+// TFLOP/s of the visible pairs' products; 512 behind 4096 38.4 us.  A unit
 // takes a CTA about 4200 cycles, its four products about 2400 of them: S, the
 // softmax, P V and the next S of a row tile follow one another, TMEM is full
 // with one S and one O of each, and the special-function units alone need 2048
 // cycles for a unit's exponentials.  (Steps of 64 keys with two S of each row
 // tile took 256 us: products of 64 columns are bound by the queries' way from
-// shared memory.)  Of the 512 tokens' time about 8 us are the way to the first
+// shared memory.)  Of the 512 tokens' time about 7 us are the way to the first
 // S (lengths, cut, page numbers, first tiles) and 6 us the merge of the parts.
 //
 // TMEM: S of the two row tiles at columns 0 and 128, O at 256 and 384; P of keys
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   volatile uint32_t* pres = tslot + 1;   // [kPres] one bit per box of the unit: page present
   Segment* segs = reinterpret_cast<Segment*>(sm + S::OFF_SEG);
   static_assert(sizeof(Segment) <= 80 && S::kSmem <= 232448);
-  uint32_t* xt = reinterpret_cast<uint32_t*>(sm + S::OFF_XT);     // [2][128] what the two threads of a row tell each other
+  uint32_t* xt = reinterpret_cast<uint32_t*>(sm + S::OFF_XT);     // [2][128] what the two threads of a row tell each other (before: the cut's pairs)
   const uint32_t G = a.n_q / a.kv.n_kv;
   const int PT = (int)t.pt, QT = 2 * PT;
   // every barrier by its own thread; arrivals: a warp each for P (8), a clean V
@@ -397,19 +397,22 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     uint64_t u = 0, u1 = 0;
     uint32_t per = 1;
     bool even = true, more = false;
-    uint64_t mine = 0, tasks = 0;
-    const uint64_t total = warp_total(a, QT, kUmKeys, lane, blockIdx.x == 0, mine, &tasks);
     const uint32_t P = t.workers;
-    per = max(1u, (uint32_t)div_up(total, P));
     // One part per CTA where that costs no more than kPartCost units over the
-    // even cut (us, against the even cut: 512 tokens of 4608 keys 45.1 / 46.4,
-    // 1024 of 2048 40.9 / 42.0, 31 single tokens and a chunk of 449 36.4 / 42.3;
-    // 128 of 1024 27.5 / 26.6).
-    u = (uint64_t)blockIdx.x * per;
-    u1 = min(u + per, total);     // even cut
-    even = !(tasks <= P && a.num_seqs <= 32 && warp_parts<5>(a, QT, kUmKeys, lane, P, per, per + kPartCost, blockIdx.x, c, run));
-    more = even ? u < u1 : run.parts != 0;
-    if (even && more) warp_find(a, QT, kUmKeys, lane, u, mine, c);
+    // even cut (us, against the even cut: 512 tokens of 4608 keys 38.4 / 43.0,
+    // 1024 of 2048 35.2 / 38.7, 31 single tokens and a chunk of 449 34.6 / 43.2;
+    // 128 of 1024 22.6 / 22.5).
+    even = !warp_parts<5>(a, QT, kUmKeys, lane, P, [](uint32_t) { return kPartCost; }, blockIdx.x == 0, blockIdx.x, xt, c, run);
+    more = run.parts != 0;
+    if (even) {
+      uint64_t mine = 0;
+      const uint64_t total = warp_total(a, QT, kUmKeys, lane, blockIdx.x == 0, mine);
+      per = max(1u, (uint32_t)div_up(total, P));
+      u = (uint64_t)blockIdx.x * per;
+      u1 = min(u + per, total);
+      more = u < u1;
+      if (more) warp_find(a, QT, kUmKeys, lane, u, mine, c);
+    }
     const uint32_t nb = kUmKeys / t.box;
     const uint32_t bi = (uint32_t)lane % nb;      // this lane's box of a unit
     uint32_t stage_use = 0, unit_no = 0;
