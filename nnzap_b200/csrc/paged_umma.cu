@@ -539,12 +539,20 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     constexpr uint32_t id_s = um_idesc<BF>(128, 128), id_o = um_idesc<BF>(128, HD) | (1u << 16);
     uint32_t stage_use = 0, np[2] = {0, 0}, unit_no = 0;
     uint32_t vphase = 0;      // bit s: parity of v_ready[s]
+    // (descriptors are formed where they are used: hoisted out of the loop they
+    // spill, and a word from local memory takes 400 cycles here)
+    auto fresh_base = [&] {
+      uint8_t* p = sm;
+      asm volatile("" : "+l"(p));
+      return p;
+    };
     auto issue_s = [&](int x, uint32_t st) {
       if (elect_one()) {
+        uint8_t* base = fresh_base();
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
-          const uint64_t da = smem_desc_sw128(sm + x * S::kTileB + h * kHalfB);
-          const uint64_t db = smem_desc_sw128(sm + S::OFF_KV + st * S::kTileB + h * kHalfB);
+          const uint64_t da = smem_desc_sw128(base + x * S::kTileB + h * kHalfB);
+          const uint64_t db = smem_desc_sw128(base + S::OFF_KV + st * S::kTileB + h * kHalfB);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) umma_f16(tmem + x * 128, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), id_s, (h | kk) != 0);
         }
@@ -554,10 +562,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     };
     auto issue_o = [&](int x, uint32_t st, bool acc) {
       if (elect_one()) {
+        const uint64_t db = smem_desc_sw128_mn(fresh_base() + S::OFF_KV + st * S::kTileB);
 #pragma unroll
         for (int kk = 0; kk < kUmKeys / 16; ++kk)
-          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + (kk < 4 ? kk * 8 : 32 + kk * 8), smem_desc_sw128_mn(sm + S::OFF_KV + st * S::kTileB + kk * 16 * 128), id_o,
-                  acc || kk != 0);
+          umma_ts(tmem + 256 + x * 128, tmem + x * 128 + (kk < 4 ? kk * 8 : 32 + kk * 8), db + (uint64_t)(kk * (16 * 128 >> 4)), id_o, acc || kk != 0);
         umma_commit(pv_done + x);
       }
       __syncwarp();
@@ -617,19 +625,17 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     const uint32_t tS = tl + x * 128 + half * 64, tO = tl + 256 + x * 128 + half * (HD / 2);
     volatile uint32_t* xr = xt + x * 128 + r;
     uint32_t ns = 0, unit_no = 0;       // units of this row tile, units of the run
-    PartHeader hdr{0, 0, 0, 0};
+    if (threadIdx.x == 0) t.ws.head[blockIdx.x] = {0, 0, 0, 0};
+    // (of a part only what its every unit needs is kept in registers: the
+    // loop's spills are read back from L2)
     for (uint32_t seg = 0;; ++seg) {
       const Segment* g = segment(seg);
       if (!g) break;
-      const int rows = g->rows, row0 = g->row0;
-      const uint32_t take = g->take, unit = g->unit, units = g->n[x], seg_parts = g->parts, kvh = g->kvh;
-      const bool gaps = g->gaps != 0;
-      const int tok = x * PT + (int)(r / G);         // token of the task
-      const bool live = r < (uint32_t)PT * G && tok < rows;
-      const int limit = live ? g->seen(tok) : 0;
-      const bool tile = x * PT < rows;
-      const int seen_all = g->seen(x * PT);
-      const int task_all = g->seen(0), task_any = g->seen(rows - 1);   // keys that all rows of the task see, that any sees
+      const uint32_t units = g->n[x];
+      auto token = [&] { return x * PT + (int)(r / G); };               // of the task
+      const bool live = r < (uint32_t)PT * G && token() < g->rows;
+      // the first unit with a key that some row of the task does not see
+      const uint32_t special = g->gaps ? 0u : (uint32_t)max(0, g->seen(0) / kUmKeys - (int)g->unit);
       // A V row past the length is zeroed (its box holds earlier keys), and so
       // is every non-finite element of a row that some rows see and others do
       // not, or 0 * V would reach the others; the epilogue adds it to those
@@ -637,7 +643,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       // flight beside the products', would need longer than a unit takes.
       auto clean = [&](uint32_t i) {
         constexpr int CH = HD / 8, N = 16 * 32;           // 16-byte chunks of a row; threads
-        const int key0 = (int)((unit + i) * kUmKeys);
+        const int key0 = (int)((g->unit + i) * kUmKeys), task_all = g->seen(0), task_any = g->seen(g->rows - 1);
+        if (key0 + kUmKeys <= task_all) return;
         const uint32_t use = 2 * (unit_no + i) + 1, st = use % S::kStages;
         const int lo = max(0, task_all - key0) * CH, hi = min(kUmKeys, max(0, task_any - key0)) * CH;
         const int base = max(0, task_any - 256);          // key of the first mark
@@ -670,19 +677,20 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       for (uint32_t i = 0; i < units; ++i) {
         wait(s_full + x, ns);
         tc_fence_after();
-        // page masks only where the part has absent pages
-        uint32_t mask = 0xFFFFu;
-        const uint32_t sh = 31 - __clz(t.box);
-        if (gaps) {
-          const uint32_t un = unit_no + i;
-          wait(pres_full + un % kPres, un / kPres);
-          mask = pres[un % kPres];
+        if (i >= special) {
+          const int key0 = (int)((g->unit + i) * kUmKeys);
+          uint32_t mask = 0xFFFFu;
+          const uint32_t sh = 31 - __clz(t.box);
+          if (g->gaps) {
+            const uint32_t un = unit_no + i;
+            wait(pres_full + un % kPres, un / kPres);
+            mask = pres[un % kPres];
+          }
+          if (g->gaps || key0 + kUmKeys > g->seen(x * PT))
+            um_mask(tS, (live ? g->seen(token()) : 0) - key0 - 64 * half, mask >> ((64 * half) >> sh), sh);
         }
-        const int key0 = (int)((unit + i) * kUmKeys);
         uint32_t w[32];
         float sum;
-        if (gaps || key0 + kUmKeys > seen_all)
-          um_mask(tS, limit - key0 - 64 * half, mask >> ((64 * half) >> sh), sh);
         for (bool first = true;; first = false) {
           sum = um_pass<T>(tS, t.sl2, m, w);
           // Out of range: a sum of 2^15 or more (or NaN), or of less than 1/4
@@ -723,26 +731,28 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive1(p_full + x);
         ++ns;
-        if (key0 + kUmKeys > task_all) clean(i);
+        if (i >= special) clean(i);
       }
       // units that only the other row tile looks at (every tile of the ring is
       // waited for in turn: a parity tells one phase from the next, not from
       // the one after)
-      for (uint32_t i = units; i < take; ++i) {
+      for (uint32_t i = units; i < g->take; ++i) {
         for (uint32_t use = 2 * (unit_no + i), kv = 0; kv < 2; ++kv, ++use) wait(kv_full + use % S::kStages, use / S::kStages);
-        if ((int)((unit + i + 1) * kUmKeys) > task_all) clean(i);
+        clean(i);
       }
-      unit_no += take;
-      if (tile) {
+      unit_no += g->take;
+      if (x * PT < g->rows) {
         // the row's sum: both halves', in one order
         l = pair_tell(bar, xr, half, 0, l) + pair_tell(bar, xr, half, 1, l);
-        const bool whole = seg_parts == 0, first = unit == 0;
+        const bool whole = g->parts == 0, first = g->unit == 0;
+        const int tok = token(), row0 = g->row0;
+        const uint32_t kvh = g->kvh;
         const float il = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         const uint32_t rr = (uint32_t)x * PT * G + r;
         uint16_t* op = a.out + (int64_t)(row0 + tok) * a.out_stride + (int64_t)(kvh * G + r % G) * HD + half * (HD / 2);
         float* slot = t.ws.slot(blockIdx.x, first ? 1 : 0, HD);
         float* part = slot + 2 * t.ws.R + (size_t)rr * 4 + (size_t)half * (HD / 2) * t.ws.R;   // [HD / 4][R][4]: lanes side by side
-        if (first && !whole) hdr = {(uint32_t)row0, kvh, (uint32_t)rows * G, seg_parts};
+        if (first && !whole && threadIdx.x == 0) t.ws.head[blockIdx.x] = {(uint32_t)row0, kvh, (uint32_t)g->rows * G, g->parts};
         if (live && !whole && half == 0) {
           slot[rr] = l == 0.f ? -INFINITY : m;
           slot[t.ws.R + rr] = l;
@@ -765,7 +775,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           }
 #pragma unroll
           for (int d = 0; d < 32; ++d) o[d] = units ? __uint_as_float(w[d]) * il : 0.f;
-          if (marks) add_nonfinite<BF>(a, *g, mk, limit, half * (HD / 2) + 32 * c, o);
+          if (marks) add_nonfinite<BF>(a, *g, mk, live ? g->seen(tok) : 0, half * (HD / 2) + 32 * c, o);
           if (live && whole) {
 #pragma unroll
             for (int d = 0; d < 32; d += 8)
@@ -781,7 +791,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       }
       segment_done(seg);
     }
-    if (threadIdx.x == 0) t.ws.head[blockIdx.x] = hdr;
   }
   if (!tries && lane == 0) atomicOr(a.err, ERR_MBAR_TIMEOUT);
   tc_fence_before();
