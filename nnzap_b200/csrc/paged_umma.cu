@@ -28,9 +28,9 @@
 // pages and past the length are loaded from beyond the pool's last page: the
 // copy engine fills them with zeros, so no stale byte meets the product.
 //
-// Measured (16 / 8 heads of 128): 4096 tokens behind 4096 keys 223 us, 920
-// TFLOP/s of the visible pairs' products; 512 behind 4096 38.4 us.  A unit
-// takes a CTA about 4200 cycles, its four products about 2400 of them: S, the
+// Measured (16 / 8 heads of 128): 4096 tokens behind 4096 keys 213 us, 965
+// TFLOP/s of the visible pairs' products; 512 behind 4096 35 - 36 us.  A unit
+// takes a CTA about 3900 cycles, its four products 2100 to 2800 of them: S, the
 // softmax, P V and the next S of a row tile follow one another, TMEM is full
 // with one S and one O of each, and the special-function units alone need 2048
 // cycles for a unit's exponentials.  (Steps of 64 keys with two S of each row
@@ -55,12 +55,12 @@ namespace nnz {
 namespace {
 
 constexpr int kUmKeys = 128;
-constexpr int kUmThreads = 640;
-// Registers a thread: 640 x 96 at launch; the four softmax warpgroups take 104
-// each (32 words of P, two eighths of S), the fifth goes down to 64: 4 x 128 x
-// 104 + 128 x 64 = 61440.
-constexpr int kUmRegsSoftmax = 104, kUmRegsIssue = 64;
-constexpr int kWTma = 16, kWMma = 17;             // warps (18 and 19 only make the fifth warpgroup whole)
+// 96 registers a thread.  (A fifth whole warpgroup that gave its registers to
+// the softmax warps, 104 / 64, took 36.4 instead of 34.9 us for 512 tokens: the
+// warps that load and issue then spill.)
+constexpr int kUmThreads = 576;
+constexpr uint32_t kUmTries = 1u << 18;          // polls of a wait: every wait is for this CTA's own warps and copies
+constexpr int kWTma = 16, kWMma = 17;             // warps
 constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
 constexpr uint32_t kPartCost = 3;                 // what a part costs besides its units, in units (queries, epilogue, merge)
@@ -73,7 +73,7 @@ struct UmShape {
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr uint32_t OFF_KV = 2 * kTileB;
   static constexpr uint32_t OFF_BAR = OFF_KV + kStages * kTileB;
-  static constexpr int kBars = 2 * kStages + 8 + 2 * kPres + 2 * kSegs;
+  static constexpr int kBars = 2 * kStages + 8 + 3 * kPres + 2 * kSegs;
   static constexpr uint32_t OFF_MISC = OFF_BAR + kBars * 8;
   static constexpr uint32_t OFF_SEG = OFF_MISC + 64, OFF_XT = OFF_SEG + kSegs * 80;
   static constexpr uint32_t kSmem = OFF_XT + 1024 + 1024;
@@ -333,7 +333,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint64_t* p_full = s_full + 2;         // [2] P written, O rescaled (8 warps)
   uint64_t* pv_done = p_full + 2;        // [2] P V complete
   uint64_t* v_ready = pv_done + 2;       // [kPres] a unit's V tile has been cleaned (units that need it; 16 warps)
-  uint64_t* pres_full = v_ready + kPres; // [kPres] page mask of a unit written
+  uint64_t* v_go = v_ready + kPres;      // [kPres] such a tile is there (it stays until it has been cleaned)
+  uint64_t* pres_full = v_go + kPres;    // [kPres] page mask of a unit written
   uint64_t* seg_full = pres_full + kPres;   // [kSegs]
   uint64_t* seg_empty = seg_full + kSegs;   // [kSegs] the 17 other warps are done with it
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + S::OFF_MISC);
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   static_assert(S::kBars <= kUmThreads);
   if (threadIdx.x < (uint32_t)S::kBars) {
     uint64_t* b = kv_full + threadIdx.x;
-    mbar_init(b, b == p_full || b == p_full + 1 ? 8 : b >= v_ready && b < pres_full ? 16 : b >= seg_empty ? 17 : 1);
+    mbar_init(b, b == p_full || b == p_full + 1 ? 8 : b >= v_ready && b < v_go ? 16 : b >= seg_empty ? 17 : 1);
     fence_barrier_init();
   }
   if (warp == kWTma && lane < 3) {
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   pdl_launch();       // the merge kernel may be set up (it waits for this one's end)
   // Bounded waits: one that gives up leaves no tries to the later ones, and the
   // error is reported at the end (nothing but the poll stands in the loop).
-  uint32_t tries = kSpinLimit;
+  uint32_t tries = kUmTries;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     for (uint32_t n = 0; !mbar_try_wait(bar, parity & 1u);)
       if (++n > tries) {
@@ -389,7 +390,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   };
 
   if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUmRegsIssue));
   if (warp == kWTma) {
     // ---------------- the run, and its TMA ----------------
     Cursor c;
@@ -570,10 +570,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       }
       __syncwarp();
     };
-    auto release = [&](uint64_t* bar) {
-      if (elect_one()) umma_commit(bar);
-      __syncwarp();
-    };
     for (uint32_t seg = 0;; ++seg) {
       const Segment* g = segment(seg);
       if (!g) break;
@@ -606,10 +602,18 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
             tc_fence_after();
             issue_s(x, ks);
           }
+          if (x == 0 && i < take && (int)((i + 1) * kUmKeys) > mixed0) {     // V of unit i has to be cleaned
+            wait(kv_full + (ku + 1) % S::kStages, (ku + 1) / S::kStages);
+            if (elect_one()) mbar_arrive1(v_go + unit_no % kPres);
+            __syncwarp();
+          }
         }
-        if (i > 0) release(kv_empty + vs);
-        if (i < take) release(kv_empty + ks);
-        if (i + 1 == take) release(q_empty);
+        if (elect_one()) {
+          if (i > 0) umma_commit(kv_empty + vs);
+          if (i < take) umma_commit(kv_empty + ks);
+          if (i + 1 == take) umma_commit(q_empty);
+        }
+        __syncwarp();
       }
       stage_use += 2 * take;
       segment_done(seg);
@@ -617,7 +621,6 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kUmRegsSoftmax));
     // ---------------- softmax and epilogue of row tile x ----------------
     const int x = warp >> 3, half = (warp >> 2) & 1, bar = 1 + 4 * x + (warp & 3);
     const uint32_t r = 32u * (warp & 3) + lane;
@@ -625,6 +628,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     const uint32_t tS = tl + x * 128 + half * 64, tO = tl + 256 + x * 128 + half * (HD / 2);
     volatile uint32_t* xr = xt + x * 128 + r;
     uint32_t ns = 0, unit_no = 0;       // units of this row tile, units of the run
+    uint32_t vphase = 0;                // bit s: parity of v_go[s]
     if (threadIdx.x == 0) t.ws.head[blockIdx.x] = {0, 0, 0, 0};
     // (of a part only what its every unit needs is kept in registers: the
     // loop's spills are read back from L2)
@@ -651,6 +655,12 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         auto chunk = [&](int e) {
           return reinterpret_cast<uint4*>(sm + S::OFF_KV + st * S::kTileB + (e % CH >> 3) * kHalfB + sw128_off((uint32_t)(e / CH), (uint32_t)(e % CH & 7)));
         };
+        // (every warp comes to every such unit, in order, so a parity cannot be
+        // mistaken for another phase's; of kv_full it could, which runs on
+        // without the warps of a row tile that does not look at a unit)
+        const uint32_t slot = (unit_no + i) % kPres;
+        wait(v_go + slot, vphase >> slot);
+        vphase ^= 1u << slot;
         wait(kv_full + st, use / S::kStages);
         for (int e = hi + (int)threadIdx.x; e < kUmKeys * CH; e += N) *chunk(e) = make_uint4(0u, 0u, 0u, 0u);
         uint4 v[kUmKeys * CH / N];
@@ -670,7 +680,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive1(v_ready + (unit_no + i) % kPres);
+        if (lane == 0) mbar_arrive1(v_ready + slot);
       };
       float m = 0.f, l = 0.f;
       bool fresh = true;              // no visible key among this thread's yet
@@ -733,13 +743,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         ++ns;
         if (i >= special) clean(i);
       }
-      // units that only the other row tile looks at (every tile of the ring is
-      // waited for in turn: a parity tells one phase from the next, not from
-      // the one after)
-      for (uint32_t i = units; i < g->take; ++i) {
-        for (uint32_t use = 2 * (unit_no + i), kv = 0; kv < 2; ++kv, ++use) wait(kv_full + use % S::kStages, use / S::kStages);
-        clean(i);
-      }
+      for (uint32_t i = max(units, special); i < g->take; ++i) clean(i);      // units that only the other row tile looks at
       unit_no += g->take;
       if (x * PT < g->rows) {
         // the row's sum: both halves', in one order

@@ -213,6 +213,17 @@ def test_paged_attention_small_batches(lens, n_q, n_kv, hd, page):
     check_attn(attn_case(5, lens, n_q, n_kv, hd, page, "bf16", "both"))
 
 
+def test_paged_attention_short_tails_after_long_epilogues():
+    """Tasks of one row tile (its partner's warps have nothing to do in them) next to tasks of two, several to a CTA."""
+    lens = [(7 + i % 11, 600 + 131 * (i % 7)) for i in range(90)]
+    c = attn_case(13, lens, 40, 2, 128, 16, "f16", "head")
+    first = check_attn(c).clone()
+    op = P().PagedAttention(P().PagedKV(c["k"], c["v"]), c["n_q"])
+    for _ in range(20):
+        assert torch.equal(op(c["q"], c["table"], c["q_start"], c["kv_len"], c["max_new"]), first)
+    P().stream_check()
+
+
 # chunks whose tiles end one short of, on and past the edges of 64 and 128 keys
 @pytest.mark.parametrize("new,keys", [(17, 17), (64, 65), (127, 128), (128, 1024), (129, 191), (255, 4099), (513, 513), (1025, 1153)])
 @pytest.mark.parametrize("n_q,n_kv,hd,page", [(16, 8, 128, 16), (8, 2, 64, 64)])
