@@ -20,8 +20,8 @@
 // scores are masked, their V rows zeroed in shared memory.
 //
 // Measured (16 / 8 heads of 128, f16): 64 single tokens over 2017 .. 4032 keys
-// 137 us, 5.8 TB/s of K and V, 0.88 of a plain copy's rate; one token
-// over 32767 keys (bf16) 30 us, 4.5 TB/s, and over 515 keys 6.7 us, which is
+// 135 us, 5.9 TB/s of K and V, 0.9 of a plain copy's rate; one token
+// over 32767 keys (bf16) 30 us, 4.5 TB/s, and over 515 keys 6.4 us, which is
 // the launch, two dependent loads, four units and the merge over the cluster.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -126,8 +126,11 @@ __device__ __forceinline__ void merge_out(const PagedAttnArgs& a, uint32_t row0,
 }
 
 // ROWS8: at most 8 query rows (the lower half of every fragment is absent).
-template <typename T, int HD, bool ROWS8>
-__global__ void __launch_bounds__(kStWarps * 32, 1) paged_stream_kernel(const __grid_constant__ StArgs t) {
+// CL: one sequence, CTAs in clusters.  (Asked for one CTA to an SM the compiler
+// takes up to 255 registers, which one token over 32767 keys gains from, 30.2
+// instead of 34.8 us, and 64 tokens lose from, 139 instead of 135.)
+template <typename T, int HD, bool ROWS8, bool CL>
+__global__ void __launch_bounds__(kStWarps * 32, CL ? 1 : 0) paged_stream_kernel(const __grid_constant__ StArgs t) {
   using S = StShape<HD>;
   constexpr int NR = ROWS8 ? 1 : 2;        // fragment row halves
   constexpr int KS = HD / 16;              // K steps of S
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(kStWarps * 32, 1) paged_stream_kernel(const __
   bool even = false;
   uint64_t mine = 0, u0 = 0, u1 = 0;
   uint32_t per = 1;
-  if (t.cluster > 1) {
+  if (CL) {
     const uint32_t id = blockIdx.x / t.cluster;
     c.s = 0;
     c.kvh = id / t.clusters;
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(kStWarps * 32, 1) paged_stream_kernel(const __
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
-    if (take == c.units && t.cluster <= 1) {
+    if (take == c.units && !CL) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const int row = g + 8 * r;
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(kStWarps * 32, 1) paged_stream_kernel(const __
   }
   }
 
-  if (t.cluster > 1) {
+  if (CL) {
     // ---- one task: the CTA's parts, then the cluster's in its first CTA ----
     cg::cluster_group cl = cg::this_cluster();
     if (run.part >= run.parts) return;                    // the whole cluster
@@ -640,8 +643,6 @@ __global__ void __launch_bounds__(kStWarps * 32, 1) paged_stream_kernel(const __
 //   even cut  11.5   12.8   20.9    36.1
 template <typename K>
 void stream_clusters(K* fn, StArgs& t, cudaLaunchConfig_t cfg, std::atomic<int> (&fits)[9]) {
-  t.cluster = t.clusters = 1;
-  if (t.a.num_seqs != 1) return;
   const uint64_t keys = (uint64_t)t.a.table_stride * t.a.kv.page_size;
   for (uint32_t C = keys <= 4096 ? 8 : 4; C >= 4; C /= 2) {
     // clusters of C that the device runs at once (asked once)
@@ -671,24 +672,35 @@ void stream_clusters(K* fn, StArgs& t, cudaLaunchConfig_t cfg, std::atomic<int> 
 
 template <typename T, int HD, bool ROWS8>
 cudaError_t stream_go(StArgs t, cudaStream_t st) {
-  static std::atomic<uint64_t> ready{0};
+  static std::atomic<uint64_t> ready[2] = {};
   static std::atomic<int> fits[9];
-  const auto fn = &paged_stream_kernel<T, HD, ROWS8>;
-  const cudaError_t e = raise_smem((const void*)fn, StShape<HD>::kSmem, ready);
-  if (e != cudaSuccess) return e;
+  const auto fn = &paged_stream_kernel<T, HD, ROWS8, false>;
+  const auto fc = &paged_stream_kernel<T, HD, ROWS8, true>;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kStWarps * 32);
   cfg.dynamicSmemBytes = StShape<HD>::kSmem;
   cfg.stream = st;
-  stream_clusters(fn, t, cfg, fits);
+  t.cluster = t.clusters = 1;
+  if (t.a.num_seqs == 1) {
+    const cudaError_t e = raise_smem((const void*)fc, StShape<HD>::kSmem, ready[1]);
+    if (e != cudaSuccess) return e;
+    stream_clusters(fc, t, cfg, fits);
+  }
+  if (t.cluster == 1) {
+    const cudaError_t e = raise_smem((const void*)fn, StShape<HD>::kSmem, ready[0]);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3((uint32_t)t.a.num_sms);
+    cfg.numAttrs = 0;
+    return cudaLaunchKernelEx(&cfg, fn, t);
+  }
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = t.cluster;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(t.cluster > 1 ? t.cluster * t.clusters * t.a.kv.n_kv : (uint32_t)t.a.num_sms);
+  cfg.gridDim = dim3(t.cluster * t.clusters * t.a.kv.n_kv);
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, t);
+  return cudaLaunchKernelEx(&cfg, fc, t);
 }
 
 template <typename T>
