@@ -20,6 +20,7 @@ runs in the CUDA library; this module checks and marshals arguments.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -43,6 +44,12 @@ def _stream(device: int | None = None) -> int:
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+def _own(args):
+    """One call's own copy of an operator's constant arguments: the library reads them with the GIL released,
+    while another thread may be calling the same operator."""
+    return type(args).from_buffer_copy(args)
 
 
 def _index(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device, what: str) -> int:
@@ -117,10 +124,10 @@ class QKNormRope:
         a.k_norm = _index(k_norm, torch.float32, (hd,), kv.device, "k_norm")
         a.rope_table = _index(table, torch.float32, (table.shape[0], hd // 2, 2), kv.device, "table")
         a.table_positions = table.shape[0]
-        self._a, self._ref, self._fn = a, C.byref(a), lib().nnz_qk_norm_rope_paged
+        self._a, self._fn = a, lib().nnz_qk_norm_rope_paged
 
     def __call__(self, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        a, kv, n = self._a, self.kv, qkv.shape[0]
+        a, kv, n = _own(self._a), self.kv, qkv.shape[0]
         if out is None:
             out = torch.empty(n, self._qd, dtype=kv.dtype, device=kv.device)
         a.qkv_stride = _rows(qkv, n, self._width, kv, "qkv")
@@ -128,7 +135,7 @@ class QKNormRope:
         a.positions = _index(positions, torch.int32, (n,), kv.device, "positions")
         a.slots = _index(slots, torch.int64, (n,), kv.device, "slots")
         a.qkv, a.q_out, a.tokens = qkv.data_ptr(), out.data_ptr(), n
-        rc = self._fn(kv._ref, self._ref, _stream(kv.index))
+        rc = self._fn(kv._ref, C.byref(a), _stream(kv.index))
         if rc:
             check(rc)
         return out
@@ -142,7 +149,8 @@ class PagedAttention:
     s has rows ``q_start[s]:q_start[s + 1]`` and ``kv_len[s]`` keys, its new
     tokens' included, on the pages ``page_table[s]`` (negative: absent).
     ``max_new`` is a host-known upper bound of one sequence's new tokens.  The
-    object owns the workspace, so its calls belong on one stream at a time."""
+    object owns the workspace, so its calls belong on one stream at a time;
+    threads may share it."""
 
     def __init__(self, kv: PagedKV, num_query_heads: int, scale: float | None = None):
         self.kv, self.num_query_heads = kv, num_query_heads
@@ -153,11 +161,11 @@ class PagedAttention:
         a = capi.NnzPagedAttnArgs()
         a.num_query_heads, a.scale = num_query_heads, 0.0 if scale is None else scale
         a.workspace, a.workspace_bytes = self._ws.data_ptr(), n
-        self._a, self._ref, self._fn = a, C.byref(a), lib().nnz_paged_attn
+        self._a, self._fn, self._lock = a, lib().nnz_paged_attn, threading.Lock()
 
     def __call__(self, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, max_new: int,
                  out: torch.Tensor | None = None) -> torch.Tensor:
-        a, kv, n, seqs = self._a, self.kv, q.shape[0], kv_len.shape[0]
+        a, kv, n, seqs = _own(self._a), self.kv, q.shape[0], kv_len.shape[0]
         if out is None:   # rows outside every sequence are not written
             out = torch.zeros(n, self._qd, dtype=kv.dtype, device=kv.device)
         a.q_stride = _rows(q, n, self._qd, kv, "q")
@@ -167,7 +175,8 @@ class PagedAttention:
         a.page_table = _index(page_table, torch.int32, (seqs, page_table.shape[1]), kv.device, "page_table")
         a.table_stride = page_table.shape[1]
         a.q, a.out, a.tokens, a.num_seqs, a.max_new = q.data_ptr(), out.data_ptr(), n, seqs, max_new
-        rc = self._fn(kv._ref, self._ref, _stream(kv.index))
+        with self._lock:      # a call's kernels hand their parts on through the workspace: no other call's launch between them
+            rc = self._fn(kv._ref, C.byref(a), _stream(kv.index))
         if rc:
             check(rc)
         return out
