@@ -10,9 +10,9 @@ nnmetal/src/transformer.zig:648-700, and prefills token by token, :4032-4068):
 * :func:`token_logprobs`: log probabilities of given tokens, entropy and the
   most probable alternatives, from one read of the logits.
 
-Every call is asynchronous on torch's current stream of the tensors' device,
-which has to be the current one; errors found on the device (a page, slot or
-token out of range) are reported by :func:`stream_check`.  Tensors that a call
+Every call is asynchronous on torch's current stream of the tensors' device
+(which need not be the current device); errors found on the device (a page,
+slot or token out of range) are reported by :func:`stream_check`.  Tensors that a call
 uses must stay alive until its stream has run it, as with any torch operation
 (``record_stream`` them if they were allocated on another stream).  The math
 runs in the CUDA library; this module checks and marshals arguments.
@@ -39,6 +39,11 @@ def _stream(device: int | None = None) -> int:
     if _raw_stream is not None and device is not None:
         return _raw_stream(device)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# The library launches on the current device, and the default stream's handle is 0 on every device: a call whose
+# tensors are elsewhere makes their device the current one first.
+_current_device, _device = torch.cuda.current_device, torch.cuda.device
 
 
 def _need(ok: bool, what: str) -> None:
@@ -98,8 +103,9 @@ def rope_table(theta: float, head_dim: int, positions: int, device="cuda") -> to
     """float32 ``[positions][head_dim / 2][2]`` (cos, sin) of position times
     theta^(-2 i / head_dim), evaluated in double precision."""
     _need(positions > 0, "rope_table: positions")
-    t = torch.empty(positions, head_dim // 2, 2, dtype=torch.float32, device=device)
-    check(lib().nnz_rope_table(theta, head_dim, positions, t.data_ptr(), _stream()))
+    with _device(device):
+        t = torch.empty(positions, head_dim // 2, 2, dtype=torch.float32, device=device)
+        check(lib().nnz_rope_table(theta, head_dim, positions, t.data_ptr(), _stream(t.device.index)))
     return t
 
 
@@ -127,6 +133,9 @@ class QKNormRope:
         self._a, self._fn = a, lib().nnz_qk_norm_rope_paged
 
     def __call__(self, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        if _current_device() != self.kv.index:
+            with _device(self.kv.index):
+                return self(qkv, positions, slots, out)
         a, kv, n = _own(self._a), self.kv, qkv.shape[0]
         if out is None:
             out = torch.empty(n, self._qd, dtype=kv.dtype, device=kv.device)
@@ -155,7 +164,8 @@ class PagedAttention:
     def __init__(self, kv: PagedKV, num_query_heads: int, scale: float | None = None):
         self.kv, self.num_query_heads = kv, num_query_heads
         self._qd = num_query_heads * kv.head_dim
-        n = lib().nnz_paged_attn_workspace(kv._ref, num_query_heads)
+        with _device(kv.index):      # the workspace follows the device's number of SMs
+            n = lib().nnz_paged_attn_workspace(kv._ref, num_query_heads)
         _need(n > 0, f"paged attention over these pages does not take {num_query_heads} query heads")
         self._ws = torch.zeros(n, dtype=torch.uint8, device=kv.device)
         a = capi.NnzPagedAttnArgs()
@@ -165,6 +175,9 @@ class PagedAttention:
 
     def __call__(self, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, max_new: int,
                  out: torch.Tensor | None = None) -> torch.Tensor:
+        if _current_device() != self.kv.index:
+            with _device(self.kv.index):
+                return self(q, page_table, q_start, kv_len, max_new, out)
         a, kv, n, seqs = _own(self._a), self.kv, q.shape[0], kv_len.shape[0]
         if out is None:   # rows outside every sequence are not written
             out = torch.zeros(n, self._qd, dtype=kv.dtype, device=kv.device)
@@ -223,6 +236,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda:
         raise ValueError(f"logits: expected float32, float16 or bfloat16 [rows][n] on a CUDA device, got {logits.dtype} "
                          f"{tuple(logits.shape)} on {logits.device}")
+    if _current_device() != logits.device.index:
+        with _device(logits.device.index):
+            return token_logprobs(logits, tokens, top_k)
     rows, n = logits.shape
     _need(n > 0 and (n == 1 or logits.stride(1) == 1), "logits: adjacent elements, at least one")
     _need(0 <= top_k <= 32, "top_k must be 0 .. 32")
@@ -248,6 +264,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     return TokenLogprobs(f, None if tokens is None else tuple(tokens.shape), rows, m, top_k, ids)
 
 
-def stream_check() -> None:
-    """Waits for the current stream and raises what its kernels found wrong (``nnz_stream_check``)."""
-    check(lib().nnz_stream_check(_stream()))
+def stream_check(device=None) -> None:
+    """Waits for the current stream of ``device`` (None: the current device) and raises what its kernels found wrong
+    (``nnz_stream_check``)."""
+    with _device(device):
+        check(lib().nnz_stream_check(_stream(_current_device())))

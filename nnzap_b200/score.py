@@ -76,7 +76,8 @@ class PagedModel:
     def __init__(self, config: TransformerConfig, tensors, num_pages: int, page_size: int = 16, device="cuda"):
         """``tensors``: (checkpoint name, array) pairs as ``Model.load_weights`` takes them."""
         c, t = config, dict(tensors)
-        self.config, self.device = c, torch.device(device, torch.cuda.current_device()) if device == "cuda" else torch.device(device)
+        device = torch.device(device)
+        self.config, self.device = c, torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
         H, hd = c.hidden_size, c.head_dim
 
         def q(*names):
@@ -110,6 +111,9 @@ class PagedModel:
 
     def step(self, tokens, positions, slots, page_table, q_start, kv_len, max_new: int) -> torch.Tensor:
         """float32 logits [len(tokens)][vocab]; device tensors as the operators take them."""
+        if paged._current_device() != self.device.index:      # the GEMMs run on the current device
+            with paged._device(self.device.index):
+                return self.step(tokens, positions, slots, page_table, q_start, kv_len, max_new)
         x = self.embed.rows(tokens.long())
         for L in self.layers:
             qkv = L["qkv"].gemm(self._norm(x, L["attn_norm"]))
@@ -173,7 +177,7 @@ def score(model: PagedModel, prompts, new_tokens: int = 0, budget: int = 512, to
                                 torch.tensor([done[i] + n for i, n in take], **i32), max(n for _, n in take))
             r = paged.token_logprobs(logits, torch.tensor(nxt, **i32), top_k=top_k)
             lp, ent, ids, top = (x.cpu().tolist() for x in (r.logprob, r.entropy, r.top_ids, r.top_logprobs))
-            paged.stream_check()
+            paged.stream_check(dev)
             row = 0
             for i, n in take:
                 s = seqs[i]

@@ -13,10 +13,36 @@ def _lib(built_lib):
     yield
 
 
+class Devices:
+    """Two devices that are not there: which one is current."""
+    current = 0
+
+    def guard(self, device):
+        class Guard:
+            def __enter__(g):
+                g.back, want = self.current, torch.device(device) if isinstance(device, str) else device
+                want = getattr(want, "index", want)
+                self.current = g.back if want is None else want
+
+            def __exit__(g, *exc):
+                self.current = g.back
+        return Guard()
+
+
 @pytest.fixture
-def paged(monkeypatch):
+def devices(monkeypatch):
     from nnzap_b200 import paged
-    monkeypatch.setattr(paged, "_stream", lambda device=None: 0)
+    d = Devices()
+    # (raising=False: also where the module does not look at the device)
+    monkeypatch.setattr(paged, "_current_device", lambda: d.current, raising=False)
+    monkeypatch.setattr(paged, "_device", d.guard, raising=False)
+    monkeypatch.setattr(paged, "_stream", lambda device=None: 100 + (d.current if device is None else device))
+    return d
+
+
+@pytest.fixture
+def paged(devices):
+    from nnzap_b200 import paged
     return paged
 
 
@@ -93,3 +119,80 @@ def test_two_threads_share_an_operator(paged, which):
     assert seen == {n: (v[0].data_ptr(), len(v[0])) for n, v in x.items()}
     if which == "attention":
         assert max(overlap) == 0
+
+
+# ---- devices ---------------------------------------------------------------------
+def test_operators_run_on_the_device_of_their_tensors(paged, devices):
+    """Called while another device is current, an operator launches on its
+    tensors' device and that device's stream, and leaves the current one as it was."""
+    devices.current = 1
+    for op, inputs in ((norm_rope(paged), norm_rope_inputs), (paged.PagedAttention(host_kv(paged), 4), attn_inputs)):
+        seen = []
+        op._fn = lambda kv, ref, stream: seen.append((devices.current, stream)) or 0
+        op(*inputs(3))
+        assert seen == [(0, 100)] and devices.current == 1
+
+
+class Lib:
+    """The library's functions, which note the current device and their last argument."""
+    def __init__(self, devices, result=0):
+        self.devices, self.result, self.calls = devices, result, []
+
+    def __getattr__(self, name):
+        def f(*args):
+            self.calls.append((name, self.devices.current, args[-1]))
+            return self.result
+        return f
+
+
+def test_workspace_is_sized_on_the_pools_device(paged, devices, monkeypatch):
+    devices.current, lib = 1, Lib(devices, 512)
+    monkeypatch.setattr(paged, "lib", lambda: lib)
+    paged.PagedAttention(host_kv(paged), 4)
+    assert [c[:2] for c in lib.calls if c[0] == "nnz_paged_attn_workspace"] == [("nnz_paged_attn_workspace", 0)]
+
+
+def test_rope_table_and_checks_follow_the_device_argument(paged, devices, monkeypatch):
+    lib, empty = Lib(devices), torch.empty
+
+    class OnOne(torch.Tensor):
+        device = torch.device("cuda", 1)
+    monkeypatch.setattr(paged, "lib", lambda: lib)
+    monkeypatch.setattr(paged.torch, "empty", lambda *shape, dtype, device: empty(*shape, dtype=dtype).as_subclass(OnOne))
+    paged.rope_table(1e4, 64, 8, device="cuda:1")
+    paged.stream_check("cuda:1")
+    paged.stream_check()
+    assert lib.calls == [("nnz_rope_table", 1, 101), ("nnz_stream_check", 1, 101), ("nnz_stream_check", 0, 100)]
+    assert devices.current == 0
+
+
+def test_token_logprobs_on_another_device(paged, devices, monkeypatch):
+    lib, empty = Lib(devices), torch.empty
+
+    class OnOne(torch.Tensor):
+        device, is_cuda = torch.device("cuda", 1), True
+    monkeypatch.setattr(paged, "lib", lambda: lib)
+    monkeypatch.setattr(paged.torch, "empty", lambda *shape, dtype, device: empty(*shape, dtype=dtype))
+    paged.token_logprobs(torch.zeros(2, 8).as_subclass(OnOne), top_k=2)
+    assert lib.calls == [("nnz_token_logprobs", 1, 101)] and devices.current == 0
+
+
+def test_a_models_step_runs_on_its_device(paged, devices):
+    from nnzap_b200.score import PagedModel
+    seen = []
+
+    class Weights:
+        M = 10
+
+        def rows(self, ids):
+            seen.append(devices.current)
+            return torch.zeros(len(ids), 4)
+
+        def gemm(self, x, out=None):
+            seen.append(devices.current)
+            return out
+    m = object.__new__(PagedModel)
+    m.device, m.layers, m.embed, m.lm_head, m.final_norm = torch.device("cuda", 1), [], Weights(), Weights(), torch.ones(4)
+    m.config = type("Config", (), {"eps": 1e-6})
+    m.step(torch.zeros(3, dtype=torch.int32), None, None, None, None, None, 1)
+    assert seen == [1, 1] and devices.current == 0
