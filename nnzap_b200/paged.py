@@ -44,6 +44,7 @@ def _stream(device: int | None = None) -> int:
 # The library launches on the current device, and the default stream's handle is 0 on every device: a call whose
 # tensors are elsewhere makes their device the current one first.
 _current_device, _device = torch.cuda.current_device, torch.cuda.device
+_current_stream, _capturing = torch.cuda.current_stream, torch.cuda.is_current_stream_capturing
 
 
 def _need(ok: bool, what: str) -> None:
@@ -150,6 +151,28 @@ class QKNormRope:
         return out
 
 
+class _Workspace:
+    """Memory that a call's kernels hand their parts on through, and which every call leaves as it found it: one call
+    uses it at a time.  A call on another stream than the last one's waits for that one on the device (or, the first
+    call, for the zeros), and the allocator learns of the stream.  Inside a graph capture it does neither: the order
+    of a graph's launches is that of who replays it."""
+
+    def __init__(self, nbytes: int, device: torch.device):
+        self.lock = threading.Lock()
+        self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        self._last = _current_stream(device)
+        self._handle = self._last.cuda_stream
+
+    def on(self, handle: int) -> None:
+        """The next use is on the current stream, whose handle this is (under the lock)."""
+        if handle == self._handle or _capturing():
+            return
+        now = _current_stream(self.buf.device)
+        now.wait_stream(self._last)
+        self.buf.record_stream(now)
+        self._last, self._handle = now, handle
+
+
 class PagedAttention:
     """``op(q, page_table, q_start, kv_len, max_new)``: causal attention of
     every sequence's new tokens over its pages.
@@ -158,20 +181,20 @@ class PagedAttention:
     s has rows ``q_start[s]:q_start[s + 1]`` and ``kv_len[s]`` keys, its new
     tokens' included, on the pages ``page_table[s]`` (negative: absent).
     ``max_new`` is a host-known upper bound of one sequence's new tokens.  The
-    object owns the workspace, so its calls belong on one stream at a time;
-    threads may share it."""
+    object owns a workspace that one call uses at a time: threads may share it,
+    and a call on another stream waits for the one before."""
 
     def __init__(self, kv: PagedKV, num_query_heads: int, scale: float | None = None):
         self.kv, self.num_query_heads = kv, num_query_heads
         self._qd = num_query_heads * kv.head_dim
         with _device(kv.index):      # the workspace follows the device's number of SMs
             n = lib().nnz_paged_attn_workspace(kv._ref, num_query_heads)
-        _need(n > 0, f"paged attention over these pages does not take {num_query_heads} query heads")
-        self._ws = torch.zeros(n, dtype=torch.uint8, device=kv.device)
+            _need(n > 0, f"paged attention over these pages does not take {num_query_heads} query heads")
+            self._ws = _Workspace(n, kv.device)
         a = capi.NnzPagedAttnArgs()
         a.num_query_heads, a.scale = num_query_heads, 0.0 if scale is None else scale
-        a.workspace, a.workspace_bytes = self._ws.data_ptr(), n
-        self._a, self._fn, self._lock = a, lib().nnz_paged_attn, threading.Lock()
+        a.workspace, a.workspace_bytes = self._ws.buf.data_ptr(), n
+        self._a, self._fn = a, lib().nnz_paged_attn
 
     def __call__(self, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, max_new: int,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -188,8 +211,10 @@ class PagedAttention:
         a.page_table = _index(page_table, torch.int32, (seqs, page_table.shape[1]), kv.device, "page_table")
         a.table_stride = page_table.shape[1]
         a.q, a.out, a.tokens, a.num_seqs, a.max_new = q.data_ptr(), out.data_ptr(), n, seqs, max_new
-        with self._lock:      # a call's kernels hand their parts on through the workspace: no other call's launch between them
-            rc = self._fn(kv._ref, C.byref(a), _stream(kv.index))
+        ws, stream = self._ws, _stream(kv.index)
+        with ws.lock:         # no other call's launch between the kernels of this one
+            ws.on(stream)
+            rc = self._fn(kv._ref, C.byref(a), stream)
         if rc:
             check(rc)
         return out

@@ -367,6 +367,31 @@ def test_paged_ops_on_another_stream():
     assert torch.equal(lp.top_ids, P().token_logprobs(got.float(), top_k=3).top_ids)
 
 
+@pytest.mark.parametrize("lens", [[(1, 9000), (1, 3)], [(200, 4000)]])
+def test_paged_attention_workspace_made_on_another_stream(lens):
+    """An operator whose workspace is still to be zeroed, behind other work on
+    the stream it was made on and in memory that held ones, called at once on
+    two more streams: split tasks meet in the workspace."""
+    c = attn_case(91, lens, 8, 4, 128, 16, "f16", "head")
+    want = check_attn(c)
+    kv = P().PagedKV(c["k"], c["v"])
+    n = P().PagedAttention(kv, 8)._ws.buf.numel()
+    made, used = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(made):
+        torch.full((n,), 255, dtype=torch.uint8, device="cuda")       # the next block of this size and stream
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(20):
+            big = big @ big * 1e-3
+        op = P().PagedAttention(kv, 8)
+    with torch.cuda.stream(used):
+        first = op(c["q"], c["table"], c["q_start"], c["kv_len"], c["max_new"])
+    second = op(c["q"], c["table"], c["q_start"], c["kv_len"], c["max_new"])
+    torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(second, want)
+    P().stream_check()
+
+
 def test_paged_ops_in_a_cuda_graph():
     """Lengths, tables and tokens are read on the device: one captured step serves every later one."""
     c = attn_case(71, [(1, 1), (1, 1), (1, 1)], 8, 4, 128, 16, "f16", "head", poison=False)

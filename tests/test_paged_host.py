@@ -13,6 +13,15 @@ def _lib(built_lib):
     yield
 
 
+class Stream:
+    """A stream that notes what it waits for."""
+    def __init__(self, handle, log):
+        self.cuda_stream, self.log = handle, log
+
+    def wait_stream(self, other):
+        self.log.append(("wait", self.cuda_stream, other.cuda_stream))
+
+
 class Devices:
     """Two devices that are not there: which one is current."""
     current = 0
@@ -37,6 +46,8 @@ def devices(monkeypatch):
     monkeypatch.setattr(paged, "_current_device", lambda: d.current, raising=False)
     monkeypatch.setattr(paged, "_device", d.guard, raising=False)
     monkeypatch.setattr(paged, "_stream", lambda device=None: 100 + (d.current if device is None else device))
+    monkeypatch.setattr(paged, "_current_stream", lambda device=None: Stream(100 + d.current, []), raising=False)
+    monkeypatch.setattr(paged, "_capturing", lambda: False, raising=False)
     return d
 
 
@@ -196,3 +207,25 @@ def test_a_models_step_runs_on_its_device(paged, devices):
     m.config = type("Config", (), {"eps": 1e-6})
     m.step(torch.zeros(3, dtype=torch.int32), None, None, None, None, None, 1)
     assert seen == [1, 1] and devices.current == 0
+
+
+# ---- streams ---------------------------------------------------------------------
+def test_a_workspace_follows_its_calls_from_stream_to_stream(paged, monkeypatch):
+    """Zeroed on stream 1, used on 2, 2, 3 and 3 (in a graph's capture on 4
+    between them): a stream that is not the last use's waits for it, before the
+    launch, and the memory is marked as used there."""
+    log, zeros, now = [], torch.zeros, [1]
+
+    class Buffer(torch.Tensor):
+        def record_stream(self, stream):
+            log.append(("record", stream.cuda_stream))
+    monkeypatch.setattr(paged.torch, "zeros", lambda *a, **k: zeros(*a, **k).as_subclass(Buffer))
+    monkeypatch.setattr(paged, "_stream", lambda device=None: now[0])
+    monkeypatch.setattr(paged, "_current_stream", lambda device=None: Stream(now[0], log), raising=False)
+    monkeypatch.setattr(paged, "_capturing", lambda: now[0] == 4, raising=False)
+    op = paged.PagedAttention(host_kv(paged), 4)
+    op._fn = lambda kv, ref, stream: log.append(("launch", stream)) or 0
+    for now[0] in (2, 2, 4, 3, 3):
+        op(*attn_inputs(3))
+    assert log == [("wait", 2, 1), ("record", 2), ("launch", 2), ("launch", 2), ("launch", 4),
+                   ("wait", 3, 2), ("record", 3), ("launch", 3), ("launch", 3)]
