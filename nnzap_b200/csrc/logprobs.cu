@@ -30,12 +30,12 @@
 #include <math.h>
 
 #include <algorithm>
-#include <atomic>
 #include <string>
 #include <type_traits>
 
 #include "../../include/nnz_b200.h"
 #include "common.cuh"
+#include "device_cache.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -447,31 +447,38 @@ __global__ void __launch_bounds__(kLpThreads, sizeof(T) == 4 ? 4 : 3) logprobs_k
 
 template <typename T, bool TOP>
 cudaError_t logprobs_go(const LpArgs& a, int sms, cudaStream_t st) {
-  static std::atomic<bool> ready{false};
-  if (!ready.load(std::memory_order_relaxed)) {
-    const cudaError_t e = cudaFuncSetAttribute((const void*)&logprobs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    ready.store(true, std::memory_order_relaxed);
-  }
+  const auto fn = &logprobs_kernel<T, TOP>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  // The largest cluster: 16 CTAs where the device takes them, else the 8 that every one does.
+  static PerDevice largest;
+  const uint32_t most = (uint32_t)largest.get([&] {
+    int n = 0;
+    at[0].val.clusterDim.x = kLpMaxCluster;
+    cfg.gridDim = dim3(kLpMaxCluster);
+    if (cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&n, fn, &cfg) == cudaSuccess && n > 0)
+      return (int)kLpMaxCluster;
+    cudaGetLastError();
+    return 8;
+  });
   // CTAs per row: as many as keep the row's CTAs within two per SM, each with
   // a step of work or more (a CTA's sorts and merges cost it 3 - 4 us: 64 rows
   // of 151669 bf16 take 14.5 us with 4, 17.8 with 8, 16.9 with 2; 512 rows of
   // 151936 f32 60.9 us with 1, 69.8 with 2; one row 8.3 us with 16, 11.2 with 4)
   const uint64_t bytes = (uint64_t)a.n * sizeof(T);
   uint32_t C = 1;
-  while (C < kLpMaxCluster && (uint64_t)a.rows * 2 * C <= (uint64_t)sms * 2 && bytes / (2 * C) >= kLpThreads * kLpVec * 16) C *= 2;
+  while (C < most && (uint64_t)a.rows * 2 * C <= (uint64_t)sms * 2 && bytes / (2 * C) >= kLpThreads * kLpVec * 16) C *= 2;
   if ((uint64_t)a.rows * C > 0x7FFFFFFFull) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.rows * C);
-  cfg.blockDim = dim3(kLpThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, &logprobs_kernel<T, TOP>, a);
+  return cudaLaunchKernelEx(&cfg, fn, a);
 }
 
 template <typename T>

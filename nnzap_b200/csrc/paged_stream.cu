@@ -642,12 +642,11 @@ __global__ void __launch_bounds__(kStWarps * 32, CL ? 1 : 0) paged_stream_kernel
 //   4 x 4      8.2   11.5   16.4    32.8
 //   even cut  11.5   12.8   20.9    36.1
 template <typename K>
-void stream_clusters(K* fn, StArgs& t, cudaLaunchConfig_t cfg, std::atomic<int> (&fits)[9]) {
+void stream_clusters(K* fn, StArgs& t, cudaLaunchConfig_t cfg, PerDevice (&fits)[9]) {
   const uint64_t keys = (uint64_t)t.a.table_stride * t.a.kv.page_size;
   for (uint32_t C = keys <= 4096 ? 8 : 4; C >= 4; C /= 2) {
-    // clusters of C that the device runs at once (asked once)
-    int n = fits[C].load(std::memory_order_relaxed);
-    if (n == 0) {
+    // clusters of C that the device runs at once (asked once; -1: none)
+    const int n = fits[C].get([&] {
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim.x = C;
@@ -655,12 +654,11 @@ void stream_clusters(K* fn, StArgs& t, cudaLaunchConfig_t cfg, std::atomic<int> 
       cfg.gridDim = dim3(C);
       cfg.attrs = at;
       cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n <= 0) {
-        cudaGetLastError();
-        n = -1;
-      }
-      fits[C].store(n, std::memory_order_relaxed);
-    }
+      int most = 0;
+      if (cudaOccupancyMaxActiveClusters(&most, fn, &cfg) == cudaSuccess && most > 0) return most;
+      cudaGetLastError();
+      return -1;
+    });
     const uint32_t n_kv = t.a.kv.n_kv;
     if (n >= (int)n_kv) {
       t.cluster = C;
@@ -673,7 +671,7 @@ void stream_clusters(K* fn, StArgs& t, cudaLaunchConfig_t cfg, std::atomic<int> 
 template <typename T, int HD, bool ROWS8>
 cudaError_t stream_go(StArgs t, cudaStream_t st) {
   static std::atomic<uint64_t> ready[2] = {};
-  static std::atomic<int> fits[9];
+  static PerDevice fits[9];
   const auto fn = &paged_stream_kernel<T, HD, ROWS8, false>;
   const auto fc = &paged_stream_kernel<T, HD, ROWS8, true>;
   cudaLaunchConfig_t cfg = {};

@@ -4,8 +4,7 @@
 #pragma once
 #include <cuda.h>
 
-#include <atomic>
-
+#include "device_cache.cuh"
 #include "paged.cuh"
 
 namespace nnz {
@@ -38,17 +37,5 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tm, in
 bool paged_tensor_map(CUtensorMap* tm, const PagedPool& kv, const void* base, int hd, uint32_t keys);
 // Rows of q as [token][head][d]: boxes of `heads` heads x `tokens` tokens x 64 dims.
 bool paged_q_map(CUtensorMap* tm, const PagedAttnArgs& a, int hd, uint32_t heads, uint32_t tokens);
-
-// Raises a kernel's dynamic shared-memory limit, once per device.
-inline cudaError_t raise_smem(const void* fn, int bytes, std::atomic<uint64_t>& ready) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
-  return e;
-}
 
 }  // namespace nnz
