@@ -32,6 +32,7 @@
 #include <cuda_runtime.h>
 
 #include "attn.cuh"
+#include "device_cache.cuh"
 #include "gemm.cuh"
 #include "rope_dev.cuh"
 #include "umma.cuh"
@@ -395,15 +396,12 @@ cudaError_t attn_pf_umma_launch(const AttnArgs& a, int pdl, cudaStream_t st) {
       return cudaErrorInvalidValue;
   }
   const uint32_t G = a.n_q / a.n_kv, pb = 128 / G;
-  static bool attr[3] = {false, false, false};
+  static std::atomic<uint64_t> ready[3] = {};
   const int gi = G == 1 ? 0 : G == 2 ? 1 : 2;
   const void* fn = G == 1 ? (const void*)&attn_pf_umma_kernel<1>
                  : G == 2 ? (const void*)&attn_pf_umma_kernel<2> : (const void*)&attn_pf_umma_kernel<4>;
-  if (!attr[gi]) {
-    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPfSmem);
-    if (e != cudaSuccess) return e;
-    attr[gi] = true;
-  }
+  const cudaError_t e = raise_smem(fn, (int)kPfSmem, ready[gi]);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.n_kv, (a.rows + pb - 1) / pb);
   cfg.blockDim = dim3(512);

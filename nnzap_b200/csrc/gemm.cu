@@ -2,6 +2,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "device_cache.cuh"
 #include "gemm.cuh"
 #include "umma.cuh"
 
@@ -838,13 +839,10 @@ cudaError_t gemm_launch(const GemmArgs& a_in, const __half* x, cudaStream_t st) 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return cudaErrorInvalidValue;
     cfg.blockDim = dim3(kTsThreads);
-    static bool ats[2][3] = {};
-    auto gots = [&](auto kern, uint32_t smem, bool& attr) {
-      if (!attr) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return;
-        attr = true;
-      }
+    static std::atomic<uint64_t> ats[2][3] = {};
+    auto gots = [&](auto kern, uint32_t smem, std::atomic<uint64_t>& ready) {
+      e = raise_smem((const void*)kern, (int)smem, ready);
+      if (e != cudaSuccess) return;
       cfg.dynamicSmemBytes = smem;
       e = cudaLaunchKernelEx(&cfg, kern, tx, a);
     };
@@ -859,16 +857,13 @@ cudaError_t gemm_launch(const GemmArgs& a_in, const __half* x, cudaStream_t st) 
       else gots(&gemm_ts_kernel<FMT_Q4, 256>, TsShape<256>::kSmemBytes, ats[fi][ni]);
     }
   } else {
-  auto go = [&](auto kern, uint32_t smem, bool& attr) {
-    if (!attr) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return;
-      attr = true;
-    }
+  auto go = [&](auto kern, uint32_t smem, std::atomic<uint64_t>& ready) {
+    e = raise_smem((const void*)kern, (int)smem, ready);
+    if (e != cudaSuccess) return;
     cfg.dynamicSmemBytes = smem;
     e = cudaLaunchKernelEx(&cfg, kern, tm, a);
   };
-  static bool at[2][3] = {};
+  static std::atomic<uint64_t> at[2][3] = {};
   const int fi = a.fmt == FMT_Q1 ? 0 : 1, mi = mt == 4 ? 2 : mt - 1;
   if (a.fmt == FMT_Q1) {
     if (mt == 4) go(&gemm_kernel<FMT_Q1, 4>, GemmShape<4>::kSmemBytes, at[fi][mi]);

@@ -87,3 +87,17 @@ def test_chunks_on_every_device(runtime):
         lib.fake_use(dev)
         assert attention(lib, new=64) == 0, lib.fake_message()
     assert [x.device for x in lib.launches() if x.smem] == [0, 1, 0]
+
+
+def test_quantized_gemms_on_every_device(runtime):
+    class Args(C.Structure):
+        _fields_ = [("M", C.c_uint32), ("K", C.c_uint32), ("N", C.c_uint32), ("fmt", C.c_int), ("gs", C.c_int), ("bf16s", C.c_int),
+                    ("bf16r", C.c_int), *[(n, C.c_void_p) for n in ("w", "s", "b", "w2", "s2", "b2")], ("epi", C.c_int), ("acc", C.c_void_p),
+                    ("acc_floats", C.c_size_t), ("out", C.c_void_p), ("ldo", C.c_uint32), ("err", C.c_void_p), ("prof", C.c_int), ("pdl", C.c_int)]
+    lib = runtime("gemm")
+    a = Args(M=64, K=256, N=512, gs=128, w=0x1000, s=0x1000, out=0x1000, ldo=512)
+    launch = lib._ZN3nnz11gemm_launchERKNS_8GemmArgsEPK6__halfP11CUstream_st
+    for dev in (0, 1, 0):
+        lib.fake_use(dev)
+        assert launch(C.byref(a), C.c_void_p(0x1000), None) == 0
+    assert [x.device for x in lib.launches()] == [0, 1, 0]
