@@ -12,12 +12,24 @@
 //   O += P V            tcgen05.mma, P from TMEM, V as stored (MN-major B)
 // so while one row tile's softmax runs, the tensor cores work for the other.
 // m need not be the row's maximum: any m gives the same quotient as long as no
-// P overflows or leaves the 16-bit type's normal range.  It starts at 0, a
-// unit's P is computed with the m that the row has, in one pass over S without
-// looking for a maximum, and only if the sum of 64 P turns out to be 2^15 or
-// more (or, among the first keys that a row sees, less than 1/4) does the row
-// take its maximum for m, rescale O and compute the unit again, which after
-// the first units is rare.  Sums are f32.
+// P overflows and the largest does not fall so low that the others are lost
+// below the 16-bit type's range.  A unit's P is computed with the m that the row
+// has, in one pass over S without looking for a maximum, and only if the sum of
+// 64 P turns out to be 2^15 or more (or, among the first keys that a row sees,
+// less than kLeast) does the row take a new m, from its maximum, rescale O and
+// compute the unit again, which after the first units is rare.
+// f16: m starts at -4 and is set 4 below the maximum, so P has 4 bits more
+// towards zero, and 64 P that sum to 64 have one of 1 or more: what P loses below
+// 2^-14 is 2^-25 of the row's largest a key.  bf16 has f32's range: m starts at 0,
+// is set to the maximum, and a sum of 1/4 will do.  (f16 with m from 0 and a sum
+// of 64 took 37.4 us for 512 tokens, whose units were often computed twice;
+// from -4 36.5.)
+// Sums are f32, and of the P before they are rounded.  P enters the second
+// product in the pool's type because the tensor cores multiply 16-bit operands
+// at twice the rate of wider ones: an error of half a unit in its last place in
+// every weight, as much again as the result's own rounding at the most.
+// (The tensor cores add a product to O with about 2^-25 of O's size: tens of
+// thousands of keys that weigh less than that each are lost, in any type.)
 //
 // Roles: warps 0-7 and 8-15 softmax and epilogue of row tiles 0 and 1 (TMEM lane
 // = row; warps 0-3 of a tile have keys 0-63 of a unit and the lower half of the
@@ -65,7 +77,12 @@ constexpr uint32_t kHalfB = 128 * 128;           // 128 rows x 64 dims, swizzled
 constexpr int kSegs = 4;                          // segments in flight
 constexpr uint32_t kPartCost = 3;                 // what a part costs besides its units, in units (queries, epilogue, merge)
 constexpr int kPres = 8;                          // units whose page masks are kept
-constexpr float kMost = 32768.f, kLeast = 0.25f;  // sum of 64 P: below kMost (no P overflows), at first kLeast at least
+// sum of 64 P: below kMost (no P overflows), at first kLeast at least
+constexpr float kMost = 32768.f;
+template <typename T>
+constexpr float kLeast = T16<T>::kBf16 ? 0.25f : 64.f;
+template <typename T>
+constexpr float kLift = T16<T>::kBf16 ? 0.f : 4.f;         // m is this much below the maximum
 
 template <int HD>
 struct UmShape {
@@ -682,7 +699,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive1(v_ready + slot);
       };
-      float m = 0.f, l = 0.f;
+      float m = -kLift<T>, l = 0.f;
       bool fresh = true;              // no visible key among this thread's yet
       for (uint32_t i = 0; i < units; ++i) {
         wait(s_full + x, ns);
@@ -703,20 +720,20 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         float sum;
         for (bool first = true;; first = false) {
           sum = um_pass<T>(tS, t.sl2, m, w);
-          // Out of range: a sum of 2^15 or more (or NaN), or of less than 1/4
+          // Out of range: a sum of 2^15 or more (or NaN), or of less than kLeast
           // among the first keys that the row sees.
-          const bool off = live && (!(sum < kMost) || (fresh && sum < kLeast));
+          const bool off = live && (!(sum < kMost) || (fresh && sum < kLeast<T>));
           if (!first || !pair_any(bar, off)) break;
           // both threads of a row: the same m, from both halves' maxima
           const float top = um_top(tS) * t.sl2;
-          const float tp = fmaxf(pair_tell(bar, xr, half, 0, top), pair_tell(bar, xr, half, 1, top));
+          const float to = fmaxf(pair_tell(bar, xr, half, 0, top), pair_tell(bar, xr, half, 1, top)) - kLift<T>;
           const float say = (off ? 2.f : 0.f) + (fresh ? 1.f : 0.f);
           const float s0 = pair_tell(bar, xr, half, 0, say), s1 = pair_tell(bar, xr, half, 1, say);
           const bool all_fresh = s0 != 0.f && s0 != 2.f && s1 != 0.f && s1 != 2.f;
           float scale = 1.f;
-          if (live && (s0 >= 2.f || s1 >= 2.f) && (tp > m || (all_fresh && tp > -INFINITY))) {
-            if (!all_fresh) scale = ex2(m - tp);     // else there is nothing to rescale
-            m = tp;
+          if (live && (s0 >= 2.f || s1 >= 2.f) && (to > m || (all_fresh && to > -INFINITY))) {
+            if (!all_fresh) scale = ex2(m - to);     // else there is nothing to rescale
+            m = to;
             l *= scale;
           }
           if (i > 0) {

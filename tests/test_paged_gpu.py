@@ -293,6 +293,43 @@ def test_paged_attention_low_scores_and_nan_keys(n):
         assert torch.isnan(got[sees]).all() and torch.isfinite(got[~sees]).all(), key
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("first,rest", [(-7.9, -24.92), (-7.9, -22.6), (-5.9, -24.4), (-39.9, -56.92), (0.1, -16.92)])
+@pytest.mark.parametrize("zero_first", [True, False])
+def test_paged_attention_many_keys_far_below_the_first(dtype, first, rest, zero_first):
+    """128 keys of 2^first, then 32000 of 2^rest, which together weigh a few
+    thousandths of them: a sequence for every SM, all alike, so that one CTA
+    has all keys of its rows.  With values of 0 for the first keys only the
+    others' probabilities are seen, within the bound that holds everywhere.
+    With values near 1 for all, the products of the others meet a sum 2^24 times
+    their size, of which the tensor cores keep 2^-25: that much more a key."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n, G, hd, page, L = 16, 16, 64, 64, 128 + 32000
+    dt, ln2 = DT[dtype], float(np.log(2))
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.zeros(L // page, 1, page, hd, device="cuda")
+    k[..., 0] = rest * ln2
+    k[:2, ..., 0] = first * ln2
+    v = 1 + 0.01 * torch.randn(L // page, 1, page, hd, device="cuda", generator=g)
+    if zero_first:
+        v[:2] = 0
+    k, v = k.to(dt), v.to(dt)
+    q = torch.zeros(n, G, hd, device="cuda", dtype=dt)
+    q[..., 0] = 8.0                                          # times 1 / 8: the score is the key's first element
+    q = q.view(n, G * hd)
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda")[None]
+    want, tol = R.attention(q, k, v, table, [0, n], [L], hd ** -0.5, q)
+    if not zero_first:
+        tol = tol + L * 2.0 ** -25 * want.abs()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    got = P().PagedAttention(P().PagedKV(k, v), G)(q.repeat(sms, 1), table.repeat(sms, 1), torch.arange(sms + 1, **i32) * n,
+                                                   torch.full((sms,), L, **i32), n)
+    P().stream_check()
+    got = got.view(sms, n, G, hd)
+    assert torch.equal(got, got[:1].expand_as(got))
+    within(got[0], want, tol, f"{first} {rest}")
+
+
 def test_paged_attention_far_pages():
     """Element offsets beyond 32 bits: the last pages of a pool of 2^32 + elements."""
     page, n_kv, hd = 16, 8, 128
