@@ -57,7 +57,12 @@ class _Weights:
         return out
 
     def rows(self, ids: torch.Tensor) -> torch.Tensor:
-        """Dequantized rows, float32 [len(ids)][K] (the embedding lookup)."""
+        """Dequantized rows, float32 [len(ids)][K] (the embedding lookup); NaN for an id that is none (indexing with it
+        would stop the device)."""
+        none = (ids < 0) | (ids >= self.M)
+        return torch.where(none[:, None], torch.nan, self._rows(torch.where(none, 0, ids)))
+
+    def _rows(self, ids: torch.Tensor) -> torch.Tensor:
         g = self.s.view(self.M, self.K // self.gs)[ids].view(torch.bfloat16 if self.scale_dtype else torch.float16).float()
         if self.fmt == capi.NNZ_Q1:
             bits = self.w.view(self.M, self.K // 8)[ids]
@@ -142,7 +147,13 @@ def score(model: PagedModel, prompts, new_tokens: int = 0, budget: int = 512, to
     taken from the sequences in turn."""
     dev, page = model.device, model.page_size
     seqs = [Scored([int(t) for t in p], [], [], [], []) for p in prompts]
-    assert all(s.tokens for s in seqs) and budget > 0 and top_k >= 1
+    cfg = model.config
+    paged._need(new_tokens >= 0 and budget > 0 and 1 <= top_k <= 32, "score: new_tokens >= 0, budget > 0, top_k 1 .. 32")
+    for i, s in enumerate(seqs):
+        paged._need(len(s.tokens) > 0, f"prompt {i} is empty")
+        paged._need(all(0 <= t < cfg.vocab_size for t in s.tokens), f"prompt {i} has a token outside 0 .. {cfg.vocab_size - 1}")
+        paged._need(len(s.tokens) + new_tokens - 1 <= cfg.max_context_length,
+                    f"prompt {i}: {len(s.tokens)} and {new_tokens} new tokens do not fit a context of {cfg.max_context_length}")
     goal = [len(s.tokens) + new_tokens for s in seqs]
     pages = [[] for _ in seqs]
     done = [0] * len(seqs)                       # tokens whose keys are in the cache
