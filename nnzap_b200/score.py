@@ -195,6 +195,8 @@ def score(model: PagedModel, prompts, new_tokens: int = 0, budget: int = 512, to
                 for _ in range(n):
                     done[i] += 1
                     if nxt[row] < 0:               # generate: the most probable token
+                        if ids[row][0] < 0:
+                            raise RuntimeError(f"prompt {i}: no token to continue with after {len(s.tokens)} (no logit is a number, or nothing is allowed)")
                         s.tokens.append(ids[row][0])
                         lp[row] = top[row][0]
                     s.logprobs.append(lp[row])

@@ -70,3 +70,13 @@ def test_embedding_rows_of_ids_that_are_none(score, quant):
     rows = w.rows(torch.tensor([2, -1, M, 2 ** 31 - 1, 5]))
     assert torch.isnan(rows[1:4]).all() and torch.isfinite(rows[[0, 4]]).all()
     assert torch.equal(rows[[0, 4]], w.rows(torch.tensor([2, 5])))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), -float("inf")])
+def test_no_token_to_continue_with(score, bad):
+    m = Model(logits=lambda tokens: torch.where((tokens == 8)[:, None], bad, torch.zeros(len(tokens), VOCAB)))
+    out = score.score(m, [[8, 1]], new_tokens=1)                     # a row that nobody continues from is no error
+    assert out[0].tokens == [8, 1, 0]
+    with pytest.raises(RuntimeError, match="prompt 1"):
+        score.score(m, [[1, 2], [1, 8]], new_tokens=1)
+    assert sorted(m.free) == list(range(100))
