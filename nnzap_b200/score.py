@@ -144,7 +144,8 @@ class Scored:
 def score(model: PagedModel, prompts, new_tokens: int = 0, budget: int = 512, top_k: int = 5) -> list:
     """Log probability, entropy and alternatives of every prompt token, and of
     ``new_tokens`` greedily generated ones; at most ``budget`` tokens a step,
-    taken from the sequences in turn."""
+    taken from the sequences in turn as far as there are pages.  A sequence's
+    pages are free again when it is done; MemoryError if none can go on."""
     dev, page = model.device, model.page_size
     seqs = [Scored([int(t) for t in p], [], [], [], []) for p in prompts]
     cfg = model.config
@@ -160,22 +161,22 @@ def score(model: PagedModel, prompts, new_tokens: int = 0, budget: int = 512, to
     try:
         while True:
             # what each sequence contributes: tokens that are known and not yet run,
-            # and whose successor is still wanted
+            # whose successor is still wanted, and that pages can be had for
             left, take = budget, []
             for i, s in enumerate(seqs):
-                n = min(left, min(len(s.tokens), goal[i] - 1) - done[i])
+                n = min(left, min(len(s.tokens), goal[i] - 1) - done[i], (len(pages[i]) + len(model.free)) * page - done[i])
                 if n > 0:
                     take.append((i, n))
                     left -= n
+                    while len(pages[i]) * page < done[i] + n:
+                        pages[i].append(model.free.pop())
             if not take:
+                if any(d < g - 1 for d, g in zip(done, goal)):
+                    raise MemoryError("no free pages")
                 return seqs
             tok, pos, slot, nxt = [], [], [], []
             for i, n in take:
                 for p in range(done[i], done[i] + n):
-                    if p // page == len(pages[i]):
-                        if not model.free:
-                            raise MemoryError("no free pages")
-                        pages[i].append(model.free.pop())
                     tok.append(seqs[i].tokens[p])
                     pos.append(p)
                     slot.append(pages[i][p // page] * page + p % page)
@@ -204,6 +205,9 @@ def score(model: PagedModel, prompts, new_tokens: int = 0, budget: int = 512, to
                     s.top_ids.append(ids[row])
                     s.top_logprobs.append(top[row])
                     row += 1
+                if done[i] == goal[i] - 1:         # nothing of it is read again
+                    model.free.extend(pages[i])
+                    pages[i] = []
     finally:
         for p in pages:
             model.free.extend(p)

@@ -80,3 +80,19 @@ def test_no_token_to_continue_with(score, bad):
     with pytest.raises(RuntimeError, match="prompt 1"):
         score.score(m, [[1, 2], [1, 8]], new_tokens=1)
     assert sorted(m.free) == list(range(100))
+
+
+def test_pages_of_finished_sequences_serve_the_others(score):
+    """Five sequences of 5 to 9 tokens in a pool that holds the longest alone: what a large pool gives."""
+    prompts = [list(range(n)) for n in (7, 5, 6, 5, 7)]
+    want = score.score(Model(), prompts, new_tokens=2, budget=6)
+    m = Model(pages=3)
+    got = score.score(m, prompts, new_tokens=2, budget=6)
+    assert got == want and sorted(m.free) == [0, 1, 2]
+    m = Model()
+    score.score(m, prompts, new_tokens=2, budget=100)
+    assert m.used == 10                                       # all five in the first step, 2 pages each
+    m = Model(pages=2)
+    with pytest.raises(MemoryError):
+        score.score(m, prompts, new_tokens=3, budget=6)
+    assert sorted(m.free) == [0, 1]
