@@ -151,9 +151,9 @@ class QKNormRope:
         return out
 
 
-class _Workspace:
-    """Memory that a call's kernels hand their parts on through, and which every call leaves as it found it: one call
-    uses it at a time.  A call on another stream than the last one's waits for that one on the device (or, the first
+class Workspace:
+    """Memory that a :class:`PagedAttention` call's kernels hand their parts on through, and which every call leaves as
+    it found it: one call uses it at a time, of whichever operator has it.  A call on another stream than the last one's waits for that one on the device (or, the first
     call, for the zeros), and the allocator learns of the stream.  Inside a graph capture it does neither: the order
     of a graph's launches is that of who replays it."""
 
@@ -181,19 +181,23 @@ class PagedAttention:
     s has rows ``q_start[s]:q_start[s + 1]`` and ``kv_len[s]`` keys, its new
     tokens' included, on the pages ``page_table[s]`` (negative: absent).
     ``max_new`` is a host-known upper bound of one sequence's new tokens.  The
-    object owns a workspace that one call uses at a time: threads may share it,
-    and a call on another stream waits for the one before."""
+    object's ``workspace`` serves one call at a time: threads may share the
+    object, and a call on another stream waits for the one before.  Operators
+    whose calls follow one another (a model's layers) can have one workspace:
+    pass the first one's as ``workspace``."""
 
-    def __init__(self, kv: PagedKV, num_query_heads: int, scale: float | None = None):
+    def __init__(self, kv: PagedKV, num_query_heads: int, scale: float | None = None, workspace: Workspace | None = None):
         self.kv, self.num_query_heads = kv, num_query_heads
         self._qd = num_query_heads * kv.head_dim
         with _device(kv.index):      # the workspace follows the device's number of SMs
             n = lib().nnz_paged_attn_workspace(kv._ref, num_query_heads)
             _need(n > 0, f"paged attention over these pages does not take {num_query_heads} query heads")
-            self._ws = _Workspace(n, kv.device)
+            self.workspace = Workspace(n, kv.device) if workspace is None else workspace
+        buf = self.workspace.buf
+        _need(buf.device == kv.device and buf.numel() >= n, f"workspace: expected {n} bytes on {kv.device}, got {buf.numel()} on {buf.device}")
         a = capi.NnzPagedAttnArgs()
         a.num_query_heads, a.scale = num_query_heads, 0.0 if scale is None else scale
-        a.workspace, a.workspace_bytes = self._ws.buf.data_ptr(), n
+        a.workspace, a.workspace_bytes = buf.data_ptr(), n
         self._a, self._fn = a, lib().nnz_paged_attn
 
     def __call__(self, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, max_new: int,
@@ -211,7 +215,7 @@ class PagedAttention:
         a.page_table = _index(page_table, torch.int32, (seqs, page_table.shape[1]), kv.device, "page_table")
         a.table_stride = page_table.shape[1]
         a.q, a.out, a.tokens, a.num_seqs, a.max_new = q.data_ptr(), out.data_ptr(), n, seqs, max_new
-        ws, stream = self._ws, _stream(kv.index)
+        ws, stream = self.workspace, _stream(kv.index)
         with ws.lock:         # no other call's launch between the kernels of this one
             ws.on(stream)
             rc = self._fn(kv._ref, C.byref(a), stream)

@@ -95,7 +95,7 @@ class PagedModel:
         self.lm_head = self.embed if c.tie_word_embeddings else _Weights(c, q("lm_head"), H, self.device)
         self.final_norm = f32("model.norm.weight")
         self.table = paged.rope_table(c.rope_theta, hd, c.max_context_length, self.device)
-        self.layers = []
+        self.layers, workspace = [], None
         for i in range(c.num_layers):
             p = f"model.layers.{i}."
             kv = paged.PagedKV.empty(num_pages, c.num_kv_heads, page_size, hd, device=self.device)
@@ -107,7 +107,8 @@ class PagedModel:
                 "down": _Weights(c, q(p + "mlp.down_proj"), c.intermediate_size, self.device),
                 "write": paged.QKNormRope(kv, c.num_query_heads, f32(p + "self_attn.q_norm.weight"), f32(p + "self_attn.k_norm.weight"),
                                           self.table, eps=c.eps, rope_style=c.rope_style),
-                "attend": paged.PagedAttention(kv, c.num_query_heads)})
+                "attend": paged.PagedAttention(kv, c.num_query_heads, workspace=workspace)})      # layers run one after the other
+            workspace = self.layers[-1]["attend"].workspace
         self.free = list(range(num_pages))[::-1]
         self.page_size = page_size
 

@@ -412,7 +412,7 @@ def test_paged_attention_workspace_made_on_another_stream(lens):
     c = attn_case(91, lens, 8, 4, 128, 16, "f16", "head")
     want = check_attn(c)
     kv = P().PagedKV(c["k"], c["v"])
-    n = P().PagedAttention(kv, 8)._ws.buf.numel()
+    n = P().PagedAttention(kv, 8).workspace.buf.numel()
     made, used = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()
     with torch.cuda.stream(made):

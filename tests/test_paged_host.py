@@ -229,3 +229,32 @@ def test_a_workspace_follows_its_calls_from_stream_to_stream(paged, monkeypatch)
         op(*attn_inputs(3))
     assert log == [("wait", 2, 1), ("record", 2), ("launch", 2), ("launch", 2), ("launch", 4),
                    ("wait", 3, 2), ("record", 3), ("launch", 3), ("launch", 3)]
+
+
+def test_operators_share_a_workspace(paged):
+    """One after the other, from two threads too; a workspace that is too small or elsewhere is refused."""
+    first = paged.PagedAttention(host_kv(paged, hd=128), 4)
+    second = paged.PagedAttention(host_kv(paged), 4, workspace=first.workspace)
+    inside, overlap, where = [], [], []
+
+    def stub(kv, ref, stream):
+        overlap.append(len(inside))
+        inside.append(1)
+        where.append(struct_of(ref).workspace)
+        threading.Event().wait(0.05)
+        inside.pop()
+        return 0
+    first._fn = second._fn = stub
+    hd128 = (torch.zeros(3, 4 * 128, dtype=torch.float16), *attn_inputs(3)[1:])
+    t = [threading.Thread(target=lambda: first(*hd128)), threading.Thread(target=lambda: second(*attn_inputs(3)))]
+    for i in t:
+        i.start()
+    for i in t:
+        i.join(20)
+    assert overlap == [0, 0] and where == [first.workspace.buf.data_ptr()] * 2
+    small = paged.PagedAttention(host_kv(paged), 4).workspace
+    with pytest.raises(ValueError):
+        paged.PagedAttention(host_kv(paged, hd=128), 4, workspace=small)
+    small.buf = torch.empty(first.workspace.buf.numel(), dtype=torch.uint8, device="meta")
+    with pytest.raises(ValueError):
+        paged.PagedAttention(host_kv(paged), 4, workspace=small)

@@ -56,3 +56,11 @@ def test_score_matches_the_engine(cuda, built_lib):
     lp -= np.log(np.exp(lp).sum())
     assert np.abs(np.array(s.top_logprobs[-1]) - lp[s.top_ids[-1]]).max() <= 4e-2
     assert np.sort(lp)[-8] - lp[s.top_ids[-1]].min() <= 4e-2
+
+
+def test_the_layers_share_one_workspace(cuda, built_lib):
+    from nnzap_b200 import config_from_dims, synth
+    from nnzap_b200.score import PagedModel
+    d = synth.ModelDims(vocab=1000, hidden=256, inter=768, layers=3, n_q=4, n_kv=2, head_dim=128, gs=128, quant="q1")
+    m = PagedModel(config_from_dims(d, max_context_length=64), synth.iter_named_tensors(synth.make_model(d, seed=0)), num_pages=4)
+    assert len({id(L["attend"].workspace) for L in m.layers}) == 1
