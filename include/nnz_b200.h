@@ -271,8 +271,8 @@ int nnz_mlp(int fmt, int scale_dtype, int bf16_round, const void* gate_up, const
 /* Prefill GEMM on the tcgen05 tensor cores: out[m][n] (+)= sum_k x[m][k] *
  * W[n][k] for m < M, n < N, with W in the reference's flat layout (Q1 bits +
  * fp16 scales, or Q4 words + scales + biases; metal.zig:235-469) and x fp16
- * [M][K] (16-byte aligned, K % 64 == 0, gs >= 64).  out_kind NNZ_OUT_F16 or
- * NNZ_OUT_F32_ADD (row stride N).  No reference counterpart: the reference
+ * [M][K] (16-byte aligned, K % 64 == 0, gs >= 64).  out_kind NNZ_OUT_F16,
+ * NNZ_OUT_F32 or NNZ_OUT_F32_ADD (row stride N).  No reference counterpart: the reference
  * prefills token by token (transformer.zig:4032-4068). */
 int nnz_prefill_gemm(int fmt, int scale_dtype, const void* w, const uint16_t* scales,
                      const uint16_t* biases, uint32_t M, uint32_t K, uint32_t N, uint32_t gs,

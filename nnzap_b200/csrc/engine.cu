@@ -1852,7 +1852,7 @@ int nnz_prefill_gemm(int fmt, int scale_dtype, const void* w, const uint16_t* sc
                      const uint16_t* biases, uint32_t M, uint32_t K, uint32_t N, uint32_t gs,
                      const void* x, void* out, int out_kind, void* stream) {
   if (!w || !scales || !x || !out || (fmt == NNZ_Q4 && !biases) ||
-      (out_kind != NNZ_OUT_F16 && out_kind != NNZ_OUT_F32_ADD))
+      (out_kind != NNZ_OUT_F16 && out_kind != NNZ_OUT_F32 && out_kind != NNZ_OUT_F32_ADD))
     return fail(NNZ_EINVAL, "nnz_prefill_gemm: bad arguments");
   int dev = 0;
   NNZ_CK(cudaGetDevice(&dev));
@@ -1860,7 +1860,7 @@ int nnz_prefill_gemm(int fmt, int scale_dtype, const void* w, const uint16_t* sc
   g.M = M; g.K = K; g.N = N; g.fmt = fmt; g.gs = (int)gs;
   g.bf16s = fmt == NNZ_Q4 && scale_dtype == NNZ_SCALE_BF16; g.bf16r = 0;
   g.w = (const uint8_t*)w; g.s = scales; g.b = biases;
-  g.epi = out_kind == NNZ_OUT_F16 ? GEPI_F16 : GEPI_RESADD;
+  g.epi = out_kind == NNZ_OUT_F16 ? GEPI_F16 : out_kind == NNZ_OUT_F32 ? GEPI_F32 : GEPI_RESADD;
   g.out = out; g.ldo = N; g.err = nullptr;
   DevWs* ws;
   int rc = get_ws(&ws);

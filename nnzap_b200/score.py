@@ -46,11 +46,12 @@ class _Weights:
         self.b = None if q1 else dev("biases", np.int16)
         self.M = self.w.numel() * (8 if q1 else 2) // K
 
-    def gemm(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        """x [T][K] float16 times the transpose: float16 [T][M], or added to float32 ``out``."""
+    def gemm(self, x: torch.Tensor, out: torch.Tensor | None = None, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+        """x [T][K] float16 times the transpose: float16 or float32 [T][M], or added to float32 ``out``."""
         kind = capi.NNZ_OUT_F32_ADD
         if out is None:
-            kind, out = capi.NNZ_OUT_F16, torch.empty(x.shape[0], self.M, dtype=torch.float16, device=x.device)
+            kind = capi.NNZ_OUT_F16 if dtype is torch.float16 else capi.NNZ_OUT_F32
+            out = torch.empty(x.shape[0], self.M, dtype=dtype, device=x.device)
         check(lib().nnz_prefill_gemm(self.fmt, self.scale_dtype, self.w.data_ptr(), self.s.data_ptr(),
                                      None if self.b is None else self.b.data_ptr(), x.shape[0], self.K, self.M, self.gs,
                                      x.data_ptr(), out.data_ptr(), kind, paged._stream(x.device.index)))
@@ -129,7 +130,7 @@ class PagedModel:
             h = self._norm(x, L["ffn_norm"])
             g, u = L["gate"].gemm(h).float(), L["up"].gemm(h).float()
             L["down"].gemm((g * torch.sigmoid(g) * u).half(), out=x)
-        return self.lm_head.gemm(self._norm(x, self.final_norm), out=torch.zeros(len(x), self.lm_head.M, dtype=torch.float32, device=x.device))
+        return self.lm_head.gemm(self._norm(x, self.final_norm), dtype=torch.float32)
 
 
 @dataclasses.dataclass

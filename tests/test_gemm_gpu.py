@@ -42,3 +42,20 @@ def test_prefill_gemm_vs_oracle(cuda, built_lib, fmt, M, K, N, gs):
     tol = (1e-3, 1e-4) if fmt == 0 else (1e-2, 2e-3)
     close(y32.cpu().numpy(), base + want, *tol, "f32 add")
     close(y16.cpu().numpy().astype(np.float32), want, 2e-3 + tol[0], 2e-3 + tol[1], "f16")
+
+
+@pytest.mark.parametrize("fmt,M,K,N,gs", [(0, 5, 2048, 1000, 128), (0, 64, 256, 12301, 128), (1, 300, 512, 6144, 64), (0, 512, 2048, 4096, 128)])
+def test_prefill_gemm_writes_f32(cuda, built_lib, fmt, M, K, N, gs):
+    """NNZ_OUT_F32: over whatever the output held."""
+    torch = cuda
+    rng = np.random.default_rng(M + K + N)
+    t = synth.rand_q1(rng, N, K, gs) if fmt == 0 else synth.rand_q4(rng, N, K, gs)
+    x = rng.standard_normal((M, K)).astype(np.float16)
+    keep = [to_dev(torch, np.ascontiguousarray(t["weight"]).view(np.uint8)),
+            to_dev(torch, t["scales"]), to_dev(torch, t.get("biases", t["scales"])), to_dev(torch, x)]
+    y = torch.full((M, N), float("nan"), device="cuda")
+    check(lib().nnz_prefill_gemm(fmt, 0, ptr(keep[0]), ptr(keep[1]), ptr(keep[2]) if fmt == 1 else None, M, K, N, gs,
+                                 ptr(keep[3]), ptr(y), 1, None))
+    torch.cuda.synchronize()
+    want = R.qmv(cfg_for(fmt, gs, K), t, N, K, x.astype(np.float32))
+    close(y.cpu().numpy(), want, *((1e-3, 1e-4) if fmt == 0 else (1e-2, 2e-3)), "f32")

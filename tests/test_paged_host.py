@@ -199,7 +199,7 @@ def test_a_models_step_runs_on_its_device(paged, devices):
             seen.append(devices.current)
             return torch.zeros(len(ids), 4)
 
-        def gemm(self, x, out=None):
+        def gemm(self, x, out=None, dtype=None):
             seen.append(devices.current)
             return out
     m = object.__new__(PagedModel)
