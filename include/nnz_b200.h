@@ -214,7 +214,8 @@ int nnz_tp_init(nnz_model* m, const void* unique_id, size_t len);
 
 /* Waits for `stream` and returns the device-side errors raised since the
  * last check by the per-kernel entry points' launches on the current
- * device: NNZ_ETIMEDOUT when a bounded wait inside a kernel gave up (its
+ * device, on whatever stream they ran (one that is still running may raise
+ * one later, for the next check): NNZ_ETIMEDOUT when a bounded wait inside a kernel gave up (its
  * output is then invalid), NNZ_EDEVICE for an out-of-range position or
  * token id; the flags are cleared.  Allocates nothing.  No counterpart in
  * the reference (its kernels have no device-side error reporting: Metal

@@ -182,7 +182,7 @@ std::string err_text(int flags) {
 }  // namespace
 
 namespace nnz {
-int noalloc_take_error(int dev, int* flags);   // noalloc.cu
+int* noalloc_error_word(int dev);   // noalloc.cu
 // Lets other translation units of the library set nnz_last_error()'s text.
 void set_last_error(const std::string& msg) { g_err = msg; }
 
@@ -190,6 +190,17 @@ void set_last_error(const std::string& msg) { g_err = msg; }
 // its number of SMs, for the entry points that need nothing else.  The word
 // is a file-scope device variable, so nothing is allocated.
 static __device__ int g_op_err;
+static __device__ int g_taken_err;
+
+// Takes the device's error words: one exchange each, so that what a kernel of
+// another stream raises meanwhile is in this answer or left for the next.
+__global__ void take_errors_kernel(int* a, int* b, int* c) {
+  int flags = 0;
+  if (a) flags |= atomicExch(a, 0);
+  if (b) flags |= atomicExch(b, 0);
+  if (c) flags |= atomicExch(c, 0);
+  g_taken_err = flags;
+}
 
 int op_device(int** err, int* num_sms) {
   constexpr int kMaxDevices = 64;
@@ -1894,33 +1905,31 @@ int nnz_attn_decode(const void* qkv, const float* q_norm, const float* k_norm, v
 }
 
 // Waits for `stream`, then reports (and clears) the device error flags that
-// the per-kernel entry points' launches on the current device raised: a
-// bounded wait that gave up (NNZ_ETIMEDOUT) or an out-of-range position /
-// token (NNZ_EDEVICE).  Allocates nothing.
+// the per-kernel entry points' launches on the current device raised, on
+// whatever stream: a bounded wait that gave up (NNZ_ETIMEDOUT) or an
+// out-of-range position / token (NNZ_EDEVICE).  Allocates nothing.
 int nnz_stream_check(void* stream) {
   return host_guard([&]() -> int {
-    NNZ_CK(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    NNZ_CK(cudaStreamSynchronize(st));
     int dev = 0;
     NNZ_CK(cudaGetDevice(&dev));
-    int flags = 0;
+    int *ws_err = nullptr, *op_err = nullptr, sms = 0, flags = 0;
     {
       std::lock_guard<std::mutex> lk(g_ws_mu);
       auto it = g_ws.find(dev);
-      if (it != g_ws.end() && it->second.err) {
-        NNZ_CK(cudaMemcpy(&flags, it->second.err, sizeof(int), cudaMemcpyDeviceToHost));
-        if (flags) NNZ_CK(cudaMemset(it->second.err, 0, sizeof(int)));
-      }
+      if (it != g_ws.end()) ws_err = it->second.err;
     }
-    int na = 0;
-    int rc = noalloc_take_error(dev, &na);
+    const int rc = op_device(&op_err, &sms);
     if (rc) return rc;
-    flags |= na;
-    int *op_err = nullptr, sms = 0, no = 0;
-    rc = op_device(&op_err, &sms);
-    if (rc) return rc;
-    NNZ_CK(cudaMemcpy(&no, op_err, sizeof(int), cudaMemcpyDeviceToHost));
-    if (no) NNZ_CK(cudaMemset(op_err, 0, sizeof(int)));
-    flags |= no;
+    {
+      static std::mutex one;      // g_taken_err serves one check at a time
+      std::lock_guard<std::mutex> lk(one);
+      take_errors_kernel<<<1, 1, 0, st>>>(ws_err, noalloc_error_word(dev), op_err);
+      NNZ_CK(cudaGetLastError());
+      NNZ_CK(cudaMemcpyFromSymbolAsync(&flags, g_taken_err, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+      NNZ_CK(cudaStreamSynchronize(st));
+    }
     if (flags)
       return fail(flags & (ERR_MBAR_TIMEOUT | ERR_SPIN_TIMEOUT) ? NNZ_ETIMEDOUT : NNZ_EDEVICE, err_text(flags));
     return NNZ_OK;

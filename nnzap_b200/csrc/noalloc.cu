@@ -82,23 +82,12 @@ int setup(int dev, NoAllocDev** out) {
 
 }  // namespace
 
-// Device error flags raised by no-alloc launches on device `dev` since the
-// last call (read with a copy from the symbol, cleared; no allocation).
-int noalloc_take_error(int dev, int* flags) {
-  *flags = 0;
-  if (dev < 0 || dev >= kMaxDevices) return NNZ_OK;
-  int* p = nullptr;
-  {
-    std::lock_guard<std::mutex> lk(g_mu);
-    if (!g_dev[dev].ready) return NNZ_OK;
-    p = g_dev[dev].err;
-  }
-  if (cudaMemcpy(flags, p, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess ||
-      (*flags && cudaMemset(p, 0, sizeof(int)) != cudaSuccess)) {
-    set_last_error(std::string("nnz_stream_check: ") + cudaGetErrorString(cudaGetLastError()));
-    return NNZ_ECUDA;
-  }
-  return NNZ_OK;
+// The word that no-alloc launches on device `dev` raise errors in (device
+// memory); null before the first of them.
+int* noalloc_error_word(int dev) {
+  if (dev < 0 || dev >= kMaxDevices) return nullptr;
+  std::lock_guard<std::mutex> lk(g_mu);
+  return g_dev[dev].ready ? g_dev[dev].err : nullptr;
 }
 }  // namespace nnz
 

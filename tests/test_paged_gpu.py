@@ -404,6 +404,52 @@ def test_paged_ops_on_another_stream():
     assert torch.equal(lp.top_ids, P().token_logprobs(got.float(), top_k=3).top_ids)
 
 
+def test_errors_raised_while_others_are_collected_are_kept():
+    """Two streams raise an error of their own kind while a thread collects
+    errors on a third: every one of them is reported."""
+    import threading
+    from nnzap_b200._capi import NnzError
+    kv = P().PagedKV.empty(4, 2, 8, 128)
+    one = torch.ones(128, device="cuda")
+    op = P().QKNormRope(kv, 4, one, one, P().rope_table(1e4, 128, 64))
+    qkv = torch.zeros(1, 8 * 128, dtype=torch.float16, device="cuda")
+    i32, i64 = dict(dtype=torch.int32, device="cuda"), dict(dtype=torch.int64, device="cuda")
+    position = (torch.tensor([64], **i32), torch.tensor([0], **i64))
+    page = (torch.tensor([0], **i32), torch.tensor([32], **i64))
+    outs = [torch.zeros(1, 4 * 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+    a, b, c = (torch.cuda.Stream() for _ in range(3))
+    torch.cuda.synchronize()
+    seen, checks, stop = set(), [0], threading.Event()
+
+    def collect():
+        with torch.cuda.stream(c):
+            while not stop.is_set():
+                try:
+                    P().stream_check()
+                except NnzError as e:
+                    seen.update(w for w in ("position", "page") if w in str(e))
+                checks[0] += 1
+    t = threading.Thread(target=collect)
+    t.start()
+    lost = 0
+    try:
+        for _ in range(500):
+            seen.clear()
+            for st, bad, out in ((a, position, outs[0]), (b, page, outs[1])):
+                with torch.cuda.stream(st):
+                    op(qkv, *bad, out=out)
+            a.synchronize()
+            b.synchronize()
+            done = checks[0] + 2                        # a check that began after this
+            while checks[0] < done and t.is_alive():
+                pass
+            lost += seen != {"position", "page"}
+    finally:
+        stop.set()
+        t.join()
+    assert lost == 0
+
+
 @pytest.mark.parametrize("lens", [[(1, 9000), (1, 3)], [(200, 4000)]])
 def test_paged_attention_workspace_made_on_another_stream(lens):
     """An operator whose workspace is still to be zeroed, behind other work on
