@@ -517,7 +517,7 @@ int nnz_paged_attn(const nnz_paged_kv* kv, const nnz_paged_attn_args* p, void* s
   if (!p->q || !p->q_start || !p->kv_len || !p->page_table || !p->out || !p->workspace)
     return refuse(NNZ_EINVAL, "nnz_paged_attn: null argument");
   if (p->tokens > 0x7FFFFFFFu || p->num_seqs > 0x7FFFFFFFu || p->table_stride == 0 ||
-      (uint64_t)p->table_stride * kv->page_size > 0x7FFF0000u || !(p->scale >= 0.f))
+      (uint64_t)p->table_stride * kv->page_size > 0x7FFF0000u || !(p->scale >= 0.f && isfinite(p->scale)))
     return refuse(NNZ_EINVAL, "nnz_paged_attn: tokens, num_seqs, table_stride or scale");
   if (p->q_stride % 8 || p->q_stride < p->num_query_heads * hd || p->out_stride % 8 || p->out_stride < p->num_query_heads * hd)
     return refuse(NNZ_EINVAL, "nnz_paged_attn: row strides must be multiples of 8 elements that hold the heads");

@@ -180,13 +180,16 @@ class PagedAttention:
     ``q`` holds the new tokens of all sequences one after the other; sequence
     s has rows ``q_start[s]:q_start[s + 1]`` and ``kv_len[s]`` keys, its new
     tokens' included, on the pages ``page_table[s]`` (negative: absent).
-    ``max_new`` is a host-known upper bound of one sequence's new tokens.  The
+    ``max_new`` is a host-known upper bound of one sequence's new tokens.
+    ``scale`` is positive (None: 1 / sqrt(head_dim)).  The
     object's ``workspace`` serves one call at a time: threads may share the
     object, and a call on another stream waits for the one before.  Operators
     whose calls follow one another (a model's layers) can have one workspace:
     pass the first one's as ``workspace``."""
 
     def __init__(self, kv: PagedKV, num_query_heads: int, scale: float | None = None, workspace: Workspace | None = None):
+        # (0 is the library's word for the default)
+        _need(scale is None or 0 < C.c_float(scale).value < float("inf"), f"scale must be positive and finite, got {scale}")
         self.kv, self.num_query_heads = kv, num_query_heads
         self._qd = num_query_heads * kv.head_dim
         with _device(kv.index):      # the workspace follows the device's number of SMs
@@ -205,6 +208,7 @@ class PagedAttention:
         if _current_device() != self.kv.index:
             with _device(self.kv.index):
                 return self(q, page_table, q_start, kv_len, max_new, out)
+        _need(0 <= max_new < 1 << 31, f"max_new: {max_new}")      # (ctypes would wrap it)
         a, kv, n, seqs = _own(self._a), self.kv, q.shape[0], kv_len.shape[0]
         if out is None:   # rows outside every sequence are not written
             out = torch.zeros(n, self._qd, dtype=kv.dtype, device=kv.device)

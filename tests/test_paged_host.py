@@ -258,3 +258,29 @@ def test_operators_share_a_workspace(paged):
     small.buf = torch.empty(first.workspace.buf.numel(), dtype=torch.uint8, device="meta")
     with pytest.raises(ValueError):
         paged.PagedAttention(host_kv(paged), 4, workspace=small)
+
+
+# ---- numbers -----------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [0.0, 1e-60, -1.0, 1e60, float("inf"), float("nan")])
+def test_scales_that_are_none(paged, scale):
+    """0 would be taken for the default, an infinite one makes every row NaN."""
+    with pytest.raises(ValueError):
+        paged.PagedAttention(host_kv(paged), 4, scale=scale)
+
+
+@pytest.mark.parametrize("max_new", [-1, 1 << 31, 1 << 32])
+def test_counts_that_do_not_fit(paged, max_new):
+    op = paged.PagedAttention(host_kv(paged), 4)
+    op._fn = lambda *a: pytest.fail("called")
+    with pytest.raises(ValueError):
+        op(*attn_inputs(3)[:4], max_new)
+
+
+def test_the_library_refuses_an_infinite_scale():
+    from nnzap_b200 import _capi as capi
+    kv = capi.NnzPagedKv(k=0x1000, v=0x2000, dtype=capi.NNZ_DT_F16, num_pages=4, page_size=16, num_kv_heads=2, head_dim=128,
+                         page_stride=4096, head_stride=2048, token_stride=128)
+    a = capi.NnzPagedAttnArgs(q=0x1000, q_stride=512, tokens=3, num_query_heads=4, num_seqs=1, max_new=3, q_start=0x1000, kv_len=0x1000,
+                              page_table=0x1000, table_stride=4, scale=float("inf"), out=0x1000, out_stride=512, workspace=0x1000,
+                              workspace_bytes=1 << 30)
+    assert capi.lib().nnz_paged_attn(C.byref(kv), C.byref(a), None) == capi.NNZ_EINVAL
