@@ -169,6 +169,9 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(128) paged_attn_any_kernel(const PagedAttnArgs a) {
   constexpr int EPL = HD / 32;   // elements per lane, in 2-element words
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0)      // ranges and lengths are looked at here: no row need come across them
+    for (uint32_t s = threadIdx.x; s < a.num_seqs; s += blockDim.x)
+      if (seq_bad(a, seq_info(a, s))) atomicOr(a.err, ERR_BAD_PAGE);
   const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const uint32_t row = (uint32_t)(unit / a.n_q), h = (uint32_t)(unit % a.n_q);
   if (row >= a.tokens) return;
@@ -180,17 +183,10 @@ __global__ void __launch_bounds__(128) paged_attn_any_kernel(const PagedAttnArgs
     else hi = mid;
   }
   const int64_t qs = a.q_start[lo], qe = a.q_start[lo + 1];
-  if (row < qs || row >= qe || qs < 0) {
-    if (qs < 0 && lane == 0) atomicOr(a.err, ERR_BAD_PAGE);
-    return;
-  }
-  if (row - qs >= (int64_t)a.max_new) {
-    if (lane == 0) atomicOr(a.err, ERR_BAD_PAGE);
-    return;
-  }
+  if (row < qs || row >= qe || qs < 0 || row - qs >= (int64_t)a.max_new) return;
   const int64_t cap = (int64_t)a.table_stride * a.kv.page_size;
   int64_t len = a.kv_len[lo];
-  bool bad = len > cap || len < 0 || qe > (int64_t)a.tokens;
+  bool bad = false;         // a page outside the pool
   const int64_t last = min(len, len - (qe - qs) + (row - qs) + 1);   // keys [0, last) are visible
   len = min(last, cap);
   const uint16_t* qp = a.q + (int64_t)row * a.q_stride + h * HD;

@@ -382,6 +382,31 @@ def test_paged_attention_bad_tables_are_reported():
                 P().stream_check()
 
 
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("what", ["empty sequence", "descending", "past the end", "negative length"])
+def test_paged_attention_bad_sequences_without_rows_are_reported(page, new, what):
+    """Ranges and lengths that no row of the output comes across, in every kernel."""
+    from nnzap_b200._capi import NNZ_EDEVICE, NnzError
+    c = attn_case(53, [(new, 300), (new, 200), (new, 100)], 4, 2, 128, page, "f16", "head", poison=False, extra_cols=0)
+    q_start, kv_len = c["q_start"].tolist(), c["kv_len"].tolist()
+    if what == "empty sequence":
+        q_start, kv_len = [0, new, new, 2 * new], [300, c["table"].shape[1] * page + 1, 100]
+    elif what == "descending":
+        q_start = [0, new, 0, 2 * new]
+    elif what == "past the end":
+        q_start = [0, new, 3 * new, 4 * new]
+    else:
+        q_start, kv_len = [0, new, new, 2 * new], [300, -1, 100]
+    out = torch.full_like(c["q"], 3.0)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    P().PagedAttention(P().PagedKV(c["k"], c["v"]), 4)(c["q"], c["table"], torch.tensor(q_start, **i32), torch.tensor(kv_len, **i32), 2 * new, out=out)
+    with pytest.raises(NnzError) as e:
+        P().stream_check()
+    assert e.value.code == NNZ_EDEVICE and torch.isfinite(out).all()
+    P().stream_check()
+
+
 def test_paged_ops_on_another_stream():
     """Calls go to torch's current stream: a long-running producer on it is waited for."""
     c = attn_case(61, [(40, 400), (1, 90)], 8, 4, 128, 16, "f16", "head")
