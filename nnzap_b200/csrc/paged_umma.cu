@@ -90,9 +90,9 @@ struct UmShape {
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr uint32_t OFF_KV = 2 * kTileB;
   static constexpr uint32_t OFF_BAR = OFF_KV + kStages * kTileB;
-  static constexpr int kBars = 2 * kStages + 8 + 3 * kPres + 2 * kSegs;
+  static constexpr int kBars = 2 * kStages + 9 + 3 * kPres + 2 * kSegs;
   static constexpr uint32_t OFF_MISC = OFF_BAR + kBars * 8;
-  static constexpr uint32_t OFF_SEG = OFF_MISC + 64, OFF_XT = OFF_SEG + kSegs * 80;
+  static constexpr uint32_t OFF_SEG = OFF_MISC + 80, OFF_XT = OFF_SEG + kSegs * 80;
   static constexpr uint32_t kSmem = OFF_XT + 1024 + 1024;
 };
 
@@ -346,7 +346,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   uint64_t* kv_empty = kv_full + S::kStages;
   uint64_t* q_full = kv_empty + S::kStages;
   uint64_t* q_empty = q_full + 1;
-  uint64_t* s_full = q_empty + 1;        // [2] S of a row tile complete
+  uint64_t* drained = q_empty + 1;       // every product is complete (after a wait that gave up)
+  uint64_t* s_full = drained + 1;        // [2] S of a row tile complete
   uint64_t* p_full = s_full + 2;         // [2] P written, O rescaled (8 warps)
   uint64_t* pv_done = p_full + 2;        // [2] P V complete
   uint64_t* v_ready = pv_done + 2;       // [kPres] a unit's V tile has been cleaned (units that need it; 16 warps)
@@ -364,6 +365,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   // every barrier by its own thread; arrivals: a warp each for P (8), a clean V
   // tile (16) and a part's end (17), else 1
   static_assert(S::kBars <= kUmThreads);
+  if (threadIdx.x < 8) tslot[1 + kPres + threadIdx.x] = 0;
   if (threadIdx.x < (uint32_t)S::kBars) {
     uint64_t* b = kv_full + threadIdx.x;
     mbar_init(b, b == p_full || b == p_full + 1 ? 8 : b >= v_ready && b < v_go ? 16 : b >= seg_empty ? 17 : 1);
@@ -384,7 +386,12 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   pdl_launch();       // the merge kernel may be set up (it waits for this one's end)
   // Bounded waits: one that gives up leaves no tries to the later ones, and the
   // error is reported at the end (nothing but the poll stands in the loop).
+  // Who gave up stops at its next part, all lanes of a warp and both warps of
+  // a pair together, or those left would wait at barriers that have no bound; a
+  // part that is not finished with is not replaced, and copies and products
+  // under way are waited for, with new tries, before the CTA ends.
   uint32_t tries = kUmTries;
+  auto gave_up = [&] { return __any_sync(0xffffffffu, tries == 0) != 0; };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     for (uint32_t n = 0; !mbar_try_wait(bar, parity & 1u);)
       if (++n > tries) {
@@ -393,13 +400,13 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       }
   };
 
-  // part k of the run; warps 0-15 and 17 take them in order from warp 16
+  // part k of the run; warp 17, and 0-15 likewise, take them in order from warp 16
   // (fields are read into registers one by one: a copy indexed by the row tile
   // would live in local memory, which with this much shared memory means L2)
   auto segment = [&](uint32_t k) -> const Segment* {
     wait(seg_full + k % kSegs, k / kSegs);
     const Segment* g = segs + k % kSegs;
-    return g->take != 0 && tries ? g : nullptr;
+    return !gave_up() && g->take != 0 ? g : nullptr;
   };
   auto segment_done = [&](uint32_t k) {
     __syncwarp();
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     }
     const uint32_t nb = kUmKeys / t.box;
     const uint32_t bi = (uint32_t)lane % nb;      // this lane's box of a unit
-    uint32_t stage_use = 0, unit_no = 0;
+    uint32_t stage_use = 0, unit_no = 0, q_use = 0;
     for (uint32_t seg = 0;; ++seg) {
       // ---- the next part: to the other warps ----
       Segment o{};
@@ -468,7 +475,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           o.gaps = __any_sync(0xffffffffu, gap) ? 1u : 0u;
         }
         if (seg >= kSegs) wait(seg_empty + seg % kSegs, seg / kSegs - 1);
-        __syncwarp();
+        if (gave_up()) return;
         if (lane == 0) {
           segs[seg % kSegs] = o;
           mbar_arrive1(seg_full + seg % kSegs);
@@ -476,7 +483,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       };
       // (the first part's loads go first: nobody can use it before they land)
       if (seg || !o.take) publish();
-      if (o.take == 0 || !tries) break;
+      if (gave_up() || o.take == 0) break;
       u += o.take;
       more = even && u < u1 && cursor_next_task(a, c, QT, kUmKeys);
 
@@ -501,7 +508,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       // products have read theirs (its first K tile does not wait for that)
       auto queries = [&] {
         if (seg) wait(q_empty, seg - 1);
-        __syncwarp();
+        if (gave_up()) return;
+        ++q_use;
         const int tiles = PT < o.rows ? 2 : 1;
         if (lane == 0) {
           mbar_arrive_expect_tx(q_full, (uint32_t)tiles * NH * G * PT * 128);
@@ -512,7 +520,8 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         __syncwarp();
       };
       if (seg == 0) queries();
-      for (uint32_t i = 0; i < o.take; ++i) {
+      bool on = true;
+      for (uint32_t i = 0; on && i < o.take; ++i) {
         if (i + 1 < o.take) npg = page_of(i + 1, nat);
         const uint32_t mask = __ballot_sync(0xffffffffu, (uint32_t)lane < nb && pg >= 0);
         if (pg < 0) pg = (int)a.kv.num_pages;
@@ -524,8 +533,11 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t st = stage_use % S::kStages, round = stage_use / S::kStages;
-          if (round) wait(kv_empty + st, round - 1);
-          __syncwarp();
+          if (round) {
+            wait(kv_empty + st, round - 1);
+            on = !gave_up();
+            if (!on) break;
+          }
           if (lane == 0) mbar_arrive_expect_tx(kv_full + st, S::kTileB);
           __syncwarp();
           // one elected lane issues (a lane each takes the compiler's loop over
@@ -550,6 +562,12 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         at = nat;
         ++unit_no;
       }
+    }
+    if (gave_up()) {
+      tries = kUmTries;
+      for (uint32_t n = stage_use > (uint32_t)S::kStages ? stage_use - S::kStages : 0; n < stage_use; ++n) wait(kv_full + n % S::kStages, n / S::kStages);
+      if (q_use) wait(q_full, q_use - 1);
+      tries = 0;
     }
   } else if (warp == kWMma) {
     // ---------------- MMA ----------------
@@ -635,7 +653,15 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       stage_use += 2 * take;
       segment_done(seg);
     }
-    if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
+    if (gave_up()) {
+      tries = kUmTries;
+      if (elect_one()) umma_commit(drained);
+      __syncwarp();
+      wait(drained, 0);
+      tries = 0;
+    } else if (stage_use) {
+      wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
+    }
   }
   } else {
     // ---------------- softmax and epilogue of row tile x ----------------
@@ -647,10 +673,27 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
     uint32_t ns = 0, unit_no = 0;       // units of this row tile, units of the run
     uint32_t vphase = 0;                // bit s: parity of v_go[s]
     if (threadIdx.x == 0) t.ws.head[blockIdx.x] = {0, 0, 0, 0};
+    // Part k of the run; both warps of a pair enter it or neither does.  Who
+    // comes first decides (2 k + 2: entered, 2 k + 3: not); the other may be at
+    // an earlier part still.  (A vote at the pair's barrier: 0.7 us of 512 tokens'
+    // 36.7.)
+    uint32_t* agreed = tslot + 1 + kPres + 4 * x + (warp & 3);
+    auto enter = [&](uint32_t k) -> const Segment* {
+      wait(seg_full + k % kSegs, k / kSegs);
+      const Segment* g = segs + k % kSegs;
+      bool no = gave_up();
+      if (!no && g->take == 0) return nullptr;
+      uint32_t old = 0;
+      if (lane == 0) old = atomicCAS(agreed, 2 * k, 2 * k + (no ? 3 : 2));
+      old = __shfl_sync(0xffffffffu, old, 0);
+      if (old > 2 * k) no = old == 2 * k + 3;
+      __syncwarp();
+      return no ? nullptr : g;
+    };
     // (of a part only what its every unit needs is kept in registers: the
     // loop's spills are read back from L2)
     for (uint32_t seg = 0;; ++seg) {
-      const Segment* g = segment(seg);
+      const Segment* g = enter(seg);
       if (!g) break;
       const uint32_t units = g->n[x];
       auto token = [&] { return x * PT + (int)(r / G); };               // of the task
@@ -813,7 +856,7 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
       segment_done(seg);
     }
   }
-  if (!tries && lane == 0) atomicOr(a.err, ERR_MBAR_TIMEOUT);
+  if (gave_up() && lane == 0) atomicOr(a.err, ERR_MBAR_TIMEOUT);
   tc_fence_before();
   __syncthreads();
   if (warp == kWMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
