@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kStWarps * 32, CL ? 1 : 0) paged_stream_kernel
     pstg = pstg + 1 == S::kStages ? 0 : pstg + 1;
   }
 
-  bool failed = false;
+  uint32_t flying = (uint32_t)(u1 - u0) - left;      // units issued and not waited for yet
   int cstg = 0;
   uint32_t phase = 0;       // bit s: parity of stage s
   uint64_t u = u0;
@@ -301,7 +301,22 @@ __global__ void __launch_bounds__(kStWarps * 32, CL ? 1 : 0) paged_stream_kernel
       l[r] = 0.f;
     }
     for (uint32_t i = 0; i < take; ++i) {
-      if (!failed) failed = !mbar_wait(&bars[cstg], (phase >> cstg) & 1u, a.err);
+      // A wait that gives up ends the copies, and is tried once more: none may
+      // be under way when the ring is used again or the CTA is left.  (The
+      // units that are then not loaded are worked on as the ring is.)
+      if (flying) {
+        --flying;
+        auto landed = [&] {        // the warp as one
+          for (uint32_t n = 0; !__all_sync(0xffffffffu, mbar_try_wait(&bars[cstg], (phase >> cstg) & 1u));)
+            if (++n == kSpinLimit) return false;
+          return true;
+        };
+        if (!landed()) {
+          left = 0;
+          landed();
+          if (lane == 0) atomicOr(a.err, ERR_MBAR_TIMEOUT);
+        }
+      }
       phase ^= 1u << cstg;
       const uint32_t kb = smem_u32(ring + cstg * S::kStageB), vb = kb + S::kHalves * S::kBoxB;
       const int key0 = (int)(c.unit + i) * kStKeys;
@@ -428,7 +443,10 @@ __global__ void __launch_bounds__(kStWarps * 32, CL ? 1 : 0) paged_stream_kernel
         }
       }
       __syncwarp();
-      if (left) issue(cstg);   // refill the slot just consumed
+      if (left) {              // refill the slot just consumed
+        issue(cstg);
+        ++flying;
+      }
       cstg = cstg + 1 == S::kStages ? 0 : cstg + 1;
     }
 #pragma unroll
