@@ -108,6 +108,32 @@ def test_qk_norm_rope_in_place_and_bad_tokens():
     assert torch.equal(qkv[:, :512], ref) and torch.equal(qkv[:, 512:], src[:, 512:])
 
 
+# more heads than a thread asks for at once: 32 of 128, 64 of 64
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("style", ["pairwise", "half_split"])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n_q,n_kv,hd,T", [(32, 8, 128, 19), (64, 8, 64, 7), (70, 35, 64, 3), (128, 1, 128, 2)])
+def test_qk_norm_rope_many_heads(dtype, style, in_place, n_q, n_kv, hd, T):
+    rng = np.random.default_rng(n_q + hd)
+    dt, H = DT[dtype], n_q + 2 * n_kv
+    kv = P().PagedKV.empty(3, n_kv, 8, hd, dtype=dt)
+    qkv = dev(rng.standard_normal((T, H * hd), dtype=np.float32) * 2, dt)
+    src = qkv.clone().view(T, H, hd)
+    qn, kn = (dev(1 + 0.3 * rng.standard_normal(hd), torch.float32) for _ in range(2))
+    table = P().rope_table(1e6, hd, 5000)
+    pos, slots = dev(rng.integers(0, 5000, T).astype(np.int32)), dev(rng.permutation(24)[:T].astype(np.int64))
+    op = P().QKNormRope(kv, n_q, qn, kn, table, eps=1e-6, rope_style=style)
+    got = op(qkv, pos, slots, out=qkv[:, :n_q * hd] if in_place else None)
+    P().stream_check()
+    rows = table[pos.long()]
+    want, mag = R.norm_rope(src[:, :n_q], qn, rows, 1e-6, style)
+    within(got.reshape(T, n_q, hd), want, R.norm_rope_bound(want, mag, dt), "q")
+    wk, mk = R.norm_rope(src[:, n_q:n_q + n_kv], kn, rows, 1e-6, style)
+    within(kv.k[slots // 8, :, slots % 8], wk, R.norm_rope_bound(wk, mk, dt), "k")
+    assert torch.equal(kv.v[slots // 8, :, slots % 8], src[:, n_q + n_kv:])
+    assert torch.equal(qkv.view(T, H, hd)[:, n_q:], src[:, n_q:])
+
+
 # ---- attention over pages ------------------------------------------------------
 def attn_case(seed, lens, n_q, n_kv, hd, page, dtype, layout, absent=0.0, gap=0, poison=True, scale=None, extra_cols=1):
     """lens: [(new, keys)].  Slots that no sequence owns hold NaN and infinities."""
@@ -553,6 +579,22 @@ def test_token_logprobs(dtype, rows, n, pad, k):
     before = full.clone()
     check_lp(full[:, :n], tok, k)
     assert torch.equal(full[:, :n], before[:, :n])
+
+
+@pytest.mark.parametrize("dtype,n", [("f32", 100001), ("f32", 151936), ("f32", 200001), ("bf16", 200003), ("f16", 420001)])
+@pytest.mark.parametrize("k", [20, 32])
+def test_token_logprobs_long_rows_of_many(dtype, n, k):
+    """A row to a CTA, whose steps (4096 f32, 8192 16-bit elements) share the 24
+    slots of step maxima by two or more: the best values lie in the first,
+    second, third and last steps, several to a step."""
+    rows, step = 150, 4096 if dtype == "f32" else 8192
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(rows, n, device="cuda", generator=g)
+    at = torch.tensor([step + 5, step + 900, 3 * step - 1, 2 * step, 7, step - 1, n - 1, n - n % step, 5 * step + 2], device="cuda")
+    x[:, at] = 20 + torch.arange(len(at), device="cuda") % 4 * 0.5
+    x[1::2] = x[1::2].roll(step, -1)
+    tok = torch.randint(0, n, (rows,), device="cuda", generator=g).to(torch.int32)
+    check_lp(x.to(DT[dtype]), tok, k)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
