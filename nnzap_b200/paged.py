@@ -31,19 +31,11 @@ _DTYPES = {torch.float16: capi.NNZ_DT_F16, torch.bfloat16: capi.NNZ_DT_BF16, tor
 _ROPE = {"pairwise": capi.NNZ_ROPE_PAIRWISE, "half_split": capi.NNZ_ROPE_HALF_SPLIT}
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def _stream(device: int | None = None) -> int:
-    """The current stream's handle (the raw query skips building a Stream object, about a microsecond)."""
-    if _raw_stream is not None and device is not None:
-        return _raw_stream(device)
-    return torch.cuda.current_stream(device).cuda_stream
-
-
+# A device's current stream's handle.  (The raw query skips building a Stream object, about a microsecond.)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 # The library launches on the current device, and the default stream's handle is 0 on every device: a call whose
 # tensors are elsewhere makes their device the current one first.
-_current_device, _device = torch.cuda.current_device, torch.cuda.device
+_current_device, _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device), torch.cuda.device
 _current_stream, _capturing = torch.cuda.current_stream, torch.cuda.is_current_stream_capturing
 
 
@@ -52,10 +44,13 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _own(args):
-    """One call's own copy of an operator's constant arguments: the library reads them with the GIL released,
-    while another thread may be calling the same operator."""
-    return type(args).from_buffer_copy(args)
+class _Own(threading.local):
+    """Each thread's own copy of an operator's constant arguments, for a call to complete: the library reads them with
+    the GIL released, while another thread may be calling the same operator."""
+
+    def __init__(self, args):
+        args = type(args).from_buffer_copy(args)
+        self.args = args, C.byref(args)
 
 
 def _index(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device, what: str) -> int:
@@ -131,13 +126,14 @@ class QKNormRope:
         a.k_norm = _index(k_norm, torch.float32, (hd,), kv.device, "k_norm")
         a.rope_table = _index(table, torch.float32, (table.shape[0], hd // 2, 2), kv.device, "table")
         a.table_positions = table.shape[0]
-        self._a, self._fn = a, lib().nnz_qk_norm_rope_paged
+        self._own, self._fn = _Own(a), lib().nnz_qk_norm_rope_paged
 
     def __call__(self, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        if _current_device() != self.kv.index:
-            with _device(self.kv.index):
+        kv, n = self.kv, qkv.shape[0]
+        if _current_device() != kv.index:
+            with _device(kv.index):
                 return self(qkv, positions, slots, out)
-        a, kv, n = _own(self._a), self.kv, qkv.shape[0]
+        a, ref = self._own.args
         if out is None:
             out = torch.empty(n, self._qd, dtype=kv.dtype, device=kv.device)
         a.qkv_stride = _rows(qkv, n, self._width, kv, "qkv")
@@ -145,32 +141,34 @@ class QKNormRope:
         a.positions = _index(positions, torch.int32, (n,), kv.device, "positions")
         a.slots = _index(slots, torch.int64, (n,), kv.device, "slots")
         a.qkv, a.q_out, a.tokens = qkv.data_ptr(), out.data_ptr(), n
-        rc = self._fn(kv._ref, C.byref(a), _stream(kv.index))
+        rc = self._fn(kv._ref, ref, _stream(kv.index))
         if rc:
             check(rc)
         return out
 
 
 class Workspace:
-    """Memory that a :class:`PagedAttention` call's kernels hand their parts on through, and which every call leaves as
-    it found it: one call uses it at a time, of whichever operator has it.  A call on another stream than the last one's waits for that one on the device (or, the first
-    call, for the zeros), and the allocator learns of the stream.  Inside a graph capture it does neither: the order
-    of a graph's launches is that of who replays it."""
+    """Memory that a :class:`PagedAttention` call's kernels hand their parts on
+    through, and which every call leaves as it found it: one call uses it at a
+    time, of whichever operator has it.  A call on another stream than the last
+    one's waits for that one on the device (or, the first call, for the zeros),
+    and the allocator learns of the stream.  Inside a graph capture it does
+    neither: the order of a graph's launches is that of who replays it."""
 
     def __init__(self, nbytes: int, device: torch.device):
         self.lock = threading.Lock()
         self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         self._last = _current_stream(device)
-        self._handle = self._last.cuda_stream
+        self.handle = self._last.cuda_stream       # the stream of the last use
 
-    def on(self, handle: int) -> None:
+    def move(self, handle: int) -> None:
         """The next use is on the current stream, whose handle this is (under the lock)."""
-        if handle == self._handle or _capturing():
+        if _capturing():
             return
         now = _current_stream(self.buf.device)
         now.wait_stream(self._last)
         self.buf.record_stream(now)
-        self._last, self._handle = now, handle
+        self._last, self.handle = now, handle
 
 
 class PagedAttention:
@@ -201,28 +199,31 @@ class PagedAttention:
         a = capi.NnzPagedAttnArgs()
         a.num_query_heads, a.scale = num_query_heads, 0.0 if scale is None else scale
         a.workspace, a.workspace_bytes = buf.data_ptr(), n
-        self._a, self._fn = a, lib().nnz_paged_attn
+        self._own, self._fn = _Own(a), lib().nnz_paged_attn
 
     def __call__(self, q: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, max_new: int,
                  out: torch.Tensor | None = None) -> torch.Tensor:
-        if _current_device() != self.kv.index:
-            with _device(self.kv.index):
+        kv, n, seqs = self.kv, q.shape[0], kv_len.shape[0]
+        if _current_device() != kv.index:
+            with _device(kv.index):
                 return self(q, page_table, q_start, kv_len, max_new, out)
-        _need(0 <= max_new < 1 << 31, f"max_new: {max_new}")      # (ctypes would wrap it)
-        a, kv, n, seqs = _own(self._a), self.kv, q.shape[0], kv_len.shape[0]
+        if not 0 <= max_new < 1 << 31:      # (ctypes would wrap it)
+            raise ValueError(f"max_new: {max_new}")
+        a, ref = self._own.args
         if out is None:   # rows outside every sequence are not written
             out = torch.zeros(n, self._qd, dtype=kv.dtype, device=kv.device)
         a.q_stride = _rows(q, n, self._qd, kv, "q")
         a.out_stride = _rows(out, n, self._qd, kv, "out")
         a.q_start = _index(q_start, torch.int32, (seqs + 1,), kv.device, "q_start")
         a.kv_len = _index(kv_len, torch.int32, (seqs,), kv.device, "kv_len")
-        a.page_table = _index(page_table, torch.int32, (seqs, page_table.shape[1]), kv.device, "page_table")
-        a.table_stride = page_table.shape[1]
+        a.table_stride = width = page_table.shape[1]
+        a.page_table = _index(page_table, torch.int32, (seqs, width), kv.device, "page_table")
         a.q, a.out, a.tokens, a.num_seqs, a.max_new = q.data_ptr(), out.data_ptr(), n, seqs, max_new
         ws, stream = self.workspace, _stream(kv.index)
         with ws.lock:         # no other call's launch between the kernels of this one
-            ws.on(stream)
-            rc = self._fn(kv._ref, C.byref(a), stream)
+            if stream != ws.handle:
+                ws.move(stream)
+            rc = self._fn(kv._ref, ref, stream)
         if rc:
             check(rc)
         return out
