@@ -125,6 +125,13 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// 2^x, one instruction (to 2 units in the last place).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Order-preserving float -> u32 key (larger float => larger key).
 __device__ __forceinline__ uint32_t float_key(float f) {
   uint32_t u = __float_as_uint(f);

@@ -30,19 +30,15 @@
 #include <math.h>
 
 #include <algorithm>
-#include <string>
 #include <type_traits>
 
-#include "../../include/nnz_b200.h"
 #include "common.cuh"
 #include "device_cache.cuh"
+#include "op_entry.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace nnz {
-
-void set_last_error(const std::string& msg);   // engine.cu
-int op_device(int** err, int* num_sms);
 
 namespace {
 
@@ -122,11 +118,6 @@ __device__ __forceinline__ K lp_merge32(K a, K b, int lane) {
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -486,14 +477,6 @@ cudaError_t logprobs_t(const LpArgs& a, int sms, cudaStream_t st) {
   return a.top_k ? logprobs_go<T, true>(a, sms, st) : logprobs_go<T, false>(a, sms, st);
 }
 
-int refuse(int code, const char* what) noexcept {
-  try {
-    set_last_error(what);
-  } catch (...) {
-  }
-  return code;
-}
-
 }  // namespace
 }  // namespace nnz
 
@@ -528,12 +511,5 @@ extern "C" int nnz_token_logprobs(const nnz_logprobs_args* p, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = p->dtype == NNZ_DT_F32 ? logprobs_t<float>(a, sms, st)
                       : p->dtype == NNZ_DT_F16 ? logprobs_t<__half>(a, sms, st) : logprobs_t<__nv_bfloat16>(a, sms, st);
-  if (e != cudaSuccess) {
-    try {
-      set_last_error(std::string("nnz_token_logprobs: ") + cudaGetErrorString(e));
-    } catch (...) {
-    }
-    return NNZ_ECUDA;
-  }
-  return NNZ_OK;
+  return cuda_rc(e, "nnz_token_logprobs");
 }

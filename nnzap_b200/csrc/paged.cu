@@ -4,17 +4,13 @@
 #include <math.h>
 
 #include <algorithm>
-#include <string>
 
-#include "../../include/nnz_b200.h"
+#include "op_entry.cuh"
 #include "paged_sched.cuh"
 #include "paged_tma.cuh"
 #include "rope_dev.cuh"
 
 namespace nnz {
-
-void set_last_error(const std::string& msg);      // engine.cu
-int op_device(int** err, int* num_sms);
 
 namespace {
 
@@ -401,24 +397,6 @@ cudaError_t paged_attn_any_launch(const PagedAttnArgs& a, int dtype, int hd, cud
 using namespace nnz;
 
 namespace {
-
-// No C++ exception crosses the C ABI: building the message can throw.
-int refuse(int code, const char* what) noexcept {
-  try {
-    set_last_error(what);
-  } catch (...) {
-  }
-  return code;
-}
-
-int cuda_rc(cudaError_t e, const char* who) noexcept {
-  if (e == cudaSuccess) return NNZ_OK;
-  try {
-    set_last_error(std::string(who) + ": " + cudaGetErrorString(e));
-  } catch (...) {
-  }
-  return NNZ_ECUDA;
-}
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

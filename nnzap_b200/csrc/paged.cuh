@@ -32,6 +32,13 @@ struct T16<__nv_bfloat16> {
   }
 };
 
+// Not 0: a non-finite element among the two (exponent all ones).
+template <bool BF16>
+__device__ __forceinline__ uint32_t bad_any(uint32_t w) {
+  constexpr uint32_t e = BF16 ? 0x7F807F80u : 0x7C007C00u, one = BF16 ? 0x00800080u : 0x04000400u;
+  return ((w & e) + one) & 0x80008000u;
+}
+
 // A page pool as the kernels see it (strides in elements).
 struct PagedPool {
   uint16_t* k;

@@ -100,11 +100,6 @@ __device__ __forceinline__ uint32_t st_off(int r, int ch) {
   return (uint32_t)((ch >> 3) * (kStKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ bool finite16(uint32_t w, bool bf16) {
-  const uint32_t e = bf16 ? 0x7F807F80u : 0x7C007C00u;
-  return (w & e & 0xFFFFu) != (e & 0xFFFFu) && (w & e & 0xFFFF0000u) != (e & 0xFFFF0000u);
-}
-
 // (m, l, o) of a row plus one more part of it; lane: HD / 32 dims.
 template <int HD>
 __device__ __forceinline__ void merge_part(float pm, float pl, const float* po, float& m, float& l, float (&o)[HD / 32]) {
@@ -394,7 +389,7 @@ __global__ void __launch_bounds__(kStWarps * 32, CL ? 1 : 0) paged_stream_kernel
             uint32_t w0, w1, w2, w3;
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(vb + st_off(lane, ch)) : "memory");
             constexpr bool bf = T16<T>::kBf16;
-            bad |= !(finite16(w0, bf) && finite16(w1, bf) && finite16(w2, bf) && finite16(w3, bf));
+            bad |= bad_any<bf>(w0) | bad_any<bf>(w1) | bad_any<bf>(w2) | bad_any<bf>(w3);
           }
         uint32_t rows = __ballot_sync(0xffffffffu, bad != 0);
         while (rows) {

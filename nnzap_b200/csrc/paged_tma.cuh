@@ -18,12 +18,6 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // x: dim (0 or 64), y: token within the page.
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tm, int x, int y, int head, int page, uint64_t* bar) {
   asm volatile(

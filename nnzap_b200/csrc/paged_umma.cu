@@ -284,13 +284,6 @@ __device__ __forceinline__ uint32_t bad_mask(uint32_t w) {
   return ((w & e) == e ? 0xFFFFu : 0u) | (((w >> 16) & e) == e ? 0xFFFF0000u : 0u);
 }
 
-// Not 0: a non-finite element among the two.
-template <bool BF16>
-__device__ __forceinline__ uint32_t bad_any(uint32_t w) {
-  constexpr uint32_t e = BF16 ? 0x7F807F80u : 0x7C007C00u, one = BF16 ? 0x00800080u : 0x04000400u;
-  return ((w & e) + one) & 0x80008000u;
-}
-
 // The part of one task in a CTA's run, as warp 16 hands it to the others.
 struct Segment {
   uint32_t take;       // units (0: the run is over)
