@@ -312,6 +312,7 @@ __device__ __forceinline__ void add_nonfinite(const PagedAttnArgs& a, const Segm
       if (key >= limit) continue;
       const uint32_t pi = (uint32_t)key / a.kv.page_size;
       const int pg = __ldg(a.page_table + (size_t)g.s * a.table_stride + pi);
+      if ((uint32_t)pg >= a.kv.num_pages) continue;      // (a mark of a tile that never landed, after a wait that gave up)
       const uint16_t* vp = a.kv.v + (int64_t)pg * a.kv.page_stride + (int64_t)g.kvh * a.kv.head_stride +
                            (int64_t)((uint32_t)key - pi * a.kv.page_size) * a.kv.token_stride + d0;
 #pragma unroll
@@ -381,8 +382,9 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
   // error is reported at the end (nothing but the poll stands in the loop).
   // Who gave up stops at its next part, all lanes of a warp and both warps of
   // a pair together, or those left would wait at barriers that have no bound; a
-  // part that is not finished with is not replaced, and copies and products
-  // under way are waited for, with new tries, before the CTA ends.
+  // part that is not finished with is not replaced, no tile is given back that
+  // may not have landed, and copies and products under way are waited for
+  // (`landed`) before the CTA ends.
   uint32_t tries = kUmTries;
   auto gave_up = [&] { return __any_sync(0xffffffffu, tries == 0) != 0; };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -391,6 +393,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         tries = 0;
         break;
       }
+  };
+
+  auto landed = [&](uint64_t* bar, uint32_t parity) {
+    for (uint32_t n = 0; n < kUmTries && !mbar_try_wait(bar, parity & 1u);) ++n;
   };
 
   // part k of the run; warp 17, and 0-15 likewise, take them in order from warp 16
@@ -556,12 +562,10 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
         ++unit_no;
       }
     }
-    if (gave_up()) {
-      tries = kUmTries;
-      for (uint32_t n = stage_use > (uint32_t)S::kStages ? stage_use - S::kStages : 0; n < stage_use; ++n) wait(kv_full + n % S::kStages, n / S::kStages);
-      if (q_use) wait(q_full, q_use - 1);
-      tries = 0;
-    }
+    // (whoever gave up may not have waited for them)
+#pragma unroll 1
+    for (uint32_t n = stage_use > (uint32_t)S::kStages ? stage_use - S::kStages : 0; n < stage_use; ++n) landed(kv_full + n % S::kStages, n / S::kStages);
+    if (q_use) landed(q_full, q_use - 1);
   } else if (warp == kWMma) {
     // ---------------- MMA ----------------
     constexpr uint32_t id_s = um_idesc<BF>(128, 128), id_o = um_idesc<BF>(128, HD) | (1u << 16);
@@ -637,23 +641,20 @@ __global__ void __launch_bounds__(kUmThreads, 1) paged_umma_kernel(const __grid_
           }
         }
         if (elect_one()) {
-          if (i > 0) umma_commit(kv_empty + vs);
-          if (i < take) umma_commit(kv_empty + ks);
-          if (i + 1 == take) umma_commit(q_empty);
+          if (i > 0 && tries) umma_commit(kv_empty + vs);
+          if (i < take && tries) umma_commit(kv_empty + ks);
+          if (i + 1 == take && tries) umma_commit(q_empty);
         }
         __syncwarp();
       }
       stage_use += 2 * take;
       segment_done(seg);
     }
+    if (stage_use) wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
     if (gave_up()) {
-      tries = kUmTries;
       if (elect_one()) umma_commit(drained);
       __syncwarp();
-      wait(drained, 0);
-      tries = 0;
-    } else if (stage_use) {
-      wait(kv_empty + (stage_use - 1) % S::kStages, (stage_use - 1) / S::kStages);   // the last arrival of a commit
+      landed(drained, 0);
     }
   }
   } else {
