@@ -367,8 +367,11 @@ size_t nnz_paged_attn_workspace(const nnz_paged_kv* kv, uint32_t num_query_heads
 
 /* Causal attention of every sequence's new tokens over its pages: new token
  * i of n attends to keys 0 .. kv_len - n + i that lie on present pages; a
- * token that sees no key gets zeros.  Scores, softmax and sums in f32 (the
- * probabilities enter the second product in the pool's dtype).  Rows of q
+ * token that sees no key gets zeros.  Scores, softmax and sums in f32; the
+ * probabilities enter the second product in the pool's dtype (f16: those
+ * below 2^-14 of the row's largest lose up to 2^-25 of it), whose f32 sums the
+ * tensor cores form with about 25 bits: keys that weigh less than 2^-25 of a
+ * row's sum each are lost.  Rows of q
  * outside every sequence are not read and their output is not written.  A
  * page number >= num_pages, a kv_len beyond table_stride pages, more new
  * tokens than max_new or a q_start outside [0, tokens] raises NNZ_EDEVICE in

@@ -36,8 +36,9 @@ __global__ void rope_table_kernel(double l2theta, uint32_t half, uint32_t positi
 // 8 lanes to a head, f32 arithmetic, one rounding.  One CTA of 4 warps per
 // token; a thread asks for all its chunks (up to kNrUnroll) before it waits
 // for the position, the table row that depends on it, or the slot, so a CTA
-// pays two memory latencies and the 8 CTAs of an SM keep 128 KB in flight.
-// Measured (16 / 8 heads of 128): 8191 tokens 29.4 us, 4.7 TB/s; 512 tokens 4.0
+// pays two memory latencies and the 8 CTAs of an SM keep 64 KB in flight.
+// Measured (16 / 8 heads of 128): 8191 tokens 29.4 us, 4.7 TB/s (memory is the
+// first reason of stalls, and 2.6 of 4 instructions a cycle issue); 512 tokens 4.0
 // us, 1 token 2.45 us, which is the launch and those two latencies.
 // A lane holds four pairs of a head whole: 8 elements in a row (pairwise), or 4
 // of each half (half split: two 8-byte chunks; with 16-byte chunks the pairs

@@ -13,6 +13,11 @@
 // unit, and 8 rings of 24 KB keep 190 KB of an SM's memory in flight.  S = Q K^T and
 // O += P V are mma.m16n8k16 with the G heads of every new token as rows; the
 // online softmax keeps its f32 maximum and sum in the score fragments' lanes.
+// P enters the second product in the pool's type, the only one that the tensor
+// cores multiply with V as it is stored (the sum is of P before it is rounded):
+// half a unit in its last place in every weight, as much again as the result's
+// own rounding at the most.  (The remainder of P as a second operand would take
+// that away, and make NaN of an infinite V, by 0 times infinity.)
 // The ring runs ahead across task boundaries.  Page numbers are read 32
 // copies ahead, one per lane.
 //
@@ -20,9 +25,12 @@
 // scores are masked, their V rows zeroed in shared memory.
 //
 // Measured (16 / 8 heads of 128, f16): 64 single tokens over 2017 .. 4032 keys
-// 135 us, 5.9 TB/s of K and V, 0.9 of a plain copy's rate; one token
-// over 32767 keys (bf16) 30 us, 4.5 TB/s, and over 515 keys 6.4 us, which is
-// the launch, two dependent loads, four units and the merge over the cluster.
+// 135 - 141 us by the board, 5.6 - 5.9 TB/s of K and V, 0.87 - 0.9 of a plain
+// copy's rate; one token over 32767 keys (bf16) 30.7 us, 4.4 TB/s, and over 515
+// keys 6.5 us, which is the launch, two dependent loads, four units and the merge
+// over the cluster.  Farther from the bytes' time: 64 tokens with 8 / 2 heads of
+// 64 35 us (15), 32 sequences of 4 or 8 new tokens over 1000 .. 4000 keys 74 and 86
+// us (50).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>

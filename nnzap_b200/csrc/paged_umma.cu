@@ -40,8 +40,10 @@
 // pages and past the length are loaded from beyond the pool's last page: the
 // copy engine fills them with zeros, so no stale byte meets the product.
 //
-// Measured (16 / 8 heads of 128): 4096 tokens behind 4096 keys 213 us, 965
-// TFLOP/s of the visible pairs' products; 512 behind 4096 35 - 36 us.  A unit
+// Measured (16 / 8 heads of 128): 4096 tokens behind 4096 keys 214 us, 960
+// TFLOP/s of the visible pairs' products; 512 behind 4096 36.7 us.  Over the 4096
+// tokens the tensor pipe is busy 56 % of the time and the special-function units
+// 57 %; neither is the limit, the order between them is.  A unit
 // takes a CTA about 3900 cycles, its four products 2100 to 2800 of them: S, the
 // softmax, P V and the next S of a row tile follow one another, TMEM is full
 // with one S and one O of each, and the special-function units alone need 2048
