@@ -202,6 +202,13 @@ __global__ void take_errors_kernel(int* a, int* b, int* c) {
   g_taken_err = flags;
 }
 
+// Loads that kernel on the current device: a kernel's first launch would need
+// device memory for its code.
+cudaError_t stream_check_prepare() {
+  cudaFuncAttributes a;
+  return cudaFuncGetAttributes(&a, take_errors_kernel);
+}
+
 int op_device(int** err, int* num_sms) {
   constexpr int kMaxDevices = 64;
   struct Dev { std::atomic<int*> err{nullptr}; int sms = 0; };
@@ -216,6 +223,7 @@ int op_device(int** err, int* num_sms) {
     std::lock_guard<std::mutex> lk(mu);
     NNZ_CK(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
     NNZ_CK(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_op_err));
+    NNZ_CK(stream_check_prepare());
     d.err.store(p, std::memory_order_release);
   }
   *err = p;

@@ -17,7 +17,8 @@
 //    streams, or different host threads on one device) race -- serialise
 //    them on one stream;
 //  * the first call on a device resolves the arrays' device addresses,
-//    clears the error word and raises the kernels' shared-memory limit:
+//    clears the error word, loads the kernel of nnz_stream_check and raises
+//    the kernels' shared-memory limit:
 //    make that first call before any stream capture starts on the device;
 //  * a bounded wait that gives up inside the kernel sets the error word;
 //    nnz_stream_check() reads and clears it (the call itself returns as
@@ -33,6 +34,7 @@
 
 namespace nnz {
 void set_last_error(const std::string& msg);   // nnz_last_error() text (engine.cu)
+cudaError_t stream_check_prepare();            // engine.cu
 
 namespace {
 
@@ -70,6 +72,7 @@ int setup(int dev, NoAllocDev** out) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.num_sms, cudaDevAttrMultiProcessorCount, dev);
     if (e == cudaSuccess) e = cudaMemset(d.err, 0, sizeof(int));
     if (e == cudaSuccess) e = qmv_prepare();
+    if (e == cudaSuccess) e = stream_check_prepare();
     if (e != cudaSuccess) {
       set_last_error(std::string("nnz_qmv_noalloc set-up: ") + cudaGetErrorString(e));
       return NNZ_ECUDA;

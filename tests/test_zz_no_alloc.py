@@ -75,3 +75,28 @@ def test_noalloc_rejects_oversized_scratch(cuda, built_lib):
     assert rc == _capi.NNZ_EINVAL
     err = lib().nnz_last_error()
     assert b"fixed limits" in err and b"split-K scratch" in err
+
+
+def test_stream_check_takes_no_device_memory(cuda, built_lib):
+    """In a fresh process, after a first nnz_qmv_noalloc: checks leave the free
+    device memory as it was."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import numpy as np, torch
+from gpu_helpers import check, lib, pack, ptr, to_dev
+from nnzap_b200 import synth
+t = synth.rand_q1(np.random.default_rng(0), 128, 256, 128)
+w, x, y = to_dev(torch, pack(0, t, 128, 256, 128)), torch.zeros(256, dtype=torch.float16, device="cuda"), torch.zeros(128, device="cuda")
+check(lib().nnz_qmv_noalloc(0, 0, 0, ptr(w), 128, 256, 128, ptr(x), 256, 1, ptr(y), 128, 1, None))
+torch.cuda.synchronize()
+free = torch.cuda.mem_get_info()[0]
+for _ in range(3):
+    check(lib().nnz_stream_check(None))
+    assert torch.cuda.mem_get_info()[0] == free
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=Path(__file__).resolve().parent,
+                       env={**__import__("os").environ, "PYTHONPATH": str(Path(__file__).resolve().parent.parent)})
+    assert r.stdout.strip() == "same", r.stdout + r.stderr
