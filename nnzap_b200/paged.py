@@ -12,10 +12,10 @@ nnmetal/src/transformer.zig:648-700, and prefills token by token, :4032-4068):
 
 Every call is asynchronous on torch's current stream of the tensors' device
 (which need not be the current device); errors found on the device (a page,
-slot or token out of range) are reported by :func:`stream_check`.  Tensors that a call
-uses must stay alive until its stream has run it, as with any torch operation
-(``record_stream`` them if they were allocated on another stream).  The math
-runs in the CUDA library; this module checks and marshals arguments.
+slot or token out of range) are reported by :func:`stream_check`.  Tensors that
+a call uses must stay alive until its stream has run it, as with any torch
+operation (``record_stream`` them if they were allocated on another stream).
+The math runs in the CUDA library; this module checks and marshals arguments.
 """
 from __future__ import annotations
 
@@ -178,9 +178,10 @@ class PagedAttention:
     ``q`` holds the new tokens of all sequences one after the other; sequence
     s has rows ``q_start[s]:q_start[s + 1]`` and ``kv_len[s]`` keys, its new
     tokens' included, on the pages ``page_table[s]`` (negative: absent).
-    ``max_new`` is a host-known upper bound of one sequence's new tokens.
-    ``scale`` is positive (None: 1 / sqrt(head_dim)).  The
-    object's ``workspace`` serves one call at a time: threads may share the
+    ``max_new`` is a host-known upper bound of one sequence's new tokens,
+    ``scale`` positive (None: 1 / sqrt(head_dim)).
+
+    The object's ``workspace`` serves one call at a time: threads may share the
     object, and a call on another stream waits for the one before.  Operators
     whose calls follow one another (a model's layers) can have one workspace:
     pass the first one's as ``workspace``."""
